@@ -9,8 +9,12 @@ from .encoder import (ViT_stage1, ViT_stage2, ViT3DTower_dual_encoders, regular_
                       build_vision_tower, PatchEmbeddingBlock, TransformerBlock)
 from .projector import (VisualPacker_3d_phi_v3, resolution_attention_v3, build_mm_projector, encode_images, LamedMetaForCausalLM)  # noqa: F401
 from .clip import encode_image_cls, image_text_contrastive_learning  # noqa: F401
+from .rotary import RotaryAxes, rotary_axes  # noqa: F401
+from .diff_attn import diff_attention  # noqa: F401
+from .optim import AdamW  # noqa: F401
 
-__all__ = ["ViT_stage1", "ViT_stage2", "ViT3DTower_dual_encoders", "regular_attention", "build_vision_tower",
+__all__ = ["RotaryAxes", "rotary_axes", "diff_attention", "AdamW",
+           "ViT_stage1", "ViT_stage2", "ViT3DTower_dual_encoders", "regular_attention", "build_vision_tower",
            "VisualPacker_3d_phi_v3", "resolution_attention_v3", "build_mm_projector", "encode_images", "LamedMetaForCausalLM",
            "encode_image_cls", "image_text_contrastive_learning", "set_precision", "get_precision", "invalidate_weight_copies"]
 from .trunk2d import BiomedClipTrunk, slice_features  # noqa: F401,E402

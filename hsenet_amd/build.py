@@ -22,6 +22,13 @@ EXTRA = {"attn.hip": ["-fno-slp-vectorize", "-mllvm", "-amdgpu-mfma-vgpr-form"],
          # prep.hip: the reference applies scale and shift (and torch its interpolation taps) as separate roundings
          "prep.hip": ["-ffp-contract=off"]}
 
+# the operators beside the encoder path: a library of their own, so that the encoder library's content hash -- which the committed counters
+# carry -- does not move when an operator does.  Packed fp32 instructions are off here: some of their forms have given wrong results now and then.
+OPS_LIB = os.path.join(LIBDIR, "libhsenet_ops.so")
+OPS_SOURCES = ["ops/rotary.hip", "ops/diff_attn.hip", "ops/adamw.hip", "ops/ops.hip"]
+OPS_FLAGS = FLAGS + ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-Wno-unknown-warning-option"]
+OPS_EXTRA = {}
+
 
 def _hipcc() -> str:
     exe = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
@@ -51,6 +58,19 @@ def source_id(src: str = None) -> str:
     return h.hexdigest()[:16]
 
 
+def ops_source_id(src: str = None) -> str:
+    """source_id() of the operators' library."""
+    h = hashlib.sha256()
+    for n in [src] if src else OPS_SOURCES:
+        h.update(n.encode())
+        h.update(open(os.path.join(CSRC, n), "rb").read())
+        h.update(" ".join(OPS_FLAGS + OPS_EXTRA.get(n, [])).encode())
+    for f in _hdrs() + [os.path.join(os.path.dirname(HERE), "include", "hsenet_ops.h")]:
+        h.update(open(f, "rb").read())
+    h.update(_toolchain_id().encode())
+    return h.hexdigest()[:16]
+
+
 def _toolchain_id() -> str:
     """the compiler's identity without running it (this is hashed on every library load): the ROCm release stamp of the toolchain
     hipcc belongs to; an object built by another ROCm release is stale."""
@@ -71,15 +91,21 @@ def _read(path: str) -> str:
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
+    """both libraries; the encoder library's path."""
+    _build_lib(OPS_LIB, OPS_SOURCES, OPS_FLAGS, OPS_EXTRA, ops_source_id, "hs_ops_build_id", force, verbose)
+    return _build_lib(LIB, SOURCES, FLAGS, EXTRA, source_id, "hs_build_id", force, verbose)
+
+
+def _build_lib(lib, sources, flags, extra, source_id, id_symbol, force, verbose) -> str:
     os.makedirs(LIBDIR, exist_ok=True)
     hipcc = _hipcc()
     objs, jobs, stamps = [], [], []
-    for s in SOURCES:
-        src, obj = os.path.join(CSRC, s), os.path.join(LIBDIR, s.replace(".hip", ".o"))
+    for s in sources:
+        src, obj = os.path.join(CSRC, s), os.path.join(LIBDIR, s.replace("/", "_").replace(".hip", ".o"))
         objs.append(obj)
         sid, tag = source_id(s), obj + ".id"
         if force or not os.path.exists(obj) or _read(tag) != sid:
-            jobs.append([hipcc, *FLAGS, *EXTRA.get(s, []), "-c", src, "-o", obj])
+            jobs.append([hipcc, *flags, *extra.get(s, []), "-c", src, "-o", obj])
             stamps.append((tag, sid))
 
     def run(cmd):
@@ -96,13 +122,14 @@ def build(force: bool = False, verbose: bool = False) -> str:
             open(tag, "w").write(sid)
     # the build id: always regenerated and compiled (a few hundred ms) — every build() call runs hipcc at least once
     lid = source_id()
-    idc, ido = os.path.join(LIBDIR, "build_id.cpp"), os.path.join(LIBDIR, "build_id.o")
-    open(idc, "w").write(f'extern "C" const char* hs_build_id(void) {{ return "{lid}"; }}\n')
+    stem = os.path.join(LIBDIR, id_symbol[3:])
+    idc, ido = stem + ".cpp", stem + ".o"
+    open(idc, "w").write(f'extern "C" const char* {id_symbol}(void) {{ return "{lid}"; }}\n')
     run([hipcc, "-O1", "-fPIC", "-c", idc, "-o", ido])
-    if jobs or force or not os.path.exists(LIB) or _read(LIB + ".id") != lid:
-        run([hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB, *objs, ido])
-        open(LIB + ".id", "w").write(lid)
-    return LIB
+    if jobs or force or not os.path.exists(lib) or _read(lib + ".id") != lid:
+        run([hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", lib, *objs, ido])
+        open(lib + ".id", "w").write(lid)
+    return lib
 
 
 if __name__ == "__main__":

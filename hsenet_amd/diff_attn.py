@@ -1,0 +1,123 @@
+"""Differential attention (``hs_diff_attn_fwd`` / ``hs_diff_attn_bwd``): softmax(q1 k1^T) v - lam softmax(q2 k2^T) v, the difference of two softmax
+maps with a learned weight."""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib as L
+from . import _ops as O
+
+
+def _per_entry(t, what, B):
+    if t is not None and (not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or tuple(t.shape) != (B,) or not t.is_contiguous()):
+        raise L.HsError(f"{what} must be a dense int32 tensor of one number per batch entry ({B})")
+
+
+def _prepare(q, k, v, lam, scale, causal, q_start, kv_len):
+    """(descriptor, q, k, v, lam) with the operands where the kernels can read them; HsError for what they cannot take"""
+    for t, name in ((q, "q"), (k, "k"), (v, "v")):
+        if t.dim() != 4:
+            raise L.HsError(f"{name} must have 4 axes: [B, tokens, heads, columns]")
+    if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise L.HsError("q, k and v must all be bf16 or all fp16")
+    B, Nq, H2, d = q.shape
+    Nk, Hk2 = k.shape[1:3]
+    H, Hkv = H2 // 2, Hk2 // 2
+    if H2 % 2 or Hk2 % 2 or H < 1 or Hkv < 1 or H % Hkv:
+        raise L.HsError(f"q needs 2 H heads and k 2 Hkv, H a multiple of Hkv: got {H2} and {Hk2}")
+    if d not in (32, 64, 128):
+        raise L.HsError(f"heads of 32, 64 or 128 columns, got {d}")
+    if tuple(k.shape) != (B, Nk, Hk2, d) or tuple(v.shape) != (B, Nk, Hkv, 2 * d):
+        raise L.HsError(f"for q {tuple(q.shape)} and k {tuple(k.shape)} v must be {(B, Nk, Hkv, 2 * d)}, got {tuple(v.shape)}")
+    if lam.dtype != torch.float32 or not (lam.numel() == 1 or tuple(lam.shape) == (H,)):
+        raise L.HsError(f"lam must be fp32, one number or one per head ({H},), got {lam.dtype} {tuple(lam.shape)}")
+    _per_entry(q_start, "q_start", B)
+    _per_entry(kv_len, "kv_len", B)
+    scale = d ** -0.5 if scale is None else float(scale)
+    if not 0 < scale < 1e6:
+        raise L.HsError(f"scale must be positive (below 1e6), got {scale}")
+    q, k, v = (t if O.rows_of_heads(t, 8) else t.contiguous() for t in (q, k, v))
+    desc = O.DiffAttnDesc(B, Nq, Nk, H, Hkv, d, O.DTYPE[q.dtype], int(causal), Nk - Nq)
+    lam = lam.contiguous()
+    desc.lam_stride, desc.scale = int(lam.dim() == 1 and H > 1 and lam.numel() > 1), scale
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        for s, n in zip("bnh", O.bnh(t)):
+            setattr(desc, f"{name}_{s}", n)
+    return desc, q, k, v, lam
+
+
+def _forward(q, k, v, lam, scale, causal, q_start, kv_len, keep):
+    """-> (o, and for a backward pass the operands as they were read, the maps' outputs and statistics)"""
+    with O.on_device(q, k, v, lam, q_start, kv_len):
+        desc, q, k, v, lam = _prepare(q, k, v, lam, scale, causal, q_start, kv_len)
+        B, Nq, H, d = desc.B, desc.Nq, desc.H, desc.d
+        o = torch.empty(B, Nq, H, 2 * d, dtype=q.dtype, device=q.device)
+        maps = torch.empty(2, B, Nq, H, 2 * d, dtype=q.dtype, device=q.device) if keep else None
+        lse = torch.empty(B, H, 4, Nq, dtype=torch.float32, device=q.device) if keep else None
+        if o.numel():
+            if desc.Nk == 0:
+                o.zero_()
+            else:
+                n = O.load().hs_diff_attn_fwd_ws_bytes(C.byref(desc))
+                ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
+                O.call("hs_diff_attn_fwd", C.byref(desc), q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), _ptr(q_start), _ptr(kv_len),
+                       o.data_ptr(), _ptr(maps), _ptr(lse), _ptr(ws), n, O.stream())
+    return o, desc, q, k, v, lam, maps, lse
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+class DiffAttnFn(torch.autograd.Function):
+    """differential attention and its gradient (q, k, v and lam)."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, lam, scale, causal, q_start, kv_len):
+        o, desc, q, k, v, lam, maps, lse = _forward(q, k, v, lam, scale, causal, q_start, kv_len, True)
+        ctx.save_for_backward(q, k, v, lam, q_start, kv_len, maps, lse)
+        ctx.desc = desc
+        return o
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, go):
+        q, k, v, lam, q_start, kv_len, maps, lse = ctx.saved_tensors
+        with O.on_device(q, go):
+            go = go if O.rows_of_heads(go, 8) else go.contiguous()
+            dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+            dlam = torch.empty(lam.shape, dtype=torch.float32, device=q.device)
+            if q.numel() == 0 or k.numel() == 0:
+                return (*(t.zero_() for t in (dq, dk, dv, dlam)), None, None, None, None)
+            desc = O.DiffAttnDesc.from_buffer_copy(ctx.desc)          # (the graph may be run backward from several threads, or again)
+            for s, n in zip("bnh", O.bnh(go)):
+                setattr(desc, f"go_{s}", n)
+            n = O.load().hs_diff_attn_bwd_ws_bytes(C.byref(desc))
+            ws = torch.empty(n, dtype=torch.uint8, device=q.device)
+            O.call("hs_diff_attn_bwd", C.byref(desc), q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), _ptr(q_start), _ptr(kv_len), go.data_ptr(),
+                   maps.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dlam.data_ptr(), ws.data_ptr(), n, O.stream())
+        return dq, dk, dv, dlam, None, None, None, None
+
+
+def diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch.Tensor, *, scale: Optional[float] = None, causal: bool = False,
+                   q_start: Optional[torch.Tensor] = None, kv_len: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """o [B, Nq, H, 2 d] = softmax(scale q1 k1^T) v - lam softmax(scale q2 k2^T) v.
+
+    q [B, Nq, 2 H, d]: heads 2 h and 2 h + 1 are the two queries of head h; k [B, Nk, 2 Hkv, d] likewise; v [B, Nk, Hkv, 2 d]; head h reads key head
+    h // (H / Hkv).  bf16 or fp16, d 32, 64 or 128; views with their columns side by side and strides of multiples of 8 elements are read where they lie
+    (a cache longer than its tokens, the thirds of one projection), others are copied first.  lam: fp32, one number or [H].  scale: d^-0.5.
+
+    kv_len (int32 [B]): the keys of each entry that count (its first; 0 to Nk); what k and v hold behind them is not used.
+    causal: query i of entry b sees the keys j <= q_start[b] + i.  q_start (int32 [B]) is the position of an entry's first query: without it,
+    Nk - Nq (the queries are the last tokens).  A query that sees no key gets zeros, and nothing flows back from it.
+
+    Differentiable in q, k, v and lam, without atomics (equal inputs, equal bits); the maps' own outputs are kept for it.  A few queries against many
+    keys (a token and its cache) are split over the keys.  In fp16 a backward pass holds P (dP - D) times 16: scale the loss so that the gradients
+    of a layer stay in fp16's range."""
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (q, k, v, lam)):
+        return DiffAttnFn.apply(q, k, v, lam, scale, causal, q_start, kv_len)
+    return _forward(q, k, v, lam, scale, causal, q_start, kv_len, False)[0]

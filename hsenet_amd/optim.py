@@ -1,0 +1,212 @@
+"""AdamW over many tensors at once, moments in 32 or 8 bits (``hs_adamw_multi``): the optimizer for a module's own parameters, where the engines'
+``hs_adamw_fused`` wants one flat fp32 buffer."""
+from __future__ import annotations
+
+from array import array
+from typing import List, Optional, Sequence, Tuple
+
+import torch
+
+from . import _lib as L
+from . import _ops as O
+
+_BYTES = {8: (torch.int8, torch.uint8), 32: (torch.float32, torch.float32)}
+
+
+def _dense(t: torch.Tensor) -> bool:
+    """whether t's elements fill one stretch of memory, in whatever order of its axes"""
+    if t.is_contiguous():
+        return True
+    want = 1
+    for s, n in sorted((s, n) for n, s in zip(t.shape, t.stride()) if n > 1):
+        if s != want:
+            return False
+        want *= n
+    return True
+
+
+class AdamW(torch.optim.Optimizer):
+    """p *= 1 - lr * weight_decay; m, v the moments of the gradient; p -= lr m^ / (sqrt(v^) + eps), with all tensors of a group in a launch per 56.
+
+    Parameters: bf16, fp16 or fp32 (arithmetic in fp32, one rounding at the end), dense in any order of their axes, gradients of the same type.
+    state_bits 32: moments in fp32.  state_bits 8: int8 and uint8 codes with an fp32 scale per 256 elements of a tensor, in its order in memory
+    (include/hsenet_ops.h has the formula): 2.03 bytes an element instead of 8.  The step is taken with the new moments before they are rounded.
+    A gradient that is not finite makes its element, and with 8 bits its block's moments, NaN: skip such a step, as torch.amp.GradScaler does.
+
+    state[p]: ``step`` (int32 [4] on the device: the count and scratch), ``exp_avg``, ``exp_avg_sq`` and, with 8 bits, ``exp_avg_scale`` and
+    ``exp_avg_sq_scale``.  The count lives on the device, so a step can be captured into a graph (its lr, betas, eps and weight_decay as they were at
+    the capture).  A parameter without a gradient is left out of a step."""
+
+    def __init__(self, params, lr: float = 1e-3, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2,
+                 state_bits: int = 32):
+        if state_bits not in (8, 32):
+            raise ValueError("state_bits must be 8 or 32")
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits))
+
+    def add_param_group(self, group) -> None:
+        super().add_param_group(group)
+        g = self.param_groups[-1]
+        try:
+            self._check_numbers(g)
+            if g["state_bits"] not in (8, 32):
+                raise ValueError("state_bits must be 8 or 32")
+            for p in g["params"]:
+                if p.dtype not in O.DTYPE:
+                    raise ValueError(f"parameters must be bf16, fp16 or fp32, got {p.dtype}")
+        except ValueError:
+            self.param_groups.pop()
+            raise
+
+    @staticmethod
+    def _check_numbers(g) -> Tuple[float, float, float, float, float]:
+        lr, (b1, b2), eps, wd = g["lr"], g["betas"], g["eps"], g["weight_decay"]
+        if isinstance(lr, torch.Tensor):
+            raise ValueError("lr must be a number, not a tensor")
+        if not lr >= 0 or not 0 <= b1 < 1 or not 0 <= b2 < 1 or not eps >= 0 or not wd >= 0:
+            raise ValueError(f"bad lr, betas, eps or weight_decay: {lr}, {(b1, b2)}, {eps}, {wd}")
+        return float(lr), float(b1), float(b2), float(eps), float(wd)
+
+    def _bits(self, p) -> int:
+        return next(g["state_bits"] for g in self.param_groups if any(q is p for q in g["params"]))
+
+    def set_state(self, p: torch.Tensor, *, step: int, exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor, exp_avg_scale: Optional[torch.Tensor] = None,
+                  exp_avg_sq_scale: Optional[torch.Tensor] = None) -> None:
+        """takes the given tensors as p's state (they are updated in place from now on): of p's shape and memory order, scales [ceil(n / 256)]"""
+        bits, new = self._bits(p), {"exp_avg": exp_avg, "exp_avg_sq": exp_avg_sq}
+        if bits == 8:
+            new.update(exp_avg_scale=exp_avg_scale, exp_avg_sq_scale=exp_avg_sq_scale)
+        elif exp_avg_scale is not None or exp_avg_sq_scale is not None:
+            raise L.HsError("32-bit moments have no scales")
+        rec = torch.zeros(4, dtype=torch.int32)
+        rec[0] = int(step)
+        self._check_state(p, {"step": rec.to(p.device), **new}, bits)
+        self.state[p] = {"step": rec.to(p.device), **new}
+
+    @staticmethod
+    def _check_state(p, st, bits) -> None:
+        dm, dv = _BYTES[bits]
+        for name, dt in (("exp_avg", dm), ("exp_avg_sq", dv)):
+            t = st.get(name)
+            if not isinstance(t, torch.Tensor) or t.dtype != dt or t.shape != p.shape or t.device != p.device or (t.stride() != p.stride() and p.numel() > 1):
+                raise L.HsError(f"{name} must be a {dt} tensor of its parameter's shape, strides and device")
+        if bits == 8:
+            n = -(-p.numel() // O.ADAMW_BLOCK)
+            for name in ("exp_avg_scale", "exp_avg_sq_scale"):
+                t = st.get(name)
+                if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or tuple(t.shape) != (n,) or t.device != p.device or not t.is_contiguous():
+                    raise L.HsError(f"{name} must be a dense fp32 tensor ({n},) on its parameter's device")
+        t = st.get("step")
+        if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or tuple(t.shape) != (4,) or t.device != p.device or not t.is_contiguous():
+            raise L.HsError("step must be a dense int32 tensor (4,) on its parameter's device")
+
+    def _init_state(self, p, bits) -> dict:
+        if torch.cuda.is_current_stream_capturing():
+            raise L.HsError("the first step makes the states: take it before a graph is captured")
+        dm, dv = _BYTES[bits]
+        st = {"step": torch.zeros(4, dtype=torch.int32, device=p.device), "exp_avg": torch.zeros_like(p, dtype=dm),
+              "exp_avg_sq": torch.zeros_like(p, dtype=dv)}
+        if bits == 8:
+            n = -(-p.numel() // O.ADAMW_BLOCK)
+            st.update(exp_avg_scale=torch.zeros(n, dtype=torch.float32, device=p.device), exp_avg_sq_scale=torch.zeros(n, dtype=torch.float32, device=p.device))
+        self._check_state(p, st, bits)
+        self.state[p] = st
+        return st
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            numbers, bits = self._check_numbers(group), group["state_bits"]
+            tables = {}                                        # (device, type) -> entries
+            changed = []
+            for p in group["params"]:
+                g = p.grad
+                if g is None:
+                    continue
+                if not p.is_cuda:
+                    raise L.HsError("hsenet_amd kernels need tensors on an MI355X ('cuda') device; there is no CPU fallback")
+                if g.is_sparse or g.dtype != p.dtype or g.device != p.device:
+                    raise L.HsError("a gradient must be dense, of its parameter's type and on its device")
+                st = self.state.get(p) or self._init_state(p, bits)
+                stride = p.stride()
+                if not p.is_contiguous() and not _dense(p):
+                    raise L.HsError("a parameter's elements must fill one stretch of memory")
+                if g.stride() != stride:
+                    g = torch.empty_like(p).copy_(g)
+                m, v = st["exp_avg"], st["exp_avg_sq"]
+                if m.stride() != stride or v.stride() != stride:
+                    self._check_state(p, st, bits)
+                key = (p.get_device(), p.dtype)
+                t = tables.get(key)
+                if t is None:
+                    t = tables[key] = (array("q"), [])
+                if bits == 8:
+                    t[0].extend((p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), st["exp_avg_scale"].data_ptr(),
+                                 st["exp_avg_sq_scale"].data_ptr(), st["step"].data_ptr(), p.numel()))
+                else:
+                    t[0].extend((p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), 0, 0, st["step"].data_ptr(), p.numel()))
+                t[1].append(g)                                 # (a gradient that was copied lives until the launch)
+                changed.append(p)
+            for (dev, dtype), (words, _) in tables.items():
+                with torch.cuda.device(dev):
+                    O.call("hs_adamw_multi", words.buffer_info()[0], len(words) // 8, O.DTYPE[dtype], bits, *numbers, O.stream())
+            if changed:
+                torch.autograd.graph.increment_version(changed)
+        return loss
+
+    @torch.no_grad()
+    def read_moments(self, exp_avg: Sequence[torch.Tensor], exp_avg_sq: Sequence[torch.Tensor]) -> None:
+        """writes the moments of every parameter (in the groups' order) into the given dense tensors of its shape and strides, all bf16 or all fp32: the
+        values that 8-bit codes stand for, or a copy of 32-bit moments.  A parameter that has no state yet has moments of 0."""
+        ps = [(p, g["state_bits"]) for g in self.param_groups for p in g["params"]]
+        if len(exp_avg) != len(ps) or len(exp_avg_sq) != len(ps):
+            raise L.HsError(f"one pair of tensors per parameter expected ({len(ps)})")
+        tables = {}
+        for (p, bits), m, v in zip(ps, exp_avg, exp_avg_sq):
+            for t in (m, v):
+                if t.dtype not in (torch.float32, torch.bfloat16) or t.shape != p.shape or t.device != p.device or t.dtype != exp_avg[0].dtype \
+                        or (t.stride() != p.stride() and p.numel() > 1):
+                    raise L.HsError("moments go into bf16 or fp32 tensors of their parameter's shape, strides and device")
+            st = self.state.get(p)
+            if not st:
+                m.zero_()
+                v.zero_()
+            elif bits == 32:
+                m.copy_(st["exp_avg"])
+                v.copy_(st["exp_avg_sq"])
+            else:
+                tables.setdefault(p.get_device(), array("q")).extend(
+                    (m.data_ptr(), v.data_ptr(), st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr(), st["exp_avg_scale"].data_ptr(),
+                     st["exp_avg_sq_scale"].data_ptr(), st["step"].data_ptr(), p.numel()))
+        for dev, words in tables.items():
+            with torch.cuda.device(dev):
+                O.call("hs_adamw_moments", words.buffer_info()[0], len(words) // 8, O.DTYPE[exp_avg[0].dtype], O.stream())
+
+    def moments(self, p: torch.Tensor, dtype: torch.dtype = torch.float32) -> Tuple[torch.Tensor, torch.Tensor]:
+        """the moments (m, v) of one parameter in fp32 or bf16, whatever they are held in"""
+        m, v = torch.empty_like(p, dtype=dtype, requires_grad=False), torch.empty_like(p, dtype=dtype, requires_grad=False)
+        one = AdamW.__new__(AdamW)
+        one.param_groups, one.state = [{"params": [p], "state_bits": self._bits(p)}], {p: self.state.get(p)}
+        AdamW.read_moments(one, [m], [v])
+        return m, v
+
+    def load_state_dict(self, state_dict) -> None:
+        """as torch's, but codes and scales keep their types (torch casts a floating parameter's state to the parameter's type)"""
+        super().load_state_dict(state_dict)
+        saved: List = [i for g in state_dict["param_groups"] for i in g["params"]]
+        for i, (p, bits) in zip(saved, [(p, g["state_bits"]) for g in self.param_groups for p in g["params"]]):
+            st = state_dict["state"].get(i)
+            if st is None:
+                continue
+            new = {}
+            for k, t in st.items():
+                if k in ("exp_avg", "exp_avg_sq"):
+                    t = torch.empty_like(p, dtype=t.dtype, requires_grad=False).copy_(t)
+                elif isinstance(t, torch.Tensor):
+                    t = t.detach().to(p.device, copy=True).contiguous()
+                new[k] = t
+            self._check_state(p, new, bits)
+            self.state[p] = new

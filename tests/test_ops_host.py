@@ -1,0 +1,137 @@
+"""The operators' library without a GPU: what it exports is what its header declares, bad arguments are refused before anything could be launched
+(the pointers here are fakes that are never read), and the Python entry points refuse what the kernels cannot take."""
+import ctypes as C
+import os
+import re
+import subprocess
+
+import pytest
+import torch
+
+import hsenet_amd as H
+from hsenet_amd import _lib as L
+from hsenet_amd import _ops as O
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+P = 0x10000
+no_gpu_only = pytest.mark.skipif(torch.cuda.is_available(), reason="fake pointers: only where nothing can be launched")
+
+
+def test_library_header_and_binding_agree():
+    from hsenet_amd.build import OPS_LIB, build
+    build()
+    src = re.sub(r"/\*.*?\*/", "", open(os.path.join(ROOT, "include", "hsenet_ops.h")).read(), flags=re.S)
+    names = sorted(set(re.findall(r"\b(hs_[a-z0-9_]+)\s*\(", src)))
+    out = subprocess.run(["nm", "-D", "--defined-only", OPS_LIB], capture_output=True, text=True, check=True).stdout
+    assert names == sorted(set(re.findall(r" T (hs_[a-z0-9_]+)", out))) == sorted(O.SIGNATURES)
+    assert O.load().hs_ops_version() == O.ABI_VERSION and O.check_fresh() == O.load().hs_ops_build_id().decode()
+    assert b"gfx950" in open(OPS_LIB, "rb").read()
+
+
+@pytest.mark.parametrize("name", sorted(n for n in O.SIGNATURES if n not in ("hs_ops_version", "hs_ops_build_id")))
+def test_null_arguments_are_refused(name):
+    args = [None if a is C.c_void_p or hasattr(a, "contents") else a(0) for a in O.SIGNATURES[name]]
+    rc = getattr(O.load(), name)(*args)
+    assert rc == 0 if name.endswith("_ws_bytes") else rc in (L.HS_ERR_ARG, L.HS_ERR_SHAPE)
+
+
+def _rot(**kw):
+    d = O.RotaryDesc(2, 3, 64, 32, 3)
+    d.heads[0], d.heads[1] = 4, 2
+    for i in range(2):
+        d.x_b[i], d.x_n[i], d.x_h[i] = 3 * 4 * 64, 4 * 64, 64
+        d.y_b[i], d.y_n[i], d.y_h[i] = 3 * 4 * 64, 4 * 64, 64
+    for k, v in kw.items():
+        if k == "heads1":
+            d.heads[1] = v
+        else:
+            setattr(d, k, v)
+    return d
+
+
+@no_gpu_only
+@pytest.mark.parametrize("kw,want", [(dict(B=0), "s"), (dict(N=0), "s"), (dict(pairs=0), "s"), (dict(pairs=33), "s"), (dict(pairs=600, dh=2000), "s"),
+                                     (dict(dtype=3), "a"), (dict(pos_dtype=-1), "a"), (dict(axes=0), "s"), (dict(heads1=-1), "s"),
+                                     (dict(heads1=5000), "s"), (dict(dh=5000), "s"), (dict(struct_size=8), "a"), (dict(B=1 << 20, N=1 << 20), "s")])
+def test_rotary_refusals(kw, want):
+    rc = O.load().hs_rotary_axes(C.byref(_rot(**kw)), P, P, P, P, P, P, P, None)
+    assert rc == (L.HS_ERR_SHAPE if want == "s" else L.HS_ERR_ARG)
+
+
+def _diff(**kw):
+    d = O.DiffAttnDesc(2, 5, 7, 4, 2, 64, L.PREC_BF16, 0, 0, 1, 0.125)
+    d.q_b, d.q_n, d.q_h, d.k_b, d.k_n, d.k_h, d.v_b, d.v_n, d.v_h = 5 * 512, 512, 64, 7 * 256, 256, 64, 7 * 256, 256, 128
+    d.go_b, d.go_n, d.go_h = 5 * 512, 512, 128
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+@no_gpu_only
+@pytest.mark.parametrize("kw,want", [(dict(B=0), "s"), (dict(Nq=0), "s"), (dict(Nk=0), "s"), (dict(H=3), "s"), (dict(Hkv=0), "s"), (dict(d=48), "s"),
+                                     (dict(d=256), "s"), (dict(dtype=L.PREC_F32), "a"), (dict(scale=0.0), "a"), (dict(scale=float("nan")), "a"),
+                                     (dict(q_n=511), "s"), (dict(k_h=-64), "s"), (dict(v_b=4), "s"), (dict(go_n=3), "s"), (dict(lam_stride=-1), "a"),
+                                     (dict(struct_size=0), "a"), (dict(Nk=1 << 29), "s")])
+def test_diff_attention_refusals(kw, want):
+    lib, bad, code = O.load(), _diff(**kw), L.HS_ERR_SHAPE if want == "s" else L.HS_ERR_ARG
+    if "go_n" not in kw:
+        assert lib.hs_diff_attn_fwd(C.byref(bad), P, P, P, P, None, None, P, None, None, P, 1 << 40, None) == code
+        assert lib.hs_diff_attn_fwd_ws_bytes(C.byref(bad)) == lib.hs_diff_attn_bwd_ws_bytes(C.byref(bad)) == 0
+    assert lib.hs_diff_attn_bwd(C.byref(bad), P, P, P, P, None, None, P, P, P, P, P, P, P, P, 1 << 40, None) == code
+
+
+@no_gpu_only
+def test_diff_attention_pointers_and_workspace():
+    lib, d = O.load(), _diff()
+    assert lib.hs_diff_attn_fwd(C.byref(d), P + 8, P, P, P, None, None, P, None, None, None, 0, None) == L.HS_ERR_SHAPE
+    assert lib.hs_diff_attn_fwd(C.byref(d), P, P, P, P, None, None, P, P, None, None, 0, None) == L.HS_ERR_ARG       # maps without statistics
+    need = lib.hs_diff_attn_bwd_ws_bytes(C.byref(d))
+    assert need == 2 * 4 * 5 * 12
+    assert lib.hs_diff_attn_bwd(C.byref(d), P, P, P, P, None, None, P, P, P, P, P, P, P, P, need - 1, None) == L.HS_ERR_SHAPE
+    long = _diff(Nq=1, Nk=100000)
+    need = lib.hs_diff_attn_fwd_ws_bytes(C.byref(long))
+    assert need > 0
+    assert lib.hs_diff_attn_fwd(C.byref(long), P, P, P, P, None, None, P, None, None, P, need - 1, None) == L.HS_ERR_SHAPE
+    assert lib.hs_diff_attn_fwd(C.byref(long), P, P, P, P, None, None, P, None, None, None, 0, None) == L.HS_ERR_SHAPE
+
+
+@no_gpu_only
+def test_adamw_refusals():
+    lib = O.load()
+    def call(entry=(P, P, P, P, P, P, P, 64), count=1, dtype=L.PREC_F32, bits=8, lr=1e-3, b1=0.9, b2=0.99, eps=1e-8, wd=0.0):
+        words = (C.c_int64 * 8)(*entry)
+        return lib.hs_adamw_multi(words, count, dtype, bits, lr, b1, b2, eps, wd, None)
+    for kw in (dict(count=0), dict(dtype=3), dict(bits=16), dict(b1=1.0), dict(b2=-0.1), dict(eps=-1.0), dict(entry=(0, P, P, P, P, P, P, 64)),
+               dict(entry=(P, P, P, P, 0, P, P, 64)), dict(entry=(P, P, P, P, P, P, 0, 64)), dict(entry=(P, P, P, P, P, P, P + 4, 64)),
+               dict(entry=(P + 2, P, P, P, P, P, P, 64)), dict(entry=(P, P, P + 2, P, 0, 0, P, 64), bits=32)):
+        assert call(**kw) == L.HS_ERR_ARG
+    assert call(entry=(P, P, P, P, P, P, P, -1)) == L.HS_ERR_SHAPE
+    assert lib.hs_adamw_moments((C.c_int64 * 8)(P, P, P, P, P, P, P, 64), 1, L.PREC_F16, None) == L.HS_ERR_ARG
+
+
+def test_entry_points_refuse_host_tensors_and_bad_plans():
+    q = torch.zeros(1, 2, 4, 32, dtype=torch.bfloat16)
+    with pytest.raises(L.HsError, match="no CPU fallback"):
+        H.rotary_axes(q, None, torch.zeros(3, 2, dtype=torch.int32), H.RotaryAxes((4, 6, 6), device="cpu"))
+    with pytest.raises(L.HsError, match="no CPU fallback"):
+        H.diff_attention(q, q, torch.zeros(1, 2, 2, 64, dtype=torch.bfloat16), torch.ones(2))
+    p = torch.nn.Parameter(torch.zeros(4))
+    p.grad = torch.zeros(4)
+    with pytest.raises(L.HsError, match="no CPU fallback"):
+        H.AdamW([p]).step()
+    for kw in (dict(sections=()), dict(sections=(4, -1)), dict(sections=(0, 0)), dict(sections=(600,)), dict(sections=(4,), ladder="x"),
+               dict(sections=(4,), theta=0.0)):
+        with pytest.raises(ValueError):
+            H.RotaryAxes(**kw, device="cpu")
+    for kw in (dict(state_bits=16), dict(lr=-1.0), dict(betas=(1.0, 0.9)), dict(eps=-1.0), dict(weight_decay=-1.0), dict(lr=torch.tensor(1.0))):
+        with pytest.raises(ValueError):
+            H.AdamW([p], **kw)
+    with pytest.raises(ValueError, match="bf16, fp16 or fp32"):
+        H.AdamW([torch.nn.Parameter(torch.zeros(4, dtype=torch.float64))])
+
+
+def test_rotary_ladders():
+    shared, per = H.RotaryAxes((2, 3, 3), 100.0, "shared", device="cpu"), H.RotaryAxes((2, 3, 3), 100.0, "per_axis", device="cpu")
+    assert shared.axis.tolist() == per.axis.tolist() == [0, 0, 1, 1, 1, 2, 2, 2] and shared.freq.dtype == torch.float64
+    assert torch.allclose(shared.freq, 100.0 ** (-torch.arange(8, dtype=torch.float64) / 8), rtol=1e-14)
+    assert torch.allclose(per.freq, 100.0 ** -torch.tensor([0, 1 / 2, 0, 1 / 3, 2 / 3, 0, 1 / 3, 2 / 3], dtype=torch.float64), rtol=1e-14)
