@@ -113,10 +113,11 @@ def stream() -> int:
 
 def rows_of_heads(t: torch.Tensor, align: int) -> bool:
     """whether a [B, N, heads, columns] tensor can be read where it lies: columns side by side, other strides (of axes longer than 1)
-    positive multiples of `align` elements, its first element on a 16-byte address."""
+    positive multiples of `align` elements (tokens and heads at most 2^24 apart), its first element on a 16-byte address."""
     if t.stride(3) != 1 and t.shape[3] != 1:
         return False
-    return t.data_ptr() % 16 == 0 and all(n == 1 or (s > 0 and s % align == 0) for n, s in zip(t.shape[:3], t.stride()[:3]))
+    return t.data_ptr() % 16 == 0 and all(n == 1 or (s > 0 and s % align == 0) for n, s in zip(t.shape[:3], t.stride()[:3])) \
+        and t.stride(1) <= 1 << 24 and t.stride(2) <= 1 << 24
 
 
 def bnh(t: torch.Tensor, align: int = 1):

@@ -25,7 +25,7 @@ struct Args {
     const int *q_start, *kv_len;
     bf16_t *o, *maps;
     float* lse;                                // [B][H][hi of both maps, lo of both][Nq] (put_lse); hi = +inf: no visible key
-    float *D, *x2;                             // backward: D_m [B][H][2][Nq], D_2 in full precision [B][H][Nq]
+    float *D, *x2, *rc;                        // backward: D_m [B][H][2][Nq], D_2 in full precision [B][H][Nq], constants of the rows (diff_rows_kernel)
     bf16_t *dq, *dk, *dv;
     float* part;                               // split forward: numerators, then (maximum, sum)
     long q_b, q_n, q_h, k_b, k_n, k_h, v_b, v_n, v_h, go_b, go_n, go_h;
@@ -46,35 +46,48 @@ __device__ __forceinline__ int first_pos(const Args& a, int b) {
 // number of leading keys that query i sees
 __device__ __forceinline__ int visible(const Args& a, int len, int start, int i) { return a.causal ? max(0, min(len, start + i + 1)) : len; }
 
-// ---- a tile: ROWS rows of [two heads of d | 2d] columns, through registers into LDS images ------------------------------------------------
-// A thread always moves the same 16-byte column chunk, so its source is one pointer and one row stride.
-template <int D, int ROWS, int NT> struct Stage {
-    static constexpr int CH = D / 2, PER = ROWS * CH / NT, STEP = NT / CH, BASES = STEP < 16 ? 16 / STEP : 1;
-    const char* src;
-    long stride;
-    int row, dst[BASES];                       // (image R's swizzle repeats every 16 rows)
-    u32x4 r[PER];
-    __device__ __forceinline__ void init(int tid, const bf16_t* x, long x_n, long x_h, const bf16_t* y, long y_n) {
-        const int cc = tid % CH, col = cc * 8;
-        row = tid / CH;
-        const bool pair = cc < CH / 2;
-        src = (const char*)(pair ? x + (col / D) * x_h + col % D : y + (col - 2 * D));
-        stride = (pair ? x_n : y_n) * 2;
+// ---- a tile: ROWS rows of [two heads of d | VC value columns], sent straight into LDS images ------------------------------------------------------
+// A wave's instruction moves 8 rows of an image, 16 bytes a lane; the image's swizzle is applied to the source.  It is written out because its builtin
+// makes the compiler wait for it in front of the next LDS read, whatever that reads: issue() only starts the transfers, landed() waits for this
+// wave's; a barrier behind landed() makes a tile readable to the others.
+template <int D, int VC, int ROWS, int NW> struct Dma {
+    static constexpr int PAIRS = D / 32, IMAGES = PAIRS + VC / 64, GROUPS = ROWS / 8, PER = IMAGES * GROUPS / NW;
+    static_assert(PER * NW == IMAGES * GROUPS && (NW == 1 || NW % GROUPS == 0), "whole pieces");
+    static constexpr int BASES = NW == 1 ? 2 : 1;                         // a lone wave moves even and odd groups of 8 rows, whose swizzles differ
+    const char *x, *y;
+    long x_n, y_n, x_h;
+    int wave, row;
+    unsigned vx[BASES], vy[BASES];             // byte offsets of the lane's chunk in image 0 of the pair and of the values
+    __device__ __forceinline__ void init(int wave_, int lane, const bf16_t* x_, long x_n_, long x_h_, const bf16_t* y_, long y_n_) {
+        x = (const char*)x_; y = (const char*)y_; x_n = x_n_ * 2; y_n = y_n_ * 2; x_h = x_h_ * 2; wave = wave_;
+        row = wave % GROUPS * 8 + (lane >> 3);
 #pragma unroll
-        for (int i = 0; i < BASES; ++i) dst[i] = (cc >> 3) * (ROWS * 128) + offR(row + i * STEP, cc & 7);
-    }
-    __device__ __forceinline__ void load(int first, int end) {       // rows at or behind `end` become zeros, and are not touched
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int n = first + row + i * STEP;
-            r[i] = u32x4{0u, 0u, 0u, 0u};
-            if (n < end) r[i] = *(const u32x4*)(src + n * stride);
+        for (int i = 0; i < BASES; ++i) {
+            const int ch = (lane & 7) ^ swzR(row + 8 * i);
+            vx[i] = (unsigned)(row * x_n + (D == 32 ? (ch >> 2) * x_h + (ch & 3) * 16 : ch * 16));
+            vy[i] = (unsigned)(row * y_n + ch * 16);
         }
     }
-    __device__ __forceinline__ void write(char* lds) const {
-#pragma unroll
-        for (int i = 0; i < PER; ++i) *(u32x4*)(lds + dst[i % BASES] + i / BASES * BASES * STEP * 128) = r[i];
+    static __device__ __forceinline__ u32x4 resource(const char* p) {
+        const unsigned long long a = (unsigned long long)p;
+        return u32x4{(unsigned)__builtin_amdgcn_readfirstlane((unsigned)a), (unsigned)__builtin_amdgcn_readfirstlane((unsigned)(a >> 32)), HS_MAX_RECORDS, 0x00020000u};
     }
+    __device__ __forceinline__ void issue(unsigned lds, int first, int end) const {      // rows at or behind `end` become zeros, and are not touched
+        const u32x4 rx = resource(x + first * x_n), ry = resource(y + first * y_n);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int g = i * NW + wave, image = g / GROUPS, group = g % GROUPS, more = NW == 1 ? group * 8 : 0;
+            const bool pair = image < PAIRS;
+            const int im = pair ? image : image - PAIRS;
+            unsigned off = pair ? vx[BASES == 2 ? i & 1 : 0] : vy[BASES == 2 ? i & 1 : 0];
+            off = first + row + more < end ? off : HS_OOB_OFF;
+            const unsigned so = (unsigned)(pair ? more * x_n + (D == 32 ? 0 : D == 64 ? im * x_h : (im >> 1) * x_h + (im & 1) * 128) : more * y_n + im * 128);
+            const unsigned at = lds + image * (ROWS * 128) + group * 1024;
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+                         :: "s"(__builtin_amdgcn_readfirstlane(at)), "v"(off), "s"(pair ? rx : ry), "s"(__builtin_amdgcn_readfirstlane(so)) : "memory");
+        }
+    }
+    template <int LEFT = 0> static __device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(%0)" :: "i"(LEFT) : "memory"); }
 };
 // Where a lane's fragments lie in a tile: every fragment is one of these 8 addresses plus a constant, which becomes the LDS instruction's offset.
 struct Lane {
@@ -108,6 +121,9 @@ struct Lane {
                     __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_PTR(bf16x4))(__UINTPTR_TYPE__)(col[d][1] + o)));
     }
 };
+// Waits for the loads so far.  The compiler counts a loop's first pass into all others: operands still on their way at the loop's entry would make
+// every pass wait for the newest loads, the next tile's.
+__device__ __forceinline__ void arrived() { __builtin_amdgcn_s_waitcnt(0x0F70); }
 __device__ __forceinline__ bf16x8 load8(const bf16_t* p) { return *(const bf16x8*)p; }
 template <bool F16> __device__ __forceinline__ void store4(bf16_t* p, float a, float b, float c, float d) {
     u32x2 u;
@@ -127,11 +143,13 @@ template <int NB> __device__ __forceinline__ void clear(f32x16 (&acc)[NB]) {
     for (int i = 0; i < NB; ++i) acc[i] = zero16();
 }
 
-// One map's softmax over 32 keys of a query: s becomes 2^(c2 s - m).  m, the reference, is the largest score so far up to HEADROOM: it moves,
+// One map's softmax over 32 keys of a query is taken against a reference m: the largest score so far up to HEADROOM.  It moves,
 // and l and the numerators with it, only when a score passes it by more, which after the first tiles is rare; any reference gives the same
 // quotient.  It is one number for both halves of a query's lanes (they hold different keys of one product).
-template <int NB>
-__device__ __forceinline__ void softmax_step(f32x16& s, float c2, float& m, float& l, f32x16 (&o)[NB]) {
+// The numerators are divided by the sum of P as rounded for their product, so that a query of few keys gets their values' average with no error of P's;
+// a backward pass wants the sum of P itself (SUMS 2).
+template <int SUMS, int NB>
+__device__ __forceinline__ void follow_max(const f32x16& s, float c2, float& m, float (&l)[SUMS], f32x16 (&o)[NB]) {
     float mx = s[0];
 #pragma unroll
     for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
@@ -139,7 +157,8 @@ __device__ __forceinline__ void softmax_step(f32x16& s, float c2, float& m, floa
     if (__builtin_amdgcn_ballot_w64(mx > m + HEADROOM)) {
         mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
         const float mn = fmaxf(m, ceilf(mx)), alpha = __builtin_amdgcn_exp2f(m - mn);
-        l *= alpha;
+#pragma unroll
+        for (int i = 0; i < SUMS; ++i) l[i] *= alpha;
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
 #pragma unroll
@@ -148,14 +167,33 @@ __device__ __forceinline__ void softmax_step(f32x16& s, float c2, float& m, floa
         }
         m = mn;
     }
-    float part[4] = {0.f, 0.f, 0.f, 0.f};                                 // short sums first: l runs over thousands of keys
+}
+template <bool F16> __device__ __forceinline__ float add2(unsigned pair, float sum) {      // sum + both halves, in fp32
+    typedef __attribute__((ext_vector_type(2))) __bf16 b2;
+    typedef __attribute__((ext_vector_type(2))) _Float16 h2;
+    if constexpr (F16) return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, pair), h2{(_Float16)1.f, (_Float16)1.f}, sum, false);
+    else return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, pair), b2{(__bf16)1.f, (__bf16)1.f}, sum, false);
+}
+// p = 2^(c2 s - m) rounded for the product; l += their sums (short ones first: they run over thousands of keys)
+template <bool F16, int SUMS>
+__device__ __forceinline__ void softmax_weights(f32x16& s, float c2, float m, float (&l)[SUMS], bf16x8 (&p)[2]) {
+    float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c2, -m));
-        s[r] = p;
-        part[r & 3] += p;
+    for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c2, -m));
+    if (SUMS == 2) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) part[r & 3] += s[r];
+        l[SUMS - 1] += (part[0] + part[1]) + (part[2] + part[3]);
+        part[0] = part[1] = 0.f;
     }
-    l += (part[0] + part[1]) + (part[2] + part[3]);
+#pragma unroll
+    for (int sp = 0; sp < 2; ++sp) {
+        p[sp] = pack8<F16>(s, sp);
+        const u32x4 w = __builtin_bit_cast(u32x4, p[sp]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) part[e & 1] = add2<F16>(w[e], part[e & 1]);
+    }
+    l[0] += part[0] + part[1];
 }
 // What the backward pass needs of a row's softmax: P = 2^(c2 s - hi - lo), hi whole (the reference m is), 0 <= lo < 1.  One fp32 number of their sum's
 // size would put a common error of 5e-7 on all of a row's P, which the sum that is lam's gradient would keep.
@@ -165,55 +203,112 @@ __device__ __forceinline__ void put_lse(float* p, long next, float m, float l) {
     p[next] = l == 0.f ? 0.f : __builtin_amdgcn_logf(__builtin_amdgcn_ldexpf(l, -e));
 }
 
-// both maps of one wave's 32 queries against the 32 keys whose rows start at r0 of the tile; lim: visible keys of the lane's query, counted from
-// the tile's first row; MASK: some of them may not be visible
+// The parts of a step of one wave's 32 queries against 32 keys: both maps' scores, their softmax (lim: visible keys of the lane's query, counted from
+// the step's first; mask: some of the 32 may not be visible), the products with V.
 template <int D, bool F16, int ROWS>
-__device__ __forceinline__ void forward_step(const Lane& f, int r0, bool mask, int lim, int h, float c2, const bf16x8 (&qf)[2][D / 16], float (&m)[2],
-                                             float (&l)[2], f32x16 (&o1)[D / 16], f32x16 (&o2)[D / 16]) {
-    f32x16 s[2] = {zero16(), zero16()};
+__device__ __forceinline__ void scores(const Lane& f, const bf16x8 (&qf)[2][D / 16], f32x16 (&s)[2]) {
+    constexpr int N = D / 8, AHEAD = 4;                                   // fragments are read AHEAD products before their use
+    bf16x8 x[AHEAD];
+#pragma unroll
+    for (int n = 0; n < AHEAD; ++n) x[n] = f.template rows16<ROWS>(n * 16);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        const int i = n / (D / 16), ks = n % (D / 16);
+        s[i] = mfma32<F16>(x[n % AHEAD], qf[i][ks], ks ? s[i] : zero16());
+        if (n + AHEAD < N) x[n % AHEAD] = f.template rows16<ROWS>((n + AHEAD) * 16);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+// scores of both maps and dP: the tile's columns are [keys | values] against q and dO
+template <int D, bool F16, int ROWS>
+__device__ __forceinline__ void scores_dp(const Lane& f, const bf16x8 (&qf)[2][D / 16], const bf16x8 (&gf)[D / 8], f32x16 (&s)[2], f32x16& dp) {
+    constexpr int N = D / 4, AHEAD = 4;
+    bf16x8 x[AHEAD];
+#pragma unroll
+    for (int n = 0; n < AHEAD; ++n) x[n] = f.template rows16<ROWS>(n * 16);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        const int i = n / (D / 16), ks = n % (D / 16);
+        if (i < 2) s[i & 1] = mfma32<F16>(x[n % AHEAD], qf[i & 1][ks], ks ? s[i & 1] : zero16());
+        else dp = mfma32<F16>(x[n % AHEAD], gf[n - D / 8], n > D / 8 ? dp : zero16());
+        if (n + AHEAD < N) x[n % AHEAD] = f.template rows16<ROWS>((n + AHEAD) * 16);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+__device__ __forceinline__ void mask_keys(f32x16 (&s)[2], int lim, int h) {
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) s[i] = mfma32<F16>(f.template rows16<ROWS>(i * D + ks * 16), qf[i][ks], s[i]);
-    if (mask) {
+        for (int r = 0; r < 16; ++r) s[i][r] = acc_row(r, h) < lim ? s[i][r] : -__builtin_inff();
+}
+template <bool F16> __device__ __forceinline__ void pack2maps(const f32x16 (&s)[2], bf16x8 (&p)[2][2]) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[i][r] = r0 + acc_row(r, h) < lim ? s[i][r] : -__builtin_inff();
-    }
-    softmax_step(s[0], c2, m[0], l[0], o1);
-    softmax_step(s[1], c2, m[1], l[1], o2);
+        for (int sp = 0; sp < 2; ++sp) p[i][sp] = pack8<F16>(s[i], sp);
+}
+template <int D, bool F16, int ROWS, int NB>
+__device__ __forceinline__ void values(const Lane& f, const bf16x8 (&p)[2][2], f32x16 (&o1)[NB], f32x16 (&o2)[NB]) {
+    constexpr int N = 2 * NB, AHEAD = 4;
+    bf16x8 x[AHEAD];
+#pragma unroll
+    for (int n = 0; n < AHEAD; ++n) x[n] = f.template cols32<ROWS>(16 * (n / NB), 2 * D + n % NB * 32);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int sp = 0; sp < 2; ++sp) {
-        const bf16x8 p1 = pack8<F16>(s[0], sp), p2 = pack8<F16>(s[1], sp);
-#pragma unroll
-        for (int db = 0; db < D / 16; ++db) {
-            const bf16x8 vf = f.template cols32<ROWS>(16 * sp, 2 * D + db * 32);
-            o1[db] = mfma32<F16>(vf, p1, o1[db]);
-            o2[db] = mfma32<F16>(vf, p2, o2[db]);
-        }
+    for (int n = 0; n < N; ++n) {
+        const int sp = n / NB, db = n % NB, q = n + AHEAD;
+        o1[db] = mfma32<F16>(x[n % AHEAD], p[0][sp], o1[db]);
+        o2[db] = mfma32<F16>(x[n % AHEAD], p[1][sp], o2[db]);
+        if (q < N) x[n % AHEAD] = f.template cols32<ROWS>(16 * (q / NB), 2 * D + q % NB * 32);
+        __builtin_amdgcn_sched_barrier(0);
     }
 }
 
-// ---- forward: a block is NW waves of 32 queries of one head ------------------------------------------------------------------------------
-template <int D, bool F16, int NW>
-__global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void diff_fwd_kernel(Args a) {
-    constexpr int ROWS = D == 128 ? 32 : 64, TILE = ROWS * D * 8, NT = NW * 64, NB = D / 16;
-    extern __shared__ __attribute__((aligned(16))) char smem[];           // two tiles
+// ---- the phases of a sweep -----------------------------------------------------------------------------------------------------------------------
+// The forward, dq and dk,dv sweeps share one scheme: a wave keeps 32 rows of its own and a tile of 32 rows streams past a step.  A step is a vector phase (the
+// softmax weights of the step) and a matrix phase (the products that the weights go into, then the next step's scores), a barrier behind each.
+// At d = 32 and 64 a block has 8 waves; w and w + 4 share a SIMD, and the later four run half a step behind: while one works on the vector units, the
+// other has the matrix pipe (left to themselves both do the same thing at the same time).  At d = 128 a SIMD's registers hold one wave only, and the
+// forward pass' numerators of half of the values: two blocks then, each with the scores of all.
+// Tile t is first read in the matrix phase of step t - 1 and left in step t's, half a step later by the later waves: it is sent for in step t - LEAD
+// into the buffer of tile t - BUFS, and has landed (every wave waits for its own part) in the vector phase of the next step.
+template <int D> struct Sweep {
+    static constexpr bool PAIRED = D < 128;
+    static constexpr int NW = PAIRED ? 8 : 4, ROWS = 32, TILE = ROWS * D * 8, HALVES = PAIRED ? 1 : 2, VC = 2 * D / HALVES, BUFS = PAIRED ? 5 : 3, LEAD = PAIRED ? 3 : 2, OWN = NW * 32;
+    static __device__ __forceinline__ void fall_behind(int wave) { if (PAIRED && wave >= NW / 2) __syncthreads(); }
+    static __device__ __forceinline__ void wait_for_late(int wave) { if (PAIRED && wave < NW / 2) __syncthreads(); }
+    static __device__ __forceinline__ int next(int buf) { return buf == BUFS - 1 ? 0 : buf + 1; }
+};
+
+// ---- forward ----------------------------------------------------------------------------------------------------------------------------------
+template <int D, bool F16, bool KEEP>
+__global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void diff_fwd_kernel(Args a) {
+    typedef Sweep<D> S;
+    constexpr int ROWS = S::ROWS, VC = S::VC, TILE = ROWS * (2 * D + VC) * 2, NW = S::NW, NB = VC / 32;
+    extern __shared__ __attribute__((aligned(16))) char smem[];           // BUFS tiles
     const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, c = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int nblk = (a.Nq + NW * 32 - 1) / (NW * 32);
     int id = block_order();
+    const int half = id % S::HALVES;
+    id /= S::HALVES;
     const int blk = nblk - 1 - id % nblk;                                 // under a causal mask the last queries have most to do: first
     id /= nblk;
     const int head = id % a.H, b = id / a.H, kvh = head / a.G;
     const int len = key_count(a, b), start = first_pos(a, b);
     const int q0 = blk * (NW * 32) + wave * 32, query = q0 + c;
     const int kend = visible(a, len, start, min(blk * (NW * 32) + NW * 32, a.Nq) - 1);
-    const int lim = visible(a, len, start, query), lim_lo = visible(a, len, start, q0), lim_hi = visible(a, len, start, min(q0 + 31, a.Nq - 1));
-    const int nt = (kend + ROWS - 1) / ROWS;
+    const int lim = visible(a, len, start, query), lim_lo = visible(a, len, start, q0);
+    const int nj = (kend + ROWS - 1) / ROWS;
 
+    Lane fl;
+    fl.init(smem, lane);
+    const unsigned lds0 = lds_addr(smem);
+    Dma<D, VC, ROWS, NW> dma;
+    dma.init(wave, lane, a.k + b * a.k_b + 2 * kvh * a.k_h, a.k_n, a.k_h, a.v + b * a.v_b + kvh * a.v_h + half * VC, a.v_n);
+    for (int t = 0; t < min(S::LEAD, nj); ++t) dma.issue(lds0 + t * TILE, t * ROWS, len);
     bf16x8 qf[2][D / 16];
     {
         const bf16_t* qp = a.q + b * a.q_b + (long)min(query, a.Nq - 1) * a.q_n + 2 * head * a.q_h + 8 * h;
@@ -222,68 +317,91 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void diff_fwd_kernel(Arg
 #pragma unroll
             for (int ks = 0; ks < D / 16; ++ks) qf[i][ks] = load8(qp + i * a.q_h + ks * 16);
     }
-    float m[2] = {NONE, NONE}, l[2] = {0.f, 0.f};
-    f32x16 o1[NB], o2[NB];
-    clear(o1); clear(o2);
-    Lane fl;
-    fl.init(smem, lane);
-    Stage<D, ROWS, NT> st;
-    st.init(tid, a.k + b * a.k_b + 2 * kvh * a.k_h, a.k_n, a.k_h, a.v + b * a.v_b + kvh * a.v_h, a.v_n);
-    if (nt > 0) {
-        st.load(0, len);
-        st.write(smem);
-    }
-    __syncthreads();
-    for (int t = 0; t < nt; ++t) {
-        if (t + 1 < nt) st.load((t + 1) * ROWS, len);
-        const int k0 = t * ROWS;
-        if (q0 < a.Nq) {
-            const bool mask = k0 + ROWS > lim_lo;
-#pragma unroll 1
-            for (int r0 = 0; r0 < min(ROWS, lim_hi - k0); r0 += 32)
-                forward_step<D, F16, ROWS>(fl.at((t & 1) * TILE + r0 * 128), r0, mask, lim - k0, h, a.c2, qf, m, l, o1, o2);
+    constexpr int SUMS = KEEP ? 2 : 1;
+    float m[2], l[2][SUMS];
+    f32x16 o1[NB], o2[NB], s[2];
+    // The reference that scores are taken against is the largest of the first 32 keys' (a query that sees any key sees the first), and stays: a maximum
+    // a step would be a fifth of the vector instructions that bound this loop.  Where a sum shows that later scores passed it so far that P leaves the
+    // range (fp16: 2^15, P itself; bf16: 2^40, which leaves 2^87 for the values), the block starts again and keeps a running maximum.
+    for (bool running = false;; running = true) {
+        if (running) {
+            for (int t = 0; t < min(S::LEAD, nj); ++t) dma.issue(lds0 + t * TILE, t * ROWS, len);
         }
-        if (t + 1 < nt) st.write(smem + ((t + 1) & 1) * TILE);
+        m[0] = m[1] = NONE;
+        l[0][0] = l[1][0] = l[0][SUMS - 1] = l[1][SUMS - 1] = 0.f;
+        clear(o1); clear(o2);
+        arrived();
+        dma.landed();
         __syncthreads();
+        scores<D, F16, ROWS>(fl, qf, s);                                  // (without a tile, or behind the last: of what lies there, not used)
+        S::fall_behind(wave);
+        int buf = 0, ahead = S::LEAD;                                     // the step's buffer, and the one to send to
+        for (int j = 0; j < nj; ++j) {
+            dma.landed();
+            if (j + S::LEAD < nj) dma.issue(lds0 + ahead * TILE, (j + S::LEAD) * ROWS, len);
+            ahead = S::next(ahead);
+            if (j * 32 + 32 > lim_lo) mask_keys(s, lim - j * 32, h);
+            if (j == 0 || running) {
+                follow_max(s[0], a.c2, m[0], l[0], o1);
+                follow_max(s[1], a.c2, m[1], l[1], o2);
+            }
+            bf16x8 p[2][2];
+            softmax_weights<F16>(s[0], a.c2, m[0], l[0], p[0]);
+            softmax_weights<F16>(s[1], a.c2, m[1], l[1], p[1]);
+            __syncthreads();
+            __builtin_amdgcn_s_setprio(1);
+            values<D, F16, ROWS>(fl.at(buf * TILE), p, o1, o2);
+            buf = S::next(buf);
+            scores<D, F16, ROWS>(fl.at(buf * TILE), qf, s);
+            __builtin_amdgcn_s_setprio(0);
+            __syncthreads();
+        }
+        S::wait_for_late(wave);
+        constexpr float MOST = F16 ? 32768.f : 1.0995116e12f;
+        if (running || !__syncthreads_or(!(l[0][0] < MOST && l[1][0] < MOST))) break;
     }
     if (query >= a.Nq) return;
     const float lam = a.lam[head * a.lam_stride];
     float inv[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        l[i] += __shfl_xor(l[i], 32, 64);
-        inv[i] = l[i] > 0.f ? 1.0f / l[i] : l[i] == 0.f ? 0.f : l[i];      // (a NaN stays one)
+#pragma unroll
+        for (int k = 0; k < SUMS; ++k) l[i][k] += __shfl_xor(l[i][k], 32, 64);
+        inv[i] = l[i][0] > 0.f ? 1.0f / l[i][0] : l[i][0] == 0.f ? 0.f : l[i][0];      // (a NaN stays one)
     }
-    const long row = ((long)b * a.Nq + query) * a.H + head;
-    if (a.maps) {
-        store_rows<F16>(a.maps + row * 2 * D, o1, inv[0], h);
-        store_rows<F16>(a.maps + ((long)a.B * a.Nq * a.H + row) * 2 * D, o2, inv[1], h);
+    const long row = ((long)b * a.Nq + query) * a.H + head, at = row * 2 * D + half * VC;
+    if (KEEP) {
+        store_rows<F16>(a.maps + at, o1, inv[0], h);
+        store_rows<F16>(a.maps + (long)a.B * a.Nq * a.H * 2 * D + at, o2, inv[1], h);
         float* ls = a.lse + ((long)b * a.H + head) * 4 * a.Nq + query;
-        if (h == 0) {
-            put_lse(ls, 2 * a.Nq, m[0], l[0]);
-            put_lse(ls + a.Nq, 2 * a.Nq, m[1], l[1]);
+        if (h == 0 && half == 0) {
+            put_lse(ls, 2 * a.Nq, m[0], l[0][SUMS - 1]);
+            put_lse(ls + a.Nq, 2 * a.Nq, m[1], l[1][SUMS - 1]);
         }
     }
     const float w2 = lam * inv[1];
 #pragma unroll
     for (int db = 0; db < NB; ++db)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) o1[db][r] = o1[db][r] * inv[0] - w2 * o2[db][r];
-    store_rows<F16>(a.o + row * 2 * D, o1, 1.0f, h);
+        for (int r = 0; r < 16; ++r) o1[db][r] = __builtin_fmaf(-w2, o2[db][r], o1[db][r] * inv[0]);
+    store_rows<F16>(a.o + at, o1, 1.0f, h);
 }
 
 // ---- split forward: few queries against many keys ------------------------------------------------------------------------------------------
 // HBM-bound: K and V are read once for all query heads of a key head.  A wave's 32 rows are (head of the group, query) pairs; a block takes one
-// chunk of the keys, each of its waves every NW-th tile of 32 keys through LDS of its own (no barrier in the loop).  The waves' numerators are
+// chunk of the keys, each of its waves every NW-th tile of 32 keys through two LDS buffers of its own (no barrier in the loop).  The waves' numerators are
 // joined in LDS, and the chunks' by diff_join_kernel; with one chunk the result is written at once.
-template <int D, bool F16, int NW>
+template <int D, bool F16, bool KEEP, int NW>
 __global__ __launch_bounds__(NW * 64, 1) void diff_split_kernel(Args a) {
-    constexpr int ROWS = 32, TILE = ROWS * D * 8, NB = D / 16, NT = NW * 64, PER = 32 * 2 * D / NT;
-    extern __shared__ __attribute__((aligned(16))) char smem[];           // NW tiles; then the waves' numerators of one map
-    __shared__ float wm[2][NW][32], wl[2][NW][32];
+    typedef Sweep<D> S;
+    constexpr int ROWS = 32, VC = S::VC, TILE = ROWS * (2 * D + VC) * 2, NB = VC / 32, NT = NW * 64, PER = 32 * VC / NT;
+    extern __shared__ __attribute__((aligned(16))) char smem[];           // 2 NW tiles; then the waves' numerators of one map
+    constexpr int SUMS = KEEP ? 2 : 1;
+    __shared__ float wm[2][NW][32], wl[2][SUMS][NW][32];
     const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, c = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int id = blockIdx.x;
+    const int half = id % S::HALVES; id /= S::HALVES;
     const int split = id % a.nsplit; id /= a.nsplit;
     const int tile = id % a.tiles; id /= a.tiles;
     const int kvh = id % a.Hkv, b = id / a.Hkv;
@@ -297,6 +415,10 @@ __global__ __launch_bounds__(NW * 64, 1) void diff_split_kernel(Args a) {
 #pragma unroll
     for (int i = 16; i > 0; i >>= 1) k1 = max(k1, __shfl_xor(k1, i, 64));
     k1 = __builtin_amdgcn_readfirstlane(k1);
+    int lim_lo = lim;                                                     // keys that every row sees
+#pragma unroll
+    for (int i = 16; i > 0; i >>= 1) lim_lo = min(lim_lo, __shfl_xor(lim_lo, i, 64));
+    lim_lo = __builtin_amdgcn_readfirstlane(lim_lo);
 
     bf16x8 qf[2][D / 16];
     {
@@ -306,37 +428,52 @@ __global__ __launch_bounds__(NW * 64, 1) void diff_split_kernel(Args a) {
 #pragma unroll
             for (int ks = 0; ks < D / 16; ++ks) qf[i][ks] = load8(qp + i * a.q_h + ks * 16);
     }
-    float m[2] = {NONE, NONE}, l[2] = {0.f, 0.f};
+    float m[2] = {NONE, NONE}, l[2][SUMS] = {};
     f32x16 o[2][NB];
     clear(o[0]); clear(o[1]);
+    char* const own = smem + wave * (2 * TILE);
     Lane fl;
-    fl.init(smem, lane);
-    Stage<D, ROWS, 64> st;
-    st.init(lane, a.k + b * a.k_b + 2 * kvh * a.k_h, a.k_n, a.k_h, a.v + b * a.v_b + kvh * a.v_h, a.v_n);
-    char* lds = smem + wave * TILE;
-    int t = k0 + wave * ROWS;
-    constexpr bool AHEAD = D < 128;                                       // (at d = 128 the next tile does not fit the registers beside the numerators)
-    if (AHEAD && t < k1) st.load(t, len);
+    fl.init(own, lane);
+    Dma<D, VC, ROWS, 1> dma;
+    dma.init(0, lane, a.k + b * a.k_b + 2 * kvh * a.k_h, a.k_n, a.k_h, a.v + b * a.v_b + kvh * a.v_h + half * VC, a.v_n);
+    arrived();
+    int t = k0 + wave * ROWS, buf = 0;
+    if (t < k1) dma.issue(lds_addr(own), t, len);
     for (; t < k1; t += NW * ROWS) {
-        if (!AHEAD) st.load(t, len);
-        st.write(lds);
-        if (AHEAD && t + NW * ROWS < k1) st.load(t + NW * ROWS, len);
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        forward_step<D, F16, ROWS>(fl.at(wave * TILE), 0, true, lim - t, h, a.c2, qf, m, l, o[0], o[1]);
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (t + NW * ROWS < k1) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");            // (the last step's reads of that buffer are over)
+            dma.issue(lds_addr(own) + (buf ^ 1) * TILE, t + NW * ROWS, len);
+            dma.template landed<Dma<D, VC, ROWS, 1>::PER>();
+        } else {
+            dma.landed();
+        }
+        const Lane f = fl.at(buf * TILE);
+        buf ^= 1;
+        f32x16 s[2];
+        bf16x8 p[2][2];
+        scores<D, F16, ROWS>(f, qf, s);
+        if (t + ROWS > lim_lo) mask_keys(s, lim - t, h);
+        follow_max(s[0], a.c2, m[0], l[0], o[0]);
+        follow_max(s[1], a.c2, m[1], l[1], o[1]);
+        softmax_weights<F16>(s[0], a.c2, m[0], l[0], p[0]);
+        softmax_weights<F16>(s[1], a.c2, m[1], l[1], p[1]);
+        values<D, F16, ROWS>(f, p, o[0], o[1]);
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        l[i] += __shfl_xor(l[i], 32, 64);
-        if (h == 0) { wm[i][wave][c] = m[i]; wl[i][wave][c] = l[i]; }
+        if (h == 0) wm[i][wave][c] = m[i];
+#pragma unroll
+        for (int k = 0; k < SUMS; ++k) {
+            l[i][k] += __shfl_xor(l[i][k], 32, 64);
+            if (h == 0) wl[i][k][wave][c] = l[i][k];
+        }
     }
     float first[PER];
-    const float lam = a.lam[head * a.lam_stride];
     // a thread joins PER columns of one row: row = tid % 32, columns from (tid / 32) PER
     const int jr = tid & 31, jc = (tid >> 5) * PER, JR = tile * 32 + jr;
     const long slot = (((long)(b * a.Hkv + kvh) * a.tiles + tile) * a.nsplit + split) * 2;
     float* stats = a.part + (long)a.B * a.Hkv * a.tiles * a.nsplit * 2 * 32 * (2 * D);
-    float* num = (float*)smem;                                            // [wave][2 D][32]
+    float* num = (float*)smem;                                            // [wave][VC][32]
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         __syncthreads();
@@ -347,19 +484,18 @@ __global__ __launch_bounds__(NW * 64, 1) void diff_split_kernel(Args a) {
 #pragma unroll
         for (int db = 0; db < NB; ++db)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) num[(wave * 2 * D + db * 32 + acc_row(r, h)) * 32 + c] = o[i][db][r] * f;
+            for (int r = 0; r < 16; ++r) num[(wave * VC + db * 32 + acc_row(r, h)) * 32 + c] = o[i][db][r] * f;
         __syncthreads();
         M = NONE;
-        float L = 0.f;
+        float L[SUMS] = {};
 #pragma unroll
         for (int w = 0; w < NW; ++w) M = fmaxf(M, wm[i][w][jr]);
 #pragma unroll
-        for (int w = 0; w < NW; ++w) L += wl[i][w][jr] * __builtin_amdgcn_exp2f(wm[i][w][jr] - M);
-        const float inv = L > 0.f ? 1.0f / L : L == 0.f ? 0.f : L;
-        if (JR < rows && a.nsplit > 1 && jc == 0) {
-            stats[((slot + i) * 32 + jr) * 2] = M;
-            stats[((slot + i) * 32 + jr) * 2 + 1] = L;
-        }
+        for (int k = 0; k < SUMS; ++k)
+#pragma unroll
+            for (int w = 0; w < NW; ++w) L[k] += wl[i][k][w][jr] * __builtin_amdgcn_exp2f(wm[i][w][jr] - M);
+        const float inv = L[0] > 0.f ? 1.0f / L[0] : L[0] == 0.f ? 0.f : L[0];
+        if (JR < rows && a.nsplit > 1 && jc == 0 && half == 0) *(f32x4*)(stats + ((slot + i) * 32 + jr) * 4) = f32x4{M, L[0], L[SUMS - 1], 0.f};
         const int jh = kvh * a.G + min(JR, rows - 1) / a.Nq, jq = min(JR, rows - 1) % a.Nq;
         const long row = ((long)b * a.Nq + jq) * a.H + jh;
         const float jl = a.lam[jh * a.lam_stride];
@@ -367,19 +503,17 @@ __global__ __launch_bounds__(NW * 64, 1) void diff_split_kernel(Args a) {
         for (int e = 0; e < PER; ++e) {
             float x = 0.f;
 #pragma unroll
-            for (int w = 0; w < NW; ++w) x += num[(w * 2 * D + jc + e) * 32 + jr];
+            for (int w = 0; w < NW; ++w) x += num[(w * VC + jc + e) * 32 + jr];
             if (JR >= rows) continue;
-            if (a.nsplit > 1) a.part[((slot + i) * 32 + jr) * (2 * D) + jc + e] = x;
+            if (a.nsplit > 1) a.part[((slot + i) * 32 + jr) * (2 * D) + half * VC + jc + e] = x;
             else {
                 x *= inv;
-                if (a.maps) a.maps[(i * (long)a.B * a.Nq * a.H + row) * 2 * D + jc + e] = f2h<F16>(x);
-                if (i == 0) first[e] = x; else a.o[row * 2 * D + jc + e] = f2h<F16>(first[e] - jl * x);
+                if (KEEP) a.maps[(i * (long)a.B * a.Nq * a.H + row) * 2 * D + half * VC + jc + e] = f2h<F16>(x);
+                if (i == 0) first[e] = x; else a.o[row * 2 * D + half * VC + jc + e] = f2h<F16>(first[e] - jl * x);
             }
         }
-        if (JR < rows && a.nsplit == 1 && a.maps && jc == 0)
-            put_lse(a.lse + (((long)b * a.H + jh) * 4 + i) * a.Nq + jq, 2 * a.Nq, M, L);
+        if (KEEP && JR < rows && a.nsplit == 1 && jc == 0 && half == 0) put_lse(a.lse + (((long)b * a.H + jh) * 4 + i) * a.Nq + jq, 2 * a.Nq, M, L[SUMS - 1]);
     }
-    (void)lam;
 }
 
 // joins the chunks of a row: a wave each
@@ -393,20 +527,22 @@ __global__ __launch_bounds__(256) void diff_join_kernel(Args a) {
     const int kvh = head / a.G, R = (head % a.G) * a.Nq + query;
     const int n = (key_count(a, b) + a.chunk - 1) / a.chunk;              // <= nsplit
     const long slot = (((long)(b * a.Hkv + kvh) * a.tiles + (R >> 5)) * a.nsplit) * 2;
-    const float* stats = a.part + (long)a.B * a.Hkv * a.tiles * a.nsplit * 2 * 32 * (2 * D) + (slot * 32 + (R & 31)) * 2;
+    const float* stats = a.part + (long)a.B * a.Hkv * a.tiles * a.nsplit * 2 * 32 * (2 * D) + (slot * 32 + (R & 31)) * 4;
     const float* num = a.part + (slot * 32 + (R & 31)) * (2 * D) + lane * PER;
     float out[2][PER];
     const long row = ((long)b * a.Nq + query) * a.H + head;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        float M = NONE, L = 0.f;
-        for (int s = lane; s < n; s += 64) M = fmaxf(M, stats[(s * 2 + i) * 64]);
+        float M = NONE, L = 0.f, Lx = 0.f;
+        for (int s = lane; s < n; s += 64) M = fmaxf(M, stats[(s * 2 + i) * 128]);
         M = wave_max(M);
 #pragma unroll
         for (int e = 0; e < PER; ++e) out[i][e] = 0.f;
         for (int s = 0; s < n; ++s) {
-            const float w = __builtin_amdgcn_exp2f(stats[(s * 2 + i) * 64] - M);
-            L += w * stats[(s * 2 + i) * 64 + 1];
+            const f32x4 st = *(const f32x4*)(stats + (s * 2 + i) * 128);
+            const float w = __builtin_amdgcn_exp2f(st[0] - M);
+            L += w * st[1];
+            Lx += w * st[2];
             const float* x = num + (long)(s * 2 + i) * 32 * (2 * D);
 #pragma unroll
             for (int e = 0; e < PER; ++e) out[i][e] += w * x[e];
@@ -417,7 +553,7 @@ __global__ __launch_bounds__(256) void diff_join_kernel(Args a) {
             out[i][e] *= inv;
             if (a.maps) a.maps[(i * (long)a.B * a.Nq * a.H + row) * 2 * D + lane * PER + e] = f2h<F16>(out[i][e]);
         }
-        if (a.maps && lane == 0) put_lse(a.lse + (((long)b * a.H + head) * 4 + i) * a.Nq + query, 2 * a.Nq, M, L);
+        if (a.maps && lane == 0) put_lse(a.lse + (((long)b * a.H + head) * 4 + i) * a.Nq + query, 2 * a.Nq, M, Lx);
     }
     const float lam = a.lam[head * a.lam_stride];
 #pragma unroll
@@ -425,20 +561,23 @@ __global__ __launch_bounds__(256) void diff_join_kernel(Args a) {
 }
 
 // ---- backward ----------------------------------------------------------------------------------------------------------------------------------
-// D_m = dO . O_m: 2 d / 8 lanes a row (HBM-bound: three tensors once)
+// D_m = dO . O_m, 2 d / 8 lanes a row (HBM-bound: three tensors once), and from it the constants of a row that the dk, dv sweep reads, 32 rows together:
+// the exponents' offsets of both maps (the second with lam's size in it), -D_1 and sign(lam) (D_2 - D_1); rows behind the last have P = 0.
 template <int D, bool F16>
 __global__ __launch_bounds__(256) void diff_rows_kernel(Args a) {
     constexpr int LANES = D / 4;
-    const long id = ((long)blockIdx.x * 256 + threadIdx.x) / LANES;       // (b, query, head)
+    const int qt = (a.Nq + 31) / 32;
+    const long id = ((long)blockIdx.x * 256 + threadIdx.x) / LANES;       // (b, query of whole tiles, head)
     const int part = threadIdx.x % LANES;
+    if (id >= (long)a.B * qt * 32 * a.H) return;                          // (whole groups of LANES leave)
     const long rows = (long)a.B * a.Nq * a.H;
+    const int head = id % a.H, query = id / a.H % (qt * 32), b = id / a.H / (qt * 32);
     float d[2] = {0.f, 0.f};
-    if (id < rows) {
-        const int head = id % a.H, query = id / a.H % a.Nq, b = id / a.H / a.Nq;
+    if (query < a.Nq) {
         const u32x4 g = *(const u32x4*)(a.go + b * a.go_b + query * a.go_n + head * a.go_h + part * 8);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const u32x4 o = *(const u32x4*)(a.maps + (i * rows + id) * 2 * D + part * 8);
+            const u32x4 o = *(const u32x4*)(a.maps + (i * rows + ((long)b * a.Nq + query) * a.H + head) * 2 * D + part * 8);
 #pragma unroll
             for (int e = 0; e < 4; ++e) d[i] += unpack_lo<F16>(g[e]) * unpack_lo<F16>(o[e]) + unpack_hi<F16>(g[e]) * unpack_hi<F16>(o[e]);
         }
@@ -447,56 +586,29 @@ __global__ __launch_bounds__(256) void diff_rows_kernel(Args a) {
     for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int s = LANES / 2; s > 0; s >>= 1) d[i] += __shfl_xor(d[i], s, 64);
-    if (id < rows && part == 0) {
-        const int head = id % a.H, query = id / a.H % a.Nq, b = id / a.H / a.Nq;
-        float* p = a.D + ((long)b * a.H + head) * 2 * a.Nq + query;
+    if (part) return;
+    const long bh = (long)b * a.H + head;
+    float e[2] = {__builtin_inff(), __builtin_inff()};
+    const float lam = a.lam[head * a.lam_stride];
+    if (query < a.Nq) {
+        constexpr float UP = F16 ? SHIFT16 : 0;
+        const float* ls = a.lse + bh * 4 * a.Nq + query;
+        e[0] = ls[0] + (ls[2 * a.Nq] - UP);
+        e[1] = ls[a.Nq] + (ls[3 * a.Nq] - UP) - __builtin_amdgcn_logf(fabsf(lam));
+        float* p = a.D + bh * 2 * a.Nq + query;
         p[0] = d[0];
         p[a.Nq] = d[1];
     }
+    float* r = a.rc + (bh * qt + (query >> 5)) * 128 + (query & 31);
+    r[0] = e[0]; r[32] = e[1]; r[64] = -d[0]; r[96] = copysignf(1.0f, lam) * (d[1] - d[0]);
 }
 
 // dQ: queries stay, keys stream
-template <int D, bool F16, int ROWS>
-__device__ __forceinline__ void dq_step(const Lane& f, int r0, bool mask, int lim, int h, float c2, const bf16x8 (&qf)[2][D / 16], const bf16x8 (&gf)[D / 8],
-                                        const float (&lse)[2], const float (&Dr)[2], float& x2, f32x16 (&dq1)[D / 32], f32x16 (&dq2)[D / 32]) {
-    f32x16 s[2] = {zero16(), zero16()}, dp = zero16();
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) s[i] = mfma32<F16>(f.template rows16<ROWS>(i * D + ks * 16), qf[i][ks], s[i]);
-#pragma unroll
-    for (int ks = 0; ks < D / 8; ++ks) dp = mfma32<F16>(f.template rows16<ROWS>(2 * D + ks * 16), gf[ks], dp);
-    if (mask) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[i][r] = r0 + acc_row(r, h) < lim ? s[i][r] : -__builtin_inff();
-    }
-    float part[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][r], c2, -lse[0]));
-        const float p2 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[1][r], c2, -lse[1]));
-        part[r & 3] = __builtin_fmaf(p2, dp[r], part[r & 3]);
-        s[0][r] = p1 * (dp[r] - Dr[0]);
-        s[1][r] = p2 * (dp[r] - Dr[1]);
-    }
-    x2 += (part[0] + part[1]) + (part[2] + part[3]);
-#pragma unroll
-    for (int sp = 0; sp < 2; ++sp) {
-        const bf16x8 d1 = pack8<F16>(s[0], sp), d2 = pack8<F16>(s[1], sp);
-#pragma unroll
-        for (int db = 0; db < D / 32; ++db) {
-            dq1[db] = mfma32<F16>(f.template cols32<ROWS>(16 * sp, db * 32), d1, dq1[db]);
-            dq2[db] = mfma32<F16>(f.template cols32<ROWS>(16 * sp, D + db * 32), d2, dq2[db]);
-        }
-    }
-}
-
-template <int D, bool F16, int NW>
-__global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void diff_dq_kernel(Args a) {
-    constexpr int ROWS = 64, TILE = ROWS * D * 8, NT = NW * 64;
-    extern __shared__ __attribute__((aligned(16))) char smem[];
+template <int D, bool F16>
+__global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void diff_dq_kernel(Args a) {
+    typedef Sweep<D> S;
+    constexpr int ROWS = S::ROWS, TILE = S::TILE, NW = S::NW, NQ = D / 32;
+    extern __shared__ __attribute__((aligned(16))) char smem[];           // BUFS tiles
     const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, c = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int nblk = (a.Nq + NW * 32 - 1) / (NW * 32);
@@ -507,8 +619,15 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void diff_dq_kernel(Args
     const int len = key_count(a, b), start = first_pos(a, b);
     const int q0 = blk * (NW * 32) + wave * 32, query = q0 + c, qrow = min(query, a.Nq - 1);
     const int kend = visible(a, len, start, min(blk * (NW * 32) + NW * 32, a.Nq) - 1);
-    const int lim = visible(a, len, start, query), lim_lo = visible(a, len, start, q0), lim_hi = visible(a, len, start, min(q0 + 31, a.Nq - 1));
-    const int nt = (kend + ROWS - 1) / ROWS;
+    const int lim = visible(a, len, start, query), lim_lo = visible(a, len, start, q0);
+    const int nj = (kend + ROWS - 1) / ROWS;
+
+    Lane fl;
+    fl.init(smem, lane);
+    const unsigned lds0 = lds_addr(smem);
+    Dma<D, 2 * D, ROWS, NW> dma;
+    dma.init(wave, lane, a.k + b * a.k_b + 2 * kvh * a.k_h, a.k_n, a.k_h, a.v + b * a.v_b + kvh * a.v_h, a.v_n);
+    for (int t = 0; t < min(S::LEAD, nj); ++t) dma.issue(lds0 + t * TILE, t * ROWS, len);
     bf16x8 qf[2][D / 16], gf[D / 8];
     {
         const bf16_t* qp = a.q + b * a.q_b + qrow * a.q_n + 2 * head * a.q_h + 8 * h;
@@ -523,187 +642,241 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void diff_dq_kernel(Args
     constexpr float UP = F16 ? SHIFT16 : 0;
     const long bh = (long)b * a.H + head;
     const float* ls = a.lse + bh * 4 * a.Nq + qrow;
-    const float lse[2] = {ls[0] - UP, ls[a.Nq] - UP};                     // (P comes out times 2^lo: taken off the sums at the end)
-    const float unlo[2] = {__builtin_amdgcn_exp2f(-ls[2 * a.Nq]), __builtin_amdgcn_exp2f(-ls[3 * a.Nq])};
-    const float Dr[2] = {a.D[bh * 2 * a.Nq + qrow], a.D[(bh * 2 + 1) * a.Nq + qrow]};
+    const float hi0 = ls[0] - UP, hi1 = ls[a.Nq] - UP;                    // (P comes out times 2^lo: taken off the sums at the end)
+    const float D0 = a.D[bh * 2 * a.Nq + qrow], D1 = a.D[(bh * 2 + 1) * a.Nq + qrow];
     float x2 = 0.f;
-    f32x16 dq1[D / 32], dq2[D / 32];
-    clear(dq1); clear(dq2);
-    Lane fl;
-    fl.init(smem, lane);
-    Stage<D, ROWS, NT> st;
-    st.init(tid, a.k + b * a.k_b + 2 * kvh * a.k_h, a.k_n, a.k_h, a.v + b * a.v_b + kvh * a.v_h, a.v_n);
-    if (nt > 0) {
-        st.load(0, len);
-        st.write(smem);
-    }
+    f32x16 dq[2][NQ], s[2], dp;
+    clear(dq[0]); clear(dq[1]);
+    arrived();
+    dma.landed();
     __syncthreads();
-    for (int t = 0; t < nt; ++t) {
-        if (t + 1 < nt) st.load((t + 1) * ROWS, len);
-        const int k0 = t * ROWS;
-        if (q0 < a.Nq) {
-            const bool mask = k0 + ROWS > lim_lo;
-#pragma unroll 1
-            for (int r0 = 0; r0 < min(ROWS, lim_hi - k0); r0 += 32)
-                dq_step<D, F16, ROWS>(fl.at((t & 1) * TILE + r0 * 128), r0, mask, lim - k0, h, a.c2, qf, gf, lse, Dr, x2, dq1, dq2);
+    scores_dp<D, F16, ROWS>(fl, qf, gf, s, dp);
+    S::fall_behind(wave);
+    int buf = 0, ahead = S::LEAD;
+    for (int j = 0; j < nj; ++j) {
+        dma.landed();
+        if (j + S::LEAD < nj) dma.issue(lds0 + ahead * TILE, (j + S::LEAD) * ROWS, len);
+        ahead = S::next(ahead);
+        if (j * 32 + 32 > lim_lo) mask_keys(s, lim - j * 32, h);
+        float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][r], a.c2, -hi0));
+            const float p2 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[1][r], a.c2, -hi1));
+            part[r & 3] = __builtin_fmaf(p2, dp[r], part[r & 3]);
+            s[0][r] = p1 * (dp[r] - D0);
+            s[1][r] = p2 * (dp[r] - D1);
         }
-        if (t + 1 < nt) st.write(smem + ((t + 1) & 1) * TILE);
+        x2 += (part[0] + part[1]) + (part[2] + part[3]);
+        bf16x8 ds[2][2];
+        pack2maps<F16>(s, ds);
+        __syncthreads();
+        __builtin_amdgcn_s_setprio(1);
+        {
+            const Lane f = fl.at(buf * TILE);
+            constexpr int N = 4 * NQ, AHEAD = 4;                          // (map, sixteen keys, 32 columns)
+            auto frag = [&](int n) { return f.template cols32<ROWS>(16 * (n / NQ % 2), n / (2 * NQ) * D + n % NQ * 32); };
+            bf16x8 x[AHEAD];
+#pragma unroll
+            for (int n = 0; n < AHEAD; ++n) x[n] = frag(n);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                f32x16& acc = dq[n / (2 * NQ)][n % NQ];
+                acc = mfma32<F16>(x[n % AHEAD], ds[n / (2 * NQ)][n / NQ % 2], acc);
+                if (n + AHEAD < N) x[n % AHEAD] = frag(n + AHEAD);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        buf = S::next(buf);
+        scores_dp<D, F16, ROWS>(fl.at(buf * TILE), qf, gf, s, dp);
+        __builtin_amdgcn_s_setprio(0);
         __syncthreads();
     }
+    S::wait_for_late(wave);
     if (query >= a.Nq) return;
     const float down = F16 ? 1.0f / (1 << SHIFT16) : 1.0f, mul = a.scale * down;
+    const float un0 = __builtin_amdgcn_exp2f(-ls[2 * a.Nq]), un1 = __builtin_amdgcn_exp2f(-ls[3 * a.Nq]);
     x2 += __shfl_xor(x2, 32, 64);
-    if (h == 0) a.x2[bh * a.Nq + query] = x2 * down * unlo[1];
+    if (h == 0) a.x2[bh * a.Nq + query] = x2 * down * un1;
     bf16_t* p = a.dq + (((long)b * a.Nq + query) * a.H + head) * 2 * D;
-    store_rows<F16>(p, dq1, mul * unlo[0], h);
-    store_rows<F16>(p + D, dq2, -a.lam[head * a.lam_stride] * mul * unlo[1], h);
+    store_rows<F16>(p, dq[0], mul * un0, h);
+    store_rows<F16>(p + D, dq[1], -a.lam[head * a.lam_stride] * mul * un1, h);
 }
 
-// dK, dV: keys stay, the queries of every head of the group stream.  At d = 128 the accumulators of both do not fit a lane's registers: two
-// blocks then, one for dV (WHAT 1), one for dK (WHAT 2); else one for both (WHAT 3).
-template <int D, bool F16, int ROWS, int WHAT>
-__device__ __forceinline__ void dkv_step(const Lane& f, const float* rc, int r0, bool mask, int vis, int h, float c2, float lam, const bf16x8 (&kf)[2][D / 16],
-                                         const bf16x8 (&vf)[D / 8], f32x16 (&dk1)[D / 32], f32x16 (&dk2)[D / 32], f32x16 (&dv)[D / 16]) {
-    f32x16 s[2] = {zero16(), zero16()}, dp = zero16();
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) s[i] = mfma32<F16>(f.template rows16<ROWS>(i * D + ks * 16), kf[i][ks], s[i]);
-    if (WHAT & 2) {
-#pragma unroll
-        for (int ks = 0; ks < D / 8; ++ks) dp = mfma32<F16>(f.template rows16<ROWS>(2 * D + ks * 16), vf[ks], dp);
-    }
-    if (mask) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[i][r] = r0 + acc_row(r, h) >= vis ? s[i][r] : -__builtin_inff();
-    }
-    f32x16 pc;
+// dK, dV: keys stay, the queries of every head of the group stream.  With the constants of a row (row_constants)
+//   P1 = 2^(c2 s1 - e1),  P2' = |lam| P2 = 2^(c2 s2 - e2),  dP' = dP - D_1 (which the accumulator starts from),
+//   dS1 = P1 dP',  dS2 = sign(lam) P2' (D_2 - D_1 - dP')
+template <bool F16>
+__device__ __forceinline__ void dkv_weights(const float* rc, int h, float c2, float sign, f32x16 (&s)[2], const f32x16& dp, bf16x8 (&pc)[2], bf16x8 (&ds)[2][2]) {
+    f32x16 p;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-        const int at = r0 + 8 * g + 4 * h;                                // rows of registers 4 g .. 4 g + 3
-        const f32x4 e1 = *(const f32x4*)(rc + at), e2 = *(const f32x4*)(rc + ROWS + at);
-        f32x4 d1, d2;
-        if (WHAT & 2) { d1 = *(const f32x4*)(rc + 2 * ROWS + at); d2 = *(const f32x4*)(rc + 3 * ROWS + at); }
+        const int at = 8 * g + 4 * h;                                     // rows of registers 4 g .. 4 g + 3
+        const f32x4 e1 = *(const f32x4*)(rc + at), e2 = *(const f32x4*)(rc + 32 + at), dd = *(const f32x4*)(rc + 96 + at);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int r = 4 * g + e;
-            float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][r], c2, -e1[e]));
-            float p2 = lam * __builtin_amdgcn_exp2f(__builtin_fmaf(s[1][r], c2, -e2[e]));
-            pc[r] = p1 - p2;
-            if (WHAT & 2) {
-                s[0][r] = p1 * (dp[r] - d1[e]);
-                s[1][r] = p2 * (d2[e] - dp[r]);
-            }
+            const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][r], c2, -e1[e]));
+            const float p2 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[1][r], c2, -e2[e]));
+            p[r] = __builtin_fmaf(p2, -sign, p1);
+            s[0][r] = p1 * dp[r];
+            s[1][r] = p2 * __builtin_fmaf(dp[r], -sign, dd[e]);
         }
     }
+    pc[0] = pack8<F16>(p, 0); pc[1] = pack8<F16>(p, 1);
+    pack2maps<F16>(s, ds);
+}
+__device__ __forceinline__ f32x16 row_start(const float* rc, int h) {
+    f32x16 d;
 #pragma unroll
-    for (int sp = 0; sp < 2; ++sp) {
-        if (WHAT & 1) {
-            const bf16x8 p = pack8<F16>(pc, sp);
+    for (int g = 0; g < 4; ++g) {
+        const f32x4 t = *(const f32x4*)(rc + 64 + 8 * g + 4 * h);
 #pragma unroll
-            for (int db = 0; db < D / 16; ++db) dv[db] = mfma32<F16>(f.template cols32<ROWS>(16 * sp, 2 * D + db * 32), p, dv[db]);
-        }
-        if (WHAT & 2) {
-            const bf16x8 d1 = pack8<F16>(s[0], sp), d2 = pack8<F16>(s[1], sp);
-#pragma unroll
-            for (int db = 0; db < D / 32; ++db) {
-                dk1[db] = mfma32<F16>(f.template cols32<ROWS>(16 * sp, db * 32), d1, dk1[db]);
-                dk2[db] = mfma32<F16>(f.template cols32<ROWS>(16 * sp, D + db * 32), d2, dk2[db]);
-            }
-        }
+        for (int e = 0; e < 4; ++e) d[4 * g + e] = t[e];
     }
+    return d;
+}
+__device__ __forceinline__ void mask_queries(f32x16 (&s)[2], int vis, int h) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[i][r] = acc_row(r, h) >= vis ? s[i][r] : -__builtin_inff();
 }
 
-template <int D, bool F16, int NW, int WHAT>
-__global__ __launch_bounds__(NW * 64, 1) void diff_dkv_kernel(Args a) {
-    constexpr int ROWS = 64, TILE = ROWS * D * 8, NT = NW * 64;
-    extern __shared__ __attribute__((aligned(16))) char smem[];           // two tiles
-    __shared__ __attribute__((aligned(16))) float rc[2][4 * ROWS];        // the tile's rows: lse of both maps, D of both
+// At d = 64 the wave's keys lie in LDS and its values in registers: all of both would leave the fragments no room in the 256 registers of two waves
+// a SIMD.
+template <int D, bool F16>
+__global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void diff_dkv_kernel(Args a) {
+    typedef Sweep<D> S;
+    constexpr int ROWS = S::ROWS, TILE = S::TILE, NW = S::NW, KEYS = S::OWN, NBUF = S::BUFS, NEVER = 0x7fffffff, NQ = D / 32;
+    constexpr bool KLDS = D == 64;
+    extern __shared__ __attribute__((aligned(16))) char smem[];           // NBUF tiles, NBUF row constants, the block's keys
     const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, c = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int nblk = (a.Nk + NW * 32 - 1) / (NW * 32);
+    const int nblk = (a.Nk + KEYS - 1) / KEYS;
     int id = block_order();
     const int blk = id % nblk;                                            // under a causal mask the first keys have most to do: first
     id /= nblk;
     const int kvh = id % a.Hkv, b = id / a.Hkv;
     const int len = key_count(a, b), start = first_pos(a, b);
-    const int kb = blk * (NW * 32), k0 = kb + wave * 32, key = k0 + c, krow = min(key, a.Nk - 1);
+    const int kb = blk * KEYS, k0 = kb + wave * 32, key = k0 + c;
     // first query that sees the block's first key; the tiles of a head begin at its tile
-    const int qfirst = a.causal ? max(0, kb - start) : 0;
-    const int t0 = qfirst / ROWS, per = kb < len ? max(0, (a.Nq + ROWS - 1) / ROWS - t0) : 0, nt = per * a.G;
-    // query rows that see the lane's key: those from vis on (none where the key does not count)
-    const int vis = key >= len ? 0x7fffffff : a.causal ? key - start : -(1 << 30);
-    const int vis_all = k0 + 31 >= len ? 0x7fffffff : a.causal ? k0 + 31 - start : -(1 << 30);      // ... that see all of the wave's
-    const int vis_any = k0 >= len ? 0x7fffffff : a.causal ? k0 - start : -(1 << 30);
+    const int t0 = (a.causal ? max(0, kb - start) : 0) / ROWS, qt = (a.Nq + ROWS - 1) / ROWS;
+    const int per = kb < len ? max(0, qt - t0) : 0, nj = per * a.G;
+    // first query row that sees a key (NEVER: the key does not count)
+    auto sees = [&](int key) { return key >= len ? NEVER : a.causal ? key - start : -(1 << 30); };
+    const int vis = sees(key), vis_all = sees(k0 + 31);
 
+    const unsigned lds0 = lds_addr(smem);
+    float* const rc = (float*)(smem + NBUF * TILE);                       // [NBUF][e1, e2, -D_1, sign (D_2 - D_1)][32]
+    char* const own = smem + NBUF * (TILE + 512) + wave * (32 * D * 4);
+    Lane fl, ol;
+    fl.init(smem, lane);
+    ol.init(own, lane);
+    Dma<D, 2 * D, ROWS, NW> dma;
+    auto send = [&](int t) {                                              // tile t of the block's list
+        const int buf = t % NBUF, g = t / per, head = kvh * a.G + g, tq = t0 + t - g * per;
+        dma.init(wave, lane, a.q + b * a.q_b + 2 * head * a.q_h, a.q_n, a.q_h, a.go + b * a.go_b + head * a.go_h, a.go_n);
+        dma.issue(lds0 + buf * TILE, tq * ROWS, a.Nq);
+        if (wave < 2) {
+            const u32x4 r = Dma<D, 2 * D, ROWS, NW>::resource((const char*)(a.rc + (((long)b * a.H + head) * qt + tq) * 128));
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+                         :: "s"(__builtin_amdgcn_readfirstlane(lds0 + NBUF * TILE + buf * 512 + wave * 256)), "v"(tid * 4), "s"(r) : "memory");
+        }
+    };
+    for (int t = 0; t < min(S::LEAD, nj); ++t) send(t);
     bf16x8 kf[2][D / 16], vf[D / 8];
     {
         // (keys that do not count are not touched: their rows are cleared, so that nothing they hold can come through a product)
         const bf16x8 none = {0, 0, 0, 0, 0, 0, 0, 0};
+        const long krow = min(key, a.Nk - 1);
         const bf16_t* kp = a.k + b * a.k_b + krow * a.k_n + 2 * kvh * a.k_h + 8 * h;
         const bf16_t* vp = a.v + b * a.v_b + krow * a.v_n + kvh * a.v_h + 8 * h;
         const bool counts = key < len;
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int ks = 0; ks < D / 16; ++ks) { kf[i][ks] = none; if (counts) kf[i][ks] = load8(kp + i * a.k_h + ks * 16); }
-        if (WHAT & 2) {
+            for (int ks = 0; ks < D / 16; ++ks) {
+                bf16x8 x = none;
+                if (counts) x = load8(kp + i * a.k_h + ks * 16);
+                const int col = i * D + ks * 16;
+                if (KLDS) *(bf16x8*)(own + (col >> 6) * (32 * 128) + offR(c, ((col & 63) >> 3) + h)) = x;
+                else kf[i][ks] = x;
+            }
 #pragma unroll
-            for (int ks = 0; ks < D / 8; ++ks) { vf[ks] = none; if (counts) vf[ks] = load8(vp + ks * 16); }
-        }
+        for (int ks = 0; ks < D / 8; ++ks) { vf[ks] = none; if (counts) vf[ks] = load8(vp + ks * 16); }
     }
-    f32x16 dk1[D / 32], dk2[D / 32], dv[D / 16];
-    clear(dk1); clear(dk2); clear(dv);
-    constexpr float UP = F16 ? SHIFT16 : 0;
-    Lane fl;
-    fl.init(smem, lane);
-    Stage<D, ROWS, NT> st;
-    float rr[4 * ROWS / NT];
-    auto fetch = [&](int t) {
-        const int head = kvh * a.G + t / per, q0 = (t0 + t % per) * ROWS;
-        st.init(tid, a.q + b * a.q_b + 2 * head * a.q_h, a.q_n, a.q_h, a.go + b * a.go_b + head * a.go_h, a.go_n);
-        st.load(q0, a.Nq);
-        const long bh = ((long)b * a.H + head) * a.Nq;
+    f32x16 dk[2][NQ], dv[2 * NQ], s[2], dp;
+    clear(dk[0]); clear(dk[1]); clear(dv);
+    auto next_scores = [&](int buf) {
+        const Lane f = fl.at(buf * TILE);
+        constexpr int N = D / 4, AHEAD = KLDS ? 2 : 4;
+        dp = row_start(rc + buf * 128, h);
+        bf16x8 x[AHEAD], y[AHEAD];
 #pragma unroll
-        for (int i = 0; i < 4 * ROWS / NT; ++i) {
-            const int j = i * NT + tid, which = j / ROWS, n = q0 + j % ROWS;
-            rr[i] = which < 2 ? __builtin_inff() : 0.f;                   // a row behind the last: P = 0
-            if (n < a.Nq) rr[i] = which < 2 ? a.lse[bh * 4 + which * a.Nq + n] + (a.lse[bh * 4 + (2 + which) * a.Nq + n] - UP) : a.D[bh * 2 + (which - 2) * a.Nq + n];
+        for (int n = 0; n < AHEAD; ++n) { x[n] = f.template rows16<ROWS>(n * 16); if (KLDS) y[n] = ol.template rows16<32>(n * 16); }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int i = n / (D / 16), ks = n % (D / 16);
+            if (i < 2) s[i & 1] = mfma32<F16>(x[n % AHEAD], KLDS ? y[n % AHEAD] : kf[i & 1][ks], ks ? s[i & 1] : zero16());
+            else dp = mfma32<F16>(x[n % AHEAD], vf[n - D / 8], dp);
+            if (n + AHEAD < N) {
+                x[n % AHEAD] = f.template rows16<ROWS>((n + AHEAD) * 16);
+                if (KLDS && n + AHEAD < D / 8) y[n % AHEAD] = ol.template rows16<32>((n + AHEAD) * 16);
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
-    auto put = [&](int s) {
-        st.write(smem + s * TILE);
-#pragma unroll
-        for (int i = 0; i < 4 * ROWS / NT; ++i) rc[s][i * NT + tid] = rr[i];
-    };
-    if (nt > 0) {
-        fetch(0);
-        put(0);
-    }
+    arrived();
+    dma.landed();
     __syncthreads();
-    for (int t = 0; t < nt; ++t) {
-        const float* r = rc[t & 1];
-        if (t + 1 < nt) fetch(t + 1);
-        const int q0 = (t0 + t % per) * ROWS;
-        const float lam = a.lam[(kvh * a.G + t / per) * a.lam_stride];
-        const bool mask = q0 < vis_all;
-        const int v = vis == 0x7fffffff ? vis : vis - q0;
-#pragma unroll 1
-        for (int r0 = 0; r0 < ROWS; r0 += 32)
-            if (q0 + r0 + 31 >= vis_any) dkv_step<D, F16, ROWS, WHAT>(fl.at((t & 1) * TILE + r0 * 128), r, r0, mask, v, h, a.c2, lam, kf, vf, dk1, dk2, dv);
-        if (t + 1 < nt) put((t + 1) & 1);
+    next_scores(0);                                                       // (without a tile, or behind the last: of what lies there, not used)
+    S::fall_behind(wave);
+    int buf = 0, g = 0, tq = t0;
+    float sign = copysignf(1.0f, a.lam[kvh * a.G * a.lam_stride]);
+    for (int j = 0; j < nj; ++j) {
+        dma.landed();
+        if (j + S::LEAD < nj) send(j + S::LEAD);
+        if (tq * ROWS < vis_all) mask_queries(s, vis == NEVER ? NEVER : vis - tq * ROWS, h);
+        bf16x8 pc[2], ds[2][2];
+        dkv_weights<F16>(rc + buf * 128, h, a.c2, sign, s, dp, pc, ds);
+        __syncthreads();
+        __builtin_amdgcn_s_setprio(1);
+        {
+            const Lane f = fl.at(buf * TILE);
+            constexpr int N = 8 * NQ, AHEAD = 4;                          // (sixteen queries, 32 columns of [q1 | q2 | dO])
+            auto frag = [&](int n) { return f.template cols32<ROWS>(16 * (n / (4 * NQ)), n % (4 * NQ) * 32); };
+            bf16x8 x[AHEAD];
+#pragma unroll
+            for (int n = 0; n < AHEAD; ++n) x[n] = frag(n);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                const int sp = n / (4 * NQ), cb = n % (4 * NQ);
+                f32x16& acc = cb < 2 * NQ ? dk[cb / NQ % 2][cb % NQ] : dv[cb < 2 * NQ ? 0 : cb - 2 * NQ];
+                acc = mfma32<F16>(x[n % AHEAD], cb < 2 * NQ ? ds[cb / NQ % 2][sp] : pc[sp], acc);
+                if (n + AHEAD < N) x[n % AHEAD] = frag(n + AHEAD);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        buf = S::next(buf);
+        if (++tq == qt) {
+            tq = t0;
+            if (++g < a.G) sign = copysignf(1.0f, a.lam[(kvh * a.G + g) * a.lam_stride]);
+        }
+        next_scores(buf);
+        __builtin_amdgcn_s_setprio(0);
         __syncthreads();
     }
+    S::wait_for_late(wave);
     if (key >= a.Nk) return;
     const float down = F16 ? 1.0f / (1 << SHIFT16) : 1.0f;
     const long row = ((long)b * a.Nk + key) * a.Hkv + kvh;
-    if (WHAT & 1) store_rows<F16>(a.dv + row * 2 * D, dv, down, h);
-    if (WHAT & 2) {
-        store_rows<F16>(a.dk + row * 2 * D, dk1, a.scale * down, h);
-        store_rows<F16>(a.dk + row * 2 * D + D, dk2, a.scale * down, h);
-    }
+    store_rows<F16>(a.dv + row * 2 * D, dv, down, h);
+    store_rows<F16>(a.dk + row * 2 * D, dk[0], a.scale * down, h);
+    store_rows<F16>(a.dk + row * 2 * D + D, dk[1], a.scale * down, h);
 }
 
 // dlam[h] = - sum over entries and queries of D_2 (all heads for one shared lam): a block each, in a fixed order, summed in 64 bits
@@ -733,6 +906,8 @@ int check(const hs_diff_attn_desc* d, bool backward) {
     if ((int64_t)d->B * d->H * (((int64_t)(d->Nq > d->Nk ? d->Nq : d->Nk) + 127) / 128) > (1 << 30)) return HS_ERR_SHAPE;
     for (int64_t s : {d->q_b, d->q_n, d->q_h, d->k_b, d->k_n, d->k_h, d->v_b, d->v_n, d->v_h})
         if (s < 0 || (s & 7)) return HS_ERR_SHAPE;
+    for (int64_t s : {d->q_n, d->q_h, d->k_n, d->k_h, d->v_n, d->v_h, backward ? d->go_n : 0, backward ? d->go_h : 0})
+        if (s > (1 << 24)) return HS_ERR_SHAPE;                            // a tile's 32 rows lie inside a buffer descriptor's 2 GiB
     if (backward)
         for (int64_t s : {d->go_b, d->go_n, d->go_h})
             if (s < 0 || (s & 7)) return HS_ERR_SHAPE;
@@ -752,7 +927,7 @@ Split split_of(const hs_diff_attn_desc* d) {
     return {(int)tiles, (int)((d->Nk + chunk - 1) / chunk), (int)chunk};
 }
 size_t split_bytes(const hs_diff_attn_desc* d, const Split& s) {
-    return s.nsplit > 1 ? (size_t)d->B * d->Hkv * s.tiles * s.nsplit * 2 * 32 * (2 * d->d + 2) * 4 : 0;
+    return s.nsplit > 1 ? (size_t)d->B * d->Hkv * s.tiles * s.nsplit * 2 * 32 * (2 * d->d + 4) * 4 : 0;
 }
 Args args_of(const hs_diff_attn_desc* d) {
     Args a = {};
@@ -767,27 +942,24 @@ template <class K> void launch(K kernel, int64_t grid, int threads, size_t lds, 
     if (lds > 60000) (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(threads), lds, s, a);
 }
-template <int D, bool F16> void forward(const Args& a, const Split& sp, hipStream_t s) {
+template <int D, bool F16, bool KEEP> void forward(const Args& a, const Split& sp, hipStream_t s) {
+    typedef Sweep<D> S;
+    constexpr int TILE = S::ROWS * (2 * D + S::VC) * 2;
     if (sp.nsplit) {
-        constexpr int NW = 4;
-        launch(diff_split_kernel<D, F16, NW>, (int64_t)a.B * a.Hkv * sp.tiles * sp.nsplit, NW * 64, (size_t)NW * 256 * D, s, a);
+        constexpr int NW = D == 128 ? 2 : 4;
+        launch(diff_split_kernel<D, F16, KEEP, NW>, (int64_t)a.B * a.Hkv * sp.tiles * sp.nsplit * S::HALVES, NW * 64, (size_t)NW * 2 * TILE, s, a);
         if (sp.nsplit > 1) launch(diff_join_kernel<D, F16>, ((int64_t)a.B * a.H * a.Nq + 3) / 4, 256, 0, s, a);
         return;
     }
-    constexpr int NW = D == 128 ? 4 : 8;
-    launch(diff_fwd_kernel<D, F16, NW>, (int64_t)a.B * a.H * ((a.Nq + NW * 32 - 1) / (NW * 32)), NW * 64, (size_t)2 * (D == 128 ? 32 : 64) * D * 8, s, a);
+    launch(diff_fwd_kernel<D, F16, KEEP>, (int64_t)a.B * a.H * ((a.Nq + S::OWN - 1) / S::OWN) * S::HALVES, S::NW * 64, (size_t)S::BUFS * TILE, s, a);
 }
 template <int D, bool F16> void backward(const Args& a, hipStream_t s) {
-    constexpr int LANES = D / 4, NW = D == 128 ? 4 : 8;
-    launch(diff_rows_kernel<D, F16>, ((int64_t)a.B * a.Nq * a.H * LANES + 255) / 256, 256, 0, s, a);
-    launch(diff_dq_kernel<D, F16, NW>, (int64_t)a.B * a.H * ((a.Nq + NW * 32 - 1) / (NW * 32)), NW * 64, (size_t)2 * 64 * D * 8, s, a);
-    const int64_t blocks = (int64_t)a.B * a.Hkv * ((a.Nk + 127) / 128);
-    if constexpr (D == 128) {
-        launch(diff_dkv_kernel<D, F16, 4, 1>, blocks, 256, (size_t)2 * 64 * D * 8, s, a);
-        launch(diff_dkv_kernel<D, F16, 4, 2>, blocks, 256, (size_t)2 * 64 * D * 8, s, a);
-    } else {
-        launch(diff_dkv_kernel<D, F16, 4, 3>, blocks, 256, (size_t)2 * 64 * D * 8, s, a);
-    }
+    typedef Sweep<D> S;
+    constexpr int LANES = D / 4;
+    launch(diff_rows_kernel<D, F16>, ((int64_t)a.B * ((a.Nq + 31) / 32 * 32) * a.H * LANES + 255) / 256, 256, 0, s, a);
+    launch(diff_dq_kernel<D, F16>, (int64_t)a.B * a.H * ((a.Nq + S::OWN - 1) / S::OWN), S::NW * 64, (size_t)S::BUFS * S::TILE, s, a);
+    launch(diff_dkv_kernel<D, F16>, (int64_t)a.B * a.Hkv * ((a.Nk + S::OWN - 1) / S::OWN), S::NW * 64,
+           (size_t)S::BUFS * (S::TILE + 512) + (D == 64 ? S::OWN * D * 4 : 0), s, a);
 }
 #define HS_BY_TYPE(call)                                                               \
     do {                                                                               \
@@ -800,7 +972,7 @@ template <int D, bool F16> void backward(const Args& a, hipStream_t s) {
 }  // namespace
 
 extern "C" size_t hs_diff_attn_fwd_ws_bytes(const hs_diff_attn_desc* d) { return check(d, false) == HS_OK ? split_bytes(d, split_of(d)) : 0; }
-extern "C" size_t hs_diff_attn_bwd_ws_bytes(const hs_diff_attn_desc* d) { return check(d, false) == HS_OK ? (size_t)d->B * d->H * d->Nq * 12 : 0; }
+extern "C" size_t hs_diff_attn_bwd_ws_bytes(const hs_diff_attn_desc* d) { return check(d, false) == HS_OK ? (size_t)d->B * d->H * (d->Nq * 12 + (size_t)((d->Nq + 31) / 32) * 512) : 0; }
 
 extern "C" int hs_diff_attn_fwd(const hs_diff_attn_desc* d, const void* q, const void* k, const void* v, const float* lam, const int32_t* q_start,
                                 const int32_t* kv_len, void* o, void* maps, float* lse, void* ws, size_t ws_bytes, void* stream) {
@@ -816,7 +988,7 @@ extern "C" int hs_diff_attn_fwd(const hs_diff_attn_desc* d, const void* q, const
     a.o = (bf16_t*)o; a.maps = (bf16_t*)maps; a.lse = lse; a.part = (float*)ws;
     a.tiles = sp.tiles; a.nsplit = sp.nsplit; a.chunk = sp.chunk;
     hipStream_t s = (hipStream_t)stream;
-#define CALL(D, F) forward<D, F>(a, sp, s)
+#define CALL(D, F) maps ? forward<D, F, true>(a, sp, s) : forward<D, F, false>(a, sp, s)
     HS_BY_TYPE(CALL);
 #undef CALL
     HS_CHECK_LAUNCH();
@@ -836,6 +1008,7 @@ extern "C" int hs_diff_attn_bwd(const hs_diff_attn_desc* d, const void* q, const
     a.q = (const bf16_t*)q; a.k = (const bf16_t*)k; a.v = (const bf16_t*)v; a.go = (const bf16_t*)d_o; a.lam = lam;
     a.q_start = q_start; a.kv_len = kv_len; a.maps = (bf16_t*)maps; a.lse = (float*)lse;
     a.D = (float*)ws; a.x2 = a.D + (size_t)d->B * d->H * 2 * d->Nq;
+    a.rc = a.x2 + (size_t)d->B * d->H * d->Nq;
     a.dq = (bf16_t*)dq; a.dk = (bf16_t*)dk; a.dv = (bf16_t*)dv;
     hipStream_t s = (hipStream_t)stream;
 #define CALL(D, F) backward<D, F>(a, s)

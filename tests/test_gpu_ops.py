@@ -171,11 +171,12 @@ def diff_reference(q, k, v, lam, go, scale, causal, start, lens):
     return {n: (r[n], t[n] * 1.01 + 1e-30) for n in r}
 
 
-def diff_case(seed, B, Nq, Nk, Hq, Hkv, d, dtype, causal=False, lens=None, start=None, lam="heads", scale=None, size=1.0):
+def diff_case(seed, B, Nq, Nk, Hq, Hkv, d, dtype, causal=False, lens=None, start=None, lam="heads", scale=None, size=1.0, grow=1.0):
     g = torch.Generator("cuda").manual_seed(seed)
     q, k = rnd(g, B, Nq, 2 * Hq, d, dtype=dtype, scale=size), rnd(g, B, Nk, 2 * Hkv, d, dtype=dtype)
     v, go = rnd(g, B, Nk, Hkv, 2 * d, dtype=dtype), rnd(g, B, Nq, Hq, 2 * d, dtype=dtype)
     lm = torch.rand(Hq, generator=g, device="cuda") * 1.4 - 0.2 if lam == "heads" else torch.full((1,) if lam == "one" else (), 0.4, device="cuda")
+    k[:, Nk // 2:] *= grow                                  # scores that leave the first ones far behind
     it = lambda x: None if x is None else torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
     starts = start if start is not None else [Nk - Nq] * B
     ref = diff_reference(q, k, v, lm, go, d ** -0.5 if scale is None else scale, causal, starts, lens)
@@ -197,6 +198,8 @@ def run_diff(q, k, v, lam, go, kw):
     dict(B=3, Nq=40, Nk=200, Hq=2, Hkv=2, d=128, dtype=F16, lens=[0, 1, 200]), dict(B=2, Nq=300, Nk=129, Hq=2, Hkv=1, d=64, dtype=BF, causal=True, start=[-40, 100]),
     dict(B=1, Nq=129, Nk=577, Hq=1, Hkv=1, d=64, dtype=F16, scale=0.3), dict(B=1, Nq=70, Nk=190, Hq=2, Hkv=1, d=64, dtype=BF, size=12.0),
     dict(B=1, Nq=33, Nk=64, Hq=8, Hkv=2, d=128, dtype=BF), dict(B=2, Nq=1025, Nk=1025, Hq=1, Hkv=1, d=32, dtype=BF, causal=True),
+    dict(B=1, Nq=300, Nk=200, Hq=1, Hkv=1, d=64, dtype=BF, grow=36.0), dict(B=1, Nq=70, Nk=333, Hq=2, Hkv=1, d=32, dtype=F16, grow=36.0),
+    dict(B=1, Nq=140, Nk=150, Hq=1, Hkv=1, d=128, dtype=F16, grow=20.0, causal=True), dict(B=1, Nq=5, Nk=3000, Hq=1, Hkv=1, d=64, dtype=F16, grow=36.0),
     # few queries: the keys are cut and joined
     dict(B=2, Nq=1, Nk=255, Hq=4, Hkv=2, d=64, dtype=BF, causal=True), dict(B=2, Nq=1, Nk=257, Hq=8, Hkv=1, d=64, dtype=F16, lens=[256, 257]),
     dict(B=3, Nq=1, Nk=5000, Hq=4, Hkv=2, d=64, dtype=BF, lens=[0, 1, 4999], causal=True, start=[5, 0, 4998]),
@@ -212,6 +215,17 @@ def test_diff_attention_values_and_gradients(dev, case):
         assert torch.equal(H.diff_attention(*ins[:4], **kw), got["o"])       # without a graph: the same bits
     again = run_diff(*ins, kw)
     assert all(torch.equal(got[n], again[n]) for n in got)                    # no atomics
+
+
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("Nq", [1, 200])
+def test_diff_one_visible_key_gives_its_value(dev, d, Nq):
+    """softmax of one key is 1, and of two equal keys a half, whatever the scores: no rounding of P may show"""
+    g = torch.Generator("cuda").manual_seed(d + Nq)
+    q, k, v = rnd(g, 2, Nq, 4, d, dtype=BF), rnd(g, 2, 300, 4, d, dtype=BF), rnd(g, 2, 300, 2, 2 * d, dtype=BF)
+    k[1, 1], v[1, 1] = k[1, 0], v[1, 0]
+    o = H.diff_attention(q, k, v, torch.tensor([0.5, 0.0], device="cuda"), kv_len=torch.tensor([1, 2], dtype=torch.int32, device="cuda"))
+    assert torch.equal(o[:, :, 0], (0.5 * v[:, :1, 0]).expand_as(o[:, :, 0])) and torch.equal(o[:, :, 1], v[:, :1, 1].expand_as(o[:, :, 1]))
 
 
 def test_diff_gradient_against_differences(dev):
