@@ -54,12 +54,13 @@ template <int D, int VC, int ROWS, int NW> struct Dma {
     static constexpr int PAIRS = D / 32, IMAGES = PAIRS + VC / 64, GROUPS = ROWS / 8, PER = IMAGES * GROUPS / NW;
     static_assert(PER * NW == IMAGES * GROUPS && (NW == 1 || NW % GROUPS == 0), "whole pieces");
     static constexpr int BASES = NW == 1 ? 2 : 1;                         // a lone wave moves even and odd groups of 8 rows, whose swizzles differ
-    const char *x, *y;
+    const char *x, *y;                         // the next tile's first row
     long x_n, y_n, x_h;
-    int wave, row;
+    int wave, row, left;                       // rows left from there on
     unsigned vx[BASES], vy[BASES];             // byte offsets of the lane's chunk in image 0 of the pair and of the values
-    __device__ __forceinline__ void init(int wave_, int lane, const bf16_t* x_, long x_n_, long x_h_, const bf16_t* y_, long y_n_) {
-        x = (const char*)x_; y = (const char*)y_; x_n = x_n_ * 2; y_n = y_n_ * 2; x_h = x_h_ * 2; wave = wave_;
+    __device__ __forceinline__ void init(int wave_, int lane, const bf16_t* x_, long x_n_, long x_h_, const bf16_t* y_, long y_n_, int first, int end) {
+        x_n = x_n_ * 2; y_n = y_n_ * 2; x_h = x_h_ * 2; wave = wave_;
+        start(x_, y_, first, end);
         row = wave % GROUPS * 8 + (lane >> 3);
 #pragma unroll
         for (int i = 0; i < BASES; ++i) {
@@ -68,19 +69,29 @@ template <int D, int VC, int ROWS, int NW> struct Dma {
             vy[i] = (unsigned)(row * y_n + ch * 16);
         }
     }
+    __device__ __forceinline__ void start(const bf16_t* x_, const bf16_t* y_, int first, int end) {
+        x = (const char*)x_ + first * x_n;
+        y = (const char*)y_ + first * y_n;
+        left = end - first;
+    }
+    __device__ __forceinline__ void skip(int rows) {
+        x += rows * x_n;
+        y += rows * y_n;
+        left -= rows;
+    }
     static __device__ __forceinline__ u32x4 resource(const char* p) {
         const unsigned long long a = (unsigned long long)p;
         return u32x4{(unsigned)__builtin_amdgcn_readfirstlane((unsigned)a), (unsigned)__builtin_amdgcn_readfirstlane((unsigned)(a >> 32)), HS_MAX_RECORDS, 0x00020000u};
     }
-    __device__ __forceinline__ void issue(unsigned lds, int first, int end) const {      // rows at or behind `end` become zeros, and are not touched
-        const u32x4 rx = resource(x + first * x_n), ry = resource(y + first * y_n);
+    __device__ __forceinline__ void issue(unsigned lds) const {           // rows at or behind `end` become zeros, and are not touched
+        const u32x4 rx = resource(x), ry = resource(y);
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const int g = i * NW + wave, image = g / GROUPS, group = g % GROUPS, more = NW == 1 ? group * 8 : 0;
             const bool pair = image < PAIRS;
             const int im = pair ? image : image - PAIRS;
             unsigned off = pair ? vx[BASES == 2 ? i & 1 : 0] : vy[BASES == 2 ? i & 1 : 0];
-            off = first + row + more < end ? off : HS_OOB_OFF;
+            off = row + more < left ? off : HS_OOB_OFF;
             const unsigned so = (unsigned)(pair ? more * x_n + (D == 32 ? 0 : D == 64 ? im * x_h : (im >> 1) * x_h + (im & 1) * 128) : more * y_n + im * 128);
             const unsigned at = lds + image * (ROWS * 128) + group * 1024;
             asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
@@ -273,13 +284,23 @@ __device__ __forceinline__ void values(const Lane& f, const bf16x8 (&p)[2][2], f
 // other has the matrix pipe (left to themselves both do the same thing at the same time).  At d = 128 a SIMD's registers hold one wave only, and the
 // forward pass' numerators of half of the values: two blocks then, each with the scores of all.
 // Tile t is first read in the matrix phase of step t - 1 and left in step t's, half a step later by the later waves: it is sent for in step t - LEAD
-// into the buffer of tile t - BUFS, and has landed (every wave waits for its own part) in the vector phase of the next step.
+// into the buffer of tile t - BUFS.
 template <int D> struct Sweep {
     static constexpr bool PAIRED = D < 128;
     static constexpr int NW = PAIRED ? 8 : 4, ROWS = 32, TILE = ROWS * D * 8, HALVES = PAIRED ? 1 : 2, VC = 2 * D / HALVES, BUFS = PAIRED ? 5 : 3, LEAD = PAIRED ? 3 : 2, OWN = NW * 32;
     static __device__ __forceinline__ void fall_behind(int wave) { if (PAIRED && wave >= NW / 2) __syncthreads(); }
     static __device__ __forceinline__ void wait_for_late(int wave) { if (PAIRED && wave < NW / 2) __syncthreads(); }
     static __device__ __forceinline__ int next(int buf) { return buf == BUFS - 1 ? 0 : buf + 1; }
+    // The waits for a wave's own transfers.  Paired: at the start of a vector phase, all of them (tile j + LEAD - 1, sent for a step ago, and the next one is
+    // sent for behind the wait).  Alone, at its end, all but the youngest tile's PER instructions, or all where the list has ended; the choice is made
+    // inside the instruction text, since a branch of the program here costs copies of the accumulators.
+    template <class DMA> static __device__ __forceinline__ void before_vector() { if (PAIRED) DMA::landed(); }
+    template <class DMA> static __device__ __forceinline__ void behind_vector(bool more) {
+        if (!PAIRED)
+            asm volatile("s_cmp_eq_u32 %0, 0\n\ts_cbranch_scc1 .Lland_all%=\n\ts_waitcnt vmcnt(%1)\n\ts_branch .Lland_done%=\n"
+                         ".Lland_all%=:\n\ts_waitcnt vmcnt(0)\n.Lland_done%=:"
+                         :: "s"(__builtin_amdgcn_readfirstlane((int)more)), "i"(DMA::PER) : "memory", "scc");
+    }
 };
 
 // ---- forward ----------------------------------------------------------------------------------------------------------------------------------
@@ -307,8 +328,9 @@ __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void d
     fl.init(smem, lane);
     const unsigned lds0 = lds_addr(smem);
     Dma<D, VC, ROWS, NW> dma;
-    dma.init(wave, lane, a.k + b * a.k_b + 2 * kvh * a.k_h, a.k_n, a.k_h, a.v + b * a.v_b + kvh * a.v_h + half * VC, a.v_n);
-    for (int t = 0; t < min(S::LEAD, nj); ++t) dma.issue(lds0 + t * TILE, t * ROWS, len);
+    const bf16_t *kp = a.k + b * a.k_b + 2 * kvh * a.k_h, *vp = a.v + b * a.v_b + kvh * a.v_h + half * VC;
+    dma.init(wave, lane, kp, a.k_n, a.k_h, vp, a.v_n, 0, len);
+    for (int t = 0; t < min(S::LEAD, nj); ++t) { dma.issue(lds0 + t * TILE); dma.skip(ROWS); }
     bf16x8 qf[2][D / 16];
     {
         const bf16_t* qp = a.q + b * a.q_b + (long)min(query, a.Nq - 1) * a.q_n + 2 * head * a.q_h + 8 * h;
@@ -325,7 +347,8 @@ __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void d
     // range (fp16: 2^15, P itself; bf16: 2^40, which leaves 2^87 for the values), the block starts again and keeps a running maximum.
     for (bool running = false;; running = true) {
         if (running) {
-            for (int t = 0; t < min(S::LEAD, nj); ++t) dma.issue(lds0 + t * TILE, t * ROWS, len);
+            dma.start(kp, vp, 0, len);
+            for (int t = 0; t < min(S::LEAD, nj); ++t) { dma.issue(lds0 + t * TILE); dma.skip(ROWS); }
         }
         m[0] = m[1] = NONE;
         l[0][0] = l[1][0] = l[0][SUMS - 1] = l[1][SUMS - 1] = 0.f;
@@ -337,8 +360,9 @@ __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void d
         S::fall_behind(wave);
         int buf = 0, ahead = S::LEAD;                                     // the step's buffer, and the one to send to
         for (int j = 0; j < nj; ++j) {
-            dma.landed();
-            if (j + S::LEAD < nj) dma.issue(lds0 + ahead * TILE, (j + S::LEAD) * ROWS, len);
+            S::template before_vector<decltype(dma)>();
+            if (j + S::LEAD < nj) dma.issue(lds0 + ahead * TILE);
+            dma.skip(ROWS);
             ahead = S::next(ahead);
             if (j * 32 + 32 > lim_lo) mask_keys(s, lim - j * 32, h);
             if (j == 0 || running) {
@@ -348,6 +372,7 @@ __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void d
             bf16x8 p[2][2];
             softmax_weights<F16>(s[0], a.c2, m[0], l[0], p[0]);
             softmax_weights<F16>(s[1], a.c2, m[1], l[1], p[1]);
+            S::template behind_vector<decltype(dma)>(j + S::LEAD < nj);
             __syncthreads();
             __builtin_amdgcn_s_setprio(1);
             values<D, F16, ROWS>(fl.at(buf * TILE), p, o1, o2);
@@ -435,14 +460,15 @@ __global__ __launch_bounds__(NW * 64, 1) void diff_split_kernel(Args a) {
     Lane fl;
     fl.init(own, lane);
     Dma<D, VC, ROWS, 1> dma;
-    dma.init(0, lane, a.k + b * a.k_b + 2 * kvh * a.k_h, a.k_n, a.k_h, a.v + b * a.v_b + kvh * a.v_h + half * VC, a.v_n);
+    dma.init(0, lane, a.k + b * a.k_b + 2 * kvh * a.k_h, a.k_n, a.k_h, a.v + b * a.v_b + kvh * a.v_h + half * VC, a.v_n, k0 + wave * ROWS, len);
     arrived();
     int t = k0 + wave * ROWS, buf = 0;
-    if (t < k1) dma.issue(lds_addr(own), t, len);
+    if (t < k1) dma.issue(lds_addr(own));
     for (; t < k1; t += NW * ROWS) {
         if (t + NW * ROWS < k1) {
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");            // (the last step's reads of that buffer are over)
-            dma.issue(lds_addr(own) + (buf ^ 1) * TILE, t + NW * ROWS, len);
+            dma.skip(NW * ROWS);
+            dma.issue(lds_addr(own) + (buf ^ 1) * TILE);
             dma.template landed<Dma<D, VC, ROWS, 1>::PER>();
         } else {
             dma.landed();
@@ -562,7 +588,7 @@ __global__ __launch_bounds__(256) void diff_join_kernel(Args a) {
 
 // ---- backward ----------------------------------------------------------------------------------------------------------------------------------
 // D_m = dO . O_m, 2 d / 8 lanes a row (HBM-bound: three tensors once), and from it the constants of a row that the dk, dv sweep reads, 32 rows together:
-// the exponents' offsets of both maps (the second with lam's size in it), -D_1 and sign(lam) (D_2 - D_1); rows behind the last have P = 0.
+// the scores' offsets of both maps (the second with lam's size in it), -D_1 and sign(lam) (D_2 - D_1); rows behind the last have P = 0.
 template <int D, bool F16>
 __global__ __launch_bounds__(256) void diff_rows_kernel(Args a) {
     constexpr int LANES = D / 4;
@@ -600,7 +626,7 @@ __global__ __launch_bounds__(256) void diff_rows_kernel(Args a) {
         p[a.Nq] = d[1];
     }
     float* r = a.rc + (bh * qt + (query >> 5)) * 128 + (query & 31);
-    r[0] = e[0]; r[32] = e[1]; r[64] = -d[0]; r[96] = copysignf(1.0f, lam) * (d[1] - d[0]);
+    r[0] = -e[0] / a.c2; r[32] = -e[1] / a.c2; r[64] = -d[0]; r[96] = copysignf(1.0f, lam) * (d[1] - d[0]);
 }
 
 // dQ: queries stay, keys stream
@@ -626,8 +652,8 @@ __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void d
     fl.init(smem, lane);
     const unsigned lds0 = lds_addr(smem);
     Dma<D, 2 * D, ROWS, NW> dma;
-    dma.init(wave, lane, a.k + b * a.k_b + 2 * kvh * a.k_h, a.k_n, a.k_h, a.v + b * a.v_b + kvh * a.v_h, a.v_n);
-    for (int t = 0; t < min(S::LEAD, nj); ++t) dma.issue(lds0 + t * TILE, t * ROWS, len);
+    dma.init(wave, lane, a.k + b * a.k_b + 2 * kvh * a.k_h, a.k_n, a.k_h, a.v + b * a.v_b + kvh * a.v_h, a.v_n, 0, len);
+    for (int t = 0; t < min(S::LEAD, nj); ++t) { dma.issue(lds0 + t * TILE); dma.skip(ROWS); }
     bf16x8 qf[2][D / 16], gf[D / 8];
     {
         const bf16_t* qp = a.q + b * a.q_b + qrow * a.q_n + 2 * head * a.q_h + 8 * h;
@@ -654,8 +680,9 @@ __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void d
     S::fall_behind(wave);
     int buf = 0, ahead = S::LEAD;
     for (int j = 0; j < nj; ++j) {
-        dma.landed();
-        if (j + S::LEAD < nj) dma.issue(lds0 + ahead * TILE, (j + S::LEAD) * ROWS, len);
+        S::template before_vector<decltype(dma)>();
+        if (j + S::LEAD < nj) dma.issue(lds0 + ahead * TILE);
+        dma.skip(ROWS);
         ahead = S::next(ahead);
         if (j * 32 + 32 > lim_lo) mask_keys(s, lim - j * 32, h);
         float part[4] = {0.f, 0.f, 0.f, 0.f};
@@ -670,6 +697,7 @@ __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void d
         x2 += (part[0] + part[1]) + (part[2] + part[3]);
         bf16x8 ds[2][2];
         pack2maps<F16>(s, ds);
+        S::template behind_vector<decltype(dma)>(j + S::LEAD < nj);
         __syncthreads();
         __builtin_amdgcn_s_setprio(1);
         {
@@ -705,20 +733,18 @@ __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void d
 }
 
 // dK, dV: keys stay, the queries of every head of the group stream.  With the constants of a row (row_constants)
-//   P1 = 2^(c2 s1 - e1),  P2' = |lam| P2 = 2^(c2 s2 - e2),  dP' = dP - D_1 (which the accumulator starts from),
+//   P1 = 2^(c2 (s1 - e1)),  P2' = |lam| P2 = 2^(c2 (s2 - e2)),  dP' = dP - D_1 (the accumulators start from -e1, -e2, -D_1),
 //   dS1 = P1 dP',  dS2 = sign(lam) P2' (D_2 - D_1 - dP')
 template <bool F16>
 __device__ __forceinline__ void dkv_weights(const float* rc, int h, float c2, float sign, f32x16 (&s)[2], const f32x16& dp, bf16x8 (&pc)[2], bf16x8 (&ds)[2][2]) {
     f32x16 p;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-        const int at = 8 * g + 4 * h;                                     // rows of registers 4 g .. 4 g + 3
-        const f32x4 e1 = *(const f32x4*)(rc + at), e2 = *(const f32x4*)(rc + 32 + at), dd = *(const f32x4*)(rc + 96 + at);
+        const f32x4 dd = *(const f32x4*)(rc + 96 + 8 * g + 4 * h);        // rows of registers 4 g .. 4 g + 3
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int r = 4 * g + e;
-            const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][r], c2, -e1[e]));
-            const float p2 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[1][r], c2, -e2[e]));
+            const float p1 = __builtin_amdgcn_exp2f(s[0][r] * c2), p2 = __builtin_amdgcn_exp2f(s[1][r] * c2);
             p[r] = __builtin_fmaf(p2, -sign, p1);
             s[0][r] = p1 * dp[r];
             s[1][r] = p2 * __builtin_fmaf(dp[r], -sign, dd[e]);
@@ -731,7 +757,7 @@ __device__ __forceinline__ f32x16 row_start(const float* rc, int h) {
     f32x16 d;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-        const f32x4 t = *(const f32x4*)(rc + 64 + 8 * g + 4 * h);
+        const f32x4 t = *(const f32x4*)(rc + 8 * g + 4 * h);
 #pragma unroll
         for (int e = 0; e < 4; ++e) d[4 * g + e] = t[e];
     }
@@ -769,23 +795,38 @@ __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void d
     const int vis = sees(key), vis_all = sees(k0 + 31);
 
     const unsigned lds0 = lds_addr(smem);
-    float* const rc = (float*)(smem + NBUF * TILE);                       // [NBUF][e1, e2, -D_1, sign (D_2 - D_1)][32]
+    float* const rc = (float*)(smem + NBUF * TILE);                       // [NBUF][-e1, -e2, -D_1, sign (D_2 - D_1)][32]
     char* const own = smem + NBUF * (TILE + 512) + wave * (32 * D * 4);
     Lane fl, ol;
     fl.init(smem, lane);
     ol.init(own, lane);
     Dma<D, 2 * D, ROWS, NW> dma;
-    auto send = [&](int t) {                                              // tile t of the block's list
-        const int buf = t % NBUF, g = t / per, head = kvh * a.G + g, tq = t0 + t - g * per;
-        dma.init(wave, lane, a.q + b * a.q_b + 2 * head * a.q_h, a.q_n, a.q_h, a.go + b * a.go_b + head * a.go_h, a.go_n);
-        dma.issue(lds0 + buf * TILE, tq * ROWS, a.Nq);
+    // the block's list of tiles, head by head: what is sent next
+    int sg = 0, st = t0, sbuf = 0;
+    const char* srow = nullptr;                                           // the tile's row constants
+    auto head_start = [&]() {
+        const int head = kvh * a.G + sg;
+        dma.start(a.q + b * a.q_b + 2 * head * a.q_h, a.go + b * a.go_b + head * a.go_h, t0 * ROWS, a.Nq);
+        srow = (const char*)(a.rc + (((long)b * a.H + head) * qt + t0) * 128) + wave * 256;
+    };
+    dma.init(wave, lane, a.q, a.q_n, a.q_h, a.go, a.go_n, 0, 0);
+    head_start();
+    auto send = [&]() {
+        dma.issue(lds0 + sbuf * TILE);
         if (wave < 2) {
-            const u32x4 r = Dma<D, 2 * D, ROWS, NW>::resource((const char*)(a.rc + (((long)b * a.H + head) * qt + tq) * 128));
+            const u32x4 r = Dma<D, 2 * D, ROWS, NW>::resource(srow);
             asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
-                         :: "s"(__builtin_amdgcn_readfirstlane(lds0 + NBUF * TILE + buf * 512 + wave * 256)), "v"(tid * 4), "s"(r) : "memory");
+                         :: "s"(__builtin_amdgcn_readfirstlane(lds0 + NBUF * TILE + sbuf * 512 + wave * 256)), "v"(lane * 4), "s"(r) : "memory");
+        }
+        sbuf = S::next(sbuf);
+        dma.skip(ROWS);
+        srow += 512;
+        if (++st == qt) {
+            st = t0;
+            if (++sg < a.G) head_start();
         }
     };
-    for (int t = 0; t < min(S::LEAD, nj); ++t) send(t);
+    for (int t = 0; t < min(S::LEAD, nj); ++t) send();
     bf16x8 kf[2][D / 16], vf[D / 8];
     {
         // (keys that do not count are not touched: their rows are cleared, so that nothing they hold can come through a product)
@@ -812,7 +853,9 @@ __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void d
     auto next_scores = [&](int buf) {
         const Lane f = fl.at(buf * TILE);
         constexpr int N = D / 4, AHEAD = KLDS ? 2 : 4;
-        dp = row_start(rc + buf * 128, h);
+        s[0] = row_start(rc + buf * 128, h);
+        s[1] = row_start(rc + buf * 128 + 32, h);
+        dp = row_start(rc + buf * 128 + 64, h);
         bf16x8 x[AHEAD], y[AHEAD];
 #pragma unroll
         for (int n = 0; n < AHEAD; ++n) { x[n] = f.template rows16<ROWS>(n * 16); if (KLDS) y[n] = ol.template rows16<32>(n * 16); }
@@ -820,7 +863,7 @@ __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void d
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             const int i = n / (D / 16), ks = n % (D / 16);
-            if (i < 2) s[i & 1] = mfma32<F16>(x[n % AHEAD], KLDS ? y[n % AHEAD] : kf[i & 1][ks], ks ? s[i & 1] : zero16());
+            if (i < 2) s[i & 1] = mfma32<F16>(x[n % AHEAD], KLDS ? y[n % AHEAD] : kf[i & 1][ks], s[i & 1]);
             else dp = mfma32<F16>(x[n % AHEAD], vf[n - D / 8], dp);
             if (n + AHEAD < N) {
                 x[n % AHEAD] = f.template rows16<ROWS>((n + AHEAD) * 16);
@@ -837,11 +880,12 @@ __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void d
     int buf = 0, g = 0, tq = t0;
     float sign = copysignf(1.0f, a.lam[kvh * a.G * a.lam_stride]);
     for (int j = 0; j < nj; ++j) {
-        dma.landed();
-        if (j + S::LEAD < nj) send(j + S::LEAD);
+        S::template before_vector<decltype(dma)>();
+        if (j + S::LEAD < nj) send();
         if (tq * ROWS < vis_all) mask_queries(s, vis == NEVER ? NEVER : vis - tq * ROWS, h);
         bf16x8 pc[2], ds[2][2];
         dkv_weights<F16>(rc + buf * 128, h, a.c2, sign, s, dp, pc, ds);
+        S::template behind_vector<decltype(dma)>(j + S::LEAD < nj);
         __syncthreads();
         __builtin_amdgcn_s_setprio(1);
         {
