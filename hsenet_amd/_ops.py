@@ -2,9 +2,9 @@
 missing library or a negative status raises HsError."""
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 import os
+import struct
 import threading
 
 import torch
@@ -32,14 +32,18 @@ class DiffAttnDesc(L._Desc):
                 ("q_start0", _i), ("lam_stride", _i), ("scale", C.c_float)] + [(f"{t}_{s}", _i64) for t in ("q", "k", "v", "go") for s in "bnh"]
 
 
+# descriptors are packed in one go where a call builds them (setting a structure's fields one by one costs more than the launch)
+ROTARY_PACK, DIFF_PACK = struct.Struct("@I11i15q"), struct.Struct("@I10if12q")
+assert ROTARY_PACK.size == C.sizeof(RotaryDesc) and DIFF_PACK.size == C.sizeof(DiffAttnDesc)
+
 SIGNATURES = {
     "hs_ops_version": [],
     "hs_ops_build_id": [],
-    "hs_rotary_axes": [C.POINTER(RotaryDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
-    "hs_diff_attn_fwd_ws_bytes": [C.POINTER(DiffAttnDesc)],
-    "hs_diff_attn_bwd_ws_bytes": [C.POINTER(DiffAttnDesc)],
-    "hs_diff_attn_fwd": [C.POINTER(DiffAttnDesc)] + [_vp] * 10 + [_sz, _vp],
-    "hs_diff_attn_bwd": [C.POINTER(DiffAttnDesc)] + [_vp] * 14 + [_sz, _vp],
+    "hs_rotary_axes": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
+    "hs_diff_attn_fwd_ws_bytes": [_vp],
+    "hs_diff_attn_bwd_ws_bytes": [_vp],
+    "hs_diff_attn_fwd": [_vp] + [_vp] * 10 + [_sz, _vp],
+    "hs_diff_attn_bwd": [_vp] + [_vp] * 14 + [_sz, _vp],
     "hs_adamw_multi": [_vp, _i, _i, _i, _d, _d, _d, _d, _d, _vp],
     "hs_adamw_moments": [_vp, _i, _i, _vp],
 }
@@ -82,15 +86,8 @@ def check_fresh() -> str:
     return have
 
 
-def call(name: str, *args) -> None:
-    rc = getattr(load(), name)(*args)
-    if rc != L.HS_OK:
-        raise L.HsError(f"{name} failed: {rc} ({L._ERR.get(rc, 'unknown')})")
-
-
-def on_device(*tensors):
-    """Checks that the tensors (None: left out) are on one GPU; a context in which that GPU is the current one, as the entry points want it.
-    Work goes to that device's current stream: a caller that made a tensor on another stream orders the two, as with any torch operation."""
+def device_of(*tensors) -> int:
+    """the index of the one GPU that the tensors (None: left out) lie on; HsError where they do not"""
     dev = None
     for t in tensors:
         if t is None:
@@ -104,22 +101,39 @@ def on_device(*tensors):
             dev = i
         elif i != dev:
             raise L.HsError(f"the tensors of one call lie on different devices (cuda:{dev} and cuda:{i})")
-    return contextlib.nullcontext() if dev is None or dev == torch.cuda.current_device() else torch.cuda.device(dev)
+    return dev
 
 
-def stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+_current_device, _raw_stream = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device, None
+if hasattr(torch._C, "_cuda_getCurrentRawStream"):
+    _raw_stream = torch._C._cuda_getCurrentRawStream
 
 
-def rows_of_heads(t: torch.Tensor, align: int) -> bool:
-    """whether a [B, N, heads, columns] tensor can be read where it lies: columns side by side, other strides (of axes longer than 1)
-    positive multiples of `align` elements (tokens and heads at most 2^24 apart), its first element on a 16-byte address."""
-    if t.stride(3) != 1 and t.shape[3] != 1:
-        return False
-    return t.data_ptr() % 16 == 0 and all(n == 1 or (s > 0 and s % align == 0) for n, s in zip(t.shape[:3], t.stride()[:3])) \
-        and t.stride(1) <= 1 << 24 and t.stride(2) <= 1 << 24
+def stream(dev: int) -> int:
+    return _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream
 
 
-def bnh(t: torch.Tensor, align: int = 1):
-    """strides of batch entry, token and head; those of an axis of length 1, which no address uses, as 0 where they are not multiples of `align`"""
-    return [s if n > 1 else 0 for n, s in zip(t.shape[:3], t.stride()[:3])]
+def call(dev: int, name: str, *args) -> None:
+    """enqueues an entry point on device `dev`'s current stream (a caller that made a tensor on another stream orders the two, as with any torch
+    operation), with that device the current one"""
+    fn = getattr(_lib or load(), name)
+    if dev == _current_device():
+        rc = fn(*args, stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, stream(dev))
+    if rc != L.HS_OK:
+        raise L.HsError(f"{name} failed: {rc} ({L._ERR.get(rc, 'unknown')})")
+
+
+def rows_of_heads(shape, stride, ptr: int) -> bool:
+    """whether a [B, N, heads, columns] tensor can be read where it lies by the attention kernels: columns side by side, the other strides (of axes longer
+    than 1) positive multiples of 8 elements, tokens and heads at most 2^24 apart, its first element on a 16-byte address"""
+    (b, n, h, d), (sb, sn, sh, sd) = shape, stride
+    return ptr % 16 == 0 and (sd == 1 or d == 1) and (b == 1 or (sb > 0 and sb % 8 == 0)) and (n == 1 or (0 < sn <= 1 << 24 and sn % 8 == 0)) \
+        and (h == 1 or (0 < sh <= 1 << 24 and sh % 8 == 0))
+
+
+def bnh(shape, stride):
+    """strides of batch entry, token and head; 0 for an axis of length 1, which no address uses"""
+    return (stride[0] if shape[0] > 1 else 0, stride[1] if shape[1] > 1 else 0, stride[2] if shape[2] > 1 else 0)

@@ -2,7 +2,6 @@
 maps with a learned weight."""
 from __future__ import annotations
 
-import ctypes as C
 from typing import Optional
 
 import torch
@@ -17,56 +16,64 @@ def _per_entry(t, what, B):
         raise L.HsError(f"{what} must be a dense int32 tensor of one number per batch entry ({B})")
 
 
+def _placed(t):
+    """(t, its strides) where the kernels can read it: itself, or a dense copy"""
+    shape, stride = t.shape, t.stride()
+    if not O.rows_of_heads(shape, stride, t.data_ptr()):
+        t = t.contiguous()
+        if t.data_ptr() % 16:
+            t = t.clone()
+        stride = t.stride()
+    return t, O.bnh(shape, stride)
+
+
 def _prepare(q, k, v, lam, scale, causal, q_start, kv_len):
-    """(descriptor, q, k, v, lam) with the operands where the kernels can read them; HsError for what they cannot take"""
-    for t, name in ((q, "q"), (k, "k"), (v, "v")):
-        if t.dim() != 4:
-            raise L.HsError(f"{name} must have 4 axes: [B, tokens, heads, columns]")
-    if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
+    """(device, descriptor's numbers, q, k, v, lam) with the operands where the kernels can read them; HsError for what they cannot take"""
+    dev = O.device_of(q, k, v, lam, q_start, kv_len)
+    qs, ks, vs, dt = q.shape, k.shape, v.shape, q.dtype
+    if not len(qs) == len(ks) == len(vs) == 4:
+        raise L.HsError("q, k and v must have 4 axes: [B, tokens, heads, columns]")
+    if (dt is not torch.bfloat16 and dt is not torch.float16) or k.dtype is not dt or v.dtype is not dt:
         raise L.HsError("q, k and v must all be bf16 or all fp16")
-    B, Nq, H2, d = q.shape
-    Nk, Hk2 = k.shape[1:3]
+    B, Nq, H2, d = qs
+    Nk, Hk2 = ks[1], ks[2]
     H, Hkv = H2 // 2, Hk2 // 2
     if H2 % 2 or Hk2 % 2 or H < 1 or Hkv < 1 or H % Hkv:
         raise L.HsError(f"q needs 2 H heads and k 2 Hkv, H a multiple of Hkv: got {H2} and {Hk2}")
     if d not in (32, 64, 128):
         raise L.HsError(f"heads of 32, 64 or 128 columns, got {d}")
-    if tuple(k.shape) != (B, Nk, Hk2, d) or tuple(v.shape) != (B, Nk, Hkv, 2 * d):
-        raise L.HsError(f"for q {tuple(q.shape)} and k {tuple(k.shape)} v must be {(B, Nk, Hkv, 2 * d)}, got {tuple(v.shape)}")
-    if lam.dtype != torch.float32 or not (lam.numel() == 1 or tuple(lam.shape) == (H,)):
+    if tuple(ks) != (B, Nk, Hk2, d) or tuple(vs) != (B, Nk, Hkv, 2 * d):
+        raise L.HsError(f"for q {tuple(qs)} and k {tuple(ks)} v must be {(B, Nk, Hkv, 2 * d)}, got {tuple(vs)}")
+    if lam.dtype is not torch.float32 or not (lam.numel() == 1 or tuple(lam.shape) == (H,)):
         raise L.HsError(f"lam must be fp32, one number or one per head ({H},), got {lam.dtype} {tuple(lam.shape)}")
     _per_entry(q_start, "q_start", B)
     _per_entry(kv_len, "kv_len", B)
     scale = d ** -0.5 if scale is None else float(scale)
     if not 0 < scale < 1e6:
         raise L.HsError(f"scale must be positive (below 1e6), got {scale}")
-    q, k, v = (t if O.rows_of_heads(t, 8) else t.contiguous() for t in (q, k, v))
-    desc = O.DiffAttnDesc(B, Nq, Nk, H, Hkv, d, O.DTYPE[q.dtype], int(causal), Nk - Nq)
+    (q, sq), (k, sk), (v, sv) = _placed(q), _placed(k), _placed(v)
     lam = lam.contiguous()
-    desc.lam_stride, desc.scale = int(lam.dim() == 1 and H > 1 and lam.numel() > 1), scale
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        for s, n in zip("bnh", O.bnh(t)):
-            setattr(desc, f"{name}_{s}", n)
-    return desc, q, k, v, lam
+    numbers = (O.DIFF_PACK.size, B, Nq, Nk, H, Hkv, d, O.DTYPE[dt], bool(causal), Nk - Nq, int(H > 1 and lam.numel() > 1), scale, *sq, *sk, *sv)
+    return dev, numbers, q, k, v, lam
 
 
 def _forward(q, k, v, lam, scale, causal, q_start, kv_len, keep):
-    """-> (o, and for a backward pass the operands as they were read, the maps' outputs and statistics)"""
-    with O.on_device(q, k, v, lam, q_start, kv_len):
-        desc, q, k, v, lam = _prepare(q, k, v, lam, scale, causal, q_start, kv_len)
-        B, Nq, H, d = desc.B, desc.Nq, desc.H, desc.d
-        o = torch.empty(B, Nq, H, 2 * d, dtype=q.dtype, device=q.device)
-        maps = torch.empty(2, B, Nq, H, 2 * d, dtype=q.dtype, device=q.device) if keep else None
-        lse = torch.empty(B, H, 4, Nq, dtype=torch.float32, device=q.device) if keep else None
-        if o.numel():
-            if desc.Nk == 0:
-                o.zero_()
-            else:
-                n = O.load().hs_diff_attn_fwd_ws_bytes(C.byref(desc))
-                ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
-                O.call("hs_diff_attn_fwd", C.byref(desc), q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), _ptr(q_start), _ptr(kv_len),
-                       o.data_ptr(), _ptr(maps), _ptr(lse), _ptr(ws), n, O.stream())
-    return o, desc, q, k, v, lam, maps, lse
+    """-> (o, and for a backward pass the descriptor's numbers, the operands as they were read, the maps' outputs and statistics)"""
+    dev, numbers, q, k, v, lam = _prepare(q, k, v, lam, scale, causal, q_start, kv_len)
+    _, B, Nq, Nk, H, _, d = numbers[:7]
+    o = torch.empty(B, Nq, H, 2 * d, dtype=q.dtype, device=q.device)
+    maps = torch.empty(2, B, Nq, H, 2 * d, dtype=q.dtype, device=q.device) if keep else None
+    lse = torch.empty(B, H, 4, Nq, dtype=torch.float32, device=q.device) if keep else None
+    if B * Nq:
+        if Nk == 0:
+            o.zero_()
+        else:
+            desc = O.DIFF_PACK.pack(*numbers, 0, 0, 0)
+            n = O.load().hs_diff_attn_fwd_ws_bytes(desc)
+            ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
+            O.call(dev, "hs_diff_attn_fwd", desc, q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), _ptr(q_start), _ptr(kv_len),
+                   o.data_ptr(), _ptr(maps), _ptr(lse), _ptr(ws), n)
+    return o, numbers, q, k, v, lam, maps, lse
 
 
 def _ptr(t):
@@ -78,28 +85,26 @@ class DiffAttnFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, lam, scale, causal, q_start, kv_len):
-        o, desc, q, k, v, lam, maps, lse = _forward(q, k, v, lam, scale, causal, q_start, kv_len, True)
+        o, numbers, q, k, v, lam, maps, lse = _forward(q, k, v, lam, scale, causal, q_start, kv_len, True)
         ctx.save_for_backward(q, k, v, lam, q_start, kv_len, maps, lse)
-        ctx.desc = desc
+        ctx.numbers = numbers
         return o
 
     @staticmethod
     @once_differentiable
     def backward(ctx, go):
         q, k, v, lam, q_start, kv_len, maps, lse = ctx.saved_tensors
-        with O.on_device(q, go):
-            go = go if O.rows_of_heads(go, 8) else go.contiguous()
-            dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-            dlam = torch.empty(lam.shape, dtype=torch.float32, device=q.device)
-            if q.numel() == 0 or k.numel() == 0:
-                return (*(t.zero_() for t in (dq, dk, dv, dlam)), None, None, None, None)
-            desc = O.DiffAttnDesc.from_buffer_copy(ctx.desc)          # (the graph may be run backward from several threads, or again)
-            for s, n in zip("bnh", O.bnh(go)):
-                setattr(desc, f"go_{s}", n)
-            n = O.load().hs_diff_attn_bwd_ws_bytes(C.byref(desc))
-            ws = torch.empty(n, dtype=torch.uint8, device=q.device)
-            O.call("hs_diff_attn_bwd", C.byref(desc), q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), _ptr(q_start), _ptr(kv_len), go.data_ptr(),
-                   maps.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dlam.data_ptr(), ws.data_ptr(), n, O.stream())
+        dev = O.device_of(q, go)
+        go, sg = _placed(go)
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        dlam = torch.empty(lam.shape, dtype=torch.float32, device=q.device)
+        if q.numel() == 0 or k.numel() == 0:
+            return (*(t.zero_() for t in (dq, dk, dv, dlam)), None, None, None, None)
+        desc = O.DIFF_PACK.pack(*ctx.numbers, *sg)
+        n = O.load().hs_diff_attn_bwd_ws_bytes(desc)
+        ws = torch.empty(n, dtype=torch.uint8, device=q.device)
+        O.call(dev, "hs_diff_attn_bwd", desc, q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), _ptr(q_start), _ptr(kv_len), go.data_ptr(),
+               maps.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dlam.data_ptr(), ws.data_ptr(), n)
         return dq, dk, dv, dlam, None, None, None, None
 
 

@@ -120,39 +120,39 @@ class AdamW(torch.optim.Optimizer):
                 loss = closure()
         for group in self.param_groups:
             numbers, bits = self._check_numbers(group), group["state_bits"]
-            tables = {}                                        # (device, type) -> entries
-            changed = []
+            tables, changed, state, key, words = {}, [], self.state, None, None       # (device, type) -> (addresses, gradients)
             for p in group["params"]:
                 g = p.grad
                 if g is None:
                     continue
-                if not p.is_cuda:
+                dev, dtype = p.get_device(), p.dtype
+                if dev < 0:
                     raise L.HsError("hsenet_amd kernels need tensors on an MI355X ('cuda') device; there is no CPU fallback")
-                if g.is_sparse or g.dtype != p.dtype or g.device != p.device:
+                if g.dtype is not dtype or g.get_device() != dev or g.is_sparse:
                     raise L.HsError("a gradient must be dense, of its parameter's type and on its device")
-                st = self.state.get(p) or self._init_state(p, bits)
+                st = state.get(p) or self._init_state(p, bits)
                 stride = p.stride()
-                if not p.is_contiguous() and not _dense(p):
+                if not (p.is_contiguous() or _dense(p)):
                     raise L.HsError("a parameter's elements must fill one stretch of memory")
                 if g.stride() != stride:
                     g = torch.empty_like(p).copy_(g)
                 m, v = st["exp_avg"], st["exp_avg_sq"]
                 if m.stride() != stride or v.stride() != stride:
                     self._check_state(p, st, bits)
-                key = (p.get_device(), p.dtype)
-                t = tables.get(key)
-                if t is None:
-                    t = tables[key] = (array("q"), [])
+                if key != (dev, dtype):
+                    key = (dev, dtype)
+                    if key not in tables:
+                        tables[key] = (array("q"), [])
+                    words, held = tables[key]
+                held.append(g)                                 # (a gradient that was copied lives until the launch)
                 if bits == 8:
-                    t[0].extend((p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), st["exp_avg_scale"].data_ptr(),
-                                 st["exp_avg_sq_scale"].data_ptr(), st["step"].data_ptr(), p.numel()))
+                    words.extend((p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), st["exp_avg_scale"].data_ptr(),
+                                  st["exp_avg_sq_scale"].data_ptr(), st["step"].data_ptr(), p.numel()))
                 else:
-                    t[0].extend((p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), 0, 0, st["step"].data_ptr(), p.numel()))
-                t[1].append(g)                                 # (a gradient that was copied lives until the launch)
+                    words.extend((p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), 0, 0, st["step"].data_ptr(), p.numel()))
                 changed.append(p)
             for (dev, dtype), (words, _) in tables.items():
-                with torch.cuda.device(dev):
-                    O.call("hs_adamw_multi", words.buffer_info()[0], len(words) // 8, O.DTYPE[dtype], bits, *numbers, O.stream())
+                O.call(dev, "hs_adamw_multi", words.buffer_info()[0], len(words) // 8, O.DTYPE[dtype], bits, *numbers)
             if changed:
                 torch.autograd.graph.increment_version(changed)
         return loss
@@ -161,29 +161,35 @@ class AdamW(torch.optim.Optimizer):
     def read_moments(self, exp_avg: Sequence[torch.Tensor], exp_avg_sq: Sequence[torch.Tensor]) -> None:
         """writes the moments of every parameter (in the groups' order) into the given dense tensors of its shape and strides, all bf16 or all fp32: the
         values that 8-bit codes stand for, or a copy of 32-bit moments.  A parameter that has no state yet has moments of 0."""
-        ps = [(p, g["state_bits"]) for g in self.param_groups for p in g["params"]]
-        if len(exp_avg) != len(ps) or len(exp_avg_sq) != len(ps):
-            raise L.HsError(f"one pair of tensors per parameter expected ({len(ps)})")
-        tables = {}
-        for (p, bits), m, v in zip(ps, exp_avg, exp_avg_sq):
-            for t in (m, v):
-                if t.dtype not in (torch.float32, torch.bfloat16) or t.shape != p.shape or t.device != p.device or t.dtype != exp_avg[0].dtype \
-                        or (t.stride() != p.stride() and p.numel() > 1):
-                    raise L.HsError("moments go into bf16 or fp32 tensors of their parameter's shape, strides and device")
-            st = self.state.get(p)
-            if not st:
-                m.zero_()
-                v.zero_()
-            elif bits == 32:
-                m.copy_(st["exp_avg"])
-                v.copy_(st["exp_avg_sq"])
-            else:
-                tables.setdefault(p.get_device(), array("q")).extend(
-                    (m.data_ptr(), v.data_ptr(), st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr(), st["exp_avg_scale"].data_ptr(),
-                     st["exp_avg_sq_scale"].data_ptr(), st["step"].data_ptr(), p.numel()))
+        if not len(exp_avg) == len(exp_avg_sq) == sum(len(g["params"]) for g in self.param_groups):
+            raise L.HsError("one pair of tensors per parameter expected")
+        tables, i = {}, 0
+        dtype = exp_avg[0].dtype if exp_avg else torch.float32
+        if dtype is not torch.float32 and dtype is not torch.bfloat16:
+            raise L.HsError("moments go into bf16 or fp32 tensors")
+        for group in self.param_groups:
+            bits = group["state_bits"]
+            for p in group["params"]:
+                m, v, dev, shape, stride = exp_avg[i], exp_avg_sq[i], p.get_device(), p.shape, p.stride()
+                i += 1
+                for t in (m, v):
+                    if t.dtype is not dtype or t.get_device() != dev or t.shape != shape or (t.stride() != stride and p.numel() > 1):
+                        raise L.HsError("moments go into tensors of one type, each of its parameter's shape, strides and device")
+                st = self.state.get(p)
+                if not st:
+                    m.zero_()
+                    v.zero_()
+                elif bits == 32:
+                    m.copy_(st["exp_avg"])
+                    v.copy_(st["exp_avg_sq"])
+                else:
+                    words = tables.get(dev)
+                    if words is None:
+                        words = tables[dev] = array("q")
+                    words.extend((m.data_ptr(), v.data_ptr(), st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr(), st["exp_avg_scale"].data_ptr(),
+                                  st["exp_avg_sq_scale"].data_ptr(), 0, p.numel()))
         for dev, words in tables.items():
-            with torch.cuda.device(dev):
-                O.call("hs_adamw_moments", words.buffer_info()[0], len(words) // 8, O.DTYPE[exp_avg[0].dtype], O.stream())
+            O.call(dev, "hs_adamw_moments", words.buffer_info()[0], len(words) // 8, O.DTYPE[dtype])
 
     def moments(self, p: torch.Tensor, dtype: torch.dtype = torch.float32) -> Tuple[torch.Tensor, torch.Tensor]:
         """the moments (m, v) of one parameter in fp32 or bf16, whatever they are held in"""

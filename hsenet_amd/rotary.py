@@ -2,7 +2,6 @@
 columns of q and k in front of attention (``hs_rotary_axes``)."""
 from __future__ import annotations
 
-import ctypes as C
 from typing import Optional, Sequence
 
 import torch
@@ -51,47 +50,55 @@ def _turn(xs, positions, plan, inverse, inplace):
     """the turned tensors of xs (one or two [B, N, heads, dh] of one type), new ones or xs themselves"""
     if not isinstance(plan, RotaryAxes):
         raise L.HsError("plan must be a RotaryAxes")
-    x0, x1 = xs[0], xs[1] if len(xs) > 1 else None
-    with O.on_device(x0, x1, positions, plan.freq):
-        if x0.dtype not in O.DTYPE:
-            raise L.HsError(f"q and k must be bf16, fp16 or fp32, got {x0.dtype}")
-        for x in xs:
-            if x.dim() != 4 or x.dtype != x0.dtype or x.shape[:2] != x0.shape[:2] or x.shape[3] != x0.shape[3]:
-                raise L.HsError("q and k must be [B, N, heads, columns] of one type, equal in B, N and columns")
-        B, N, _, dh = x0.shape
-        if dh < 2 * plan.pairs:
-            raise L.HsError(f"a head of {dh} columns has no room for {plan.pairs} pairs")
-        if positions.dtype not in _POS:
-            raise L.HsError(f"positions must be int32, int64 or float32, got {positions.dtype}")
-        if tuple(positions.shape) == (plan.axes, N):
-            pa, pn, pb = positions.stride(0), positions.stride(1), 0
-        elif tuple(positions.shape) == (plan.axes, B, N):
-            pa, pb, pn = positions.stride()
-        else:
-            raise L.HsError(f"positions must be [axes, N] or [axes, B, N] = ({plan.axes}, {B}, {N}), got {tuple(positions.shape)}")
-        ins = []
-        for x in xs:
-            if x.stride(3) != 1 and dh > 1:
-                if inplace:
-                    raise L.HsError("a tensor that is turned in place must have its columns side by side")
-                x = x.contiguous()
-            if inplace and x.numel() and any(n > 1 and s == 0 for n, s in zip(x.shape, x.stride())):
+    dev = O.device_of(*xs, positions, plan.freq)
+    x0 = xs[0]
+    dt, dtype = x0.dtype, O.DTYPE.get(x0.dtype)
+    if dtype is None:
+        raise L.HsError(f"q and k must be bf16, fp16 or fp32, got {dt}")
+    shape = x0.shape
+    if len(shape) != 4:
+        raise L.HsError("q and k must be [B, N, heads, columns]")
+    B, N, _, dh = shape
+    if dh < 2 * plan.pairs:
+        raise L.HsError(f"a head of {dh} columns has no room for {plan.pairs} pairs")
+    pos_dtype = _POS.get(positions.dtype)
+    if pos_dtype is None:
+        raise L.HsError(f"positions must be int32, int64 or float32, got {positions.dtype}")
+    if tuple(positions.shape) == (plan.axes, B, N):
+        pos = positions.stride()
+    elif tuple(positions.shape) == (plan.axes, N):
+        pos = (positions.stride(0), 0, positions.stride(1))
+    else:
+        raise L.HsError(f"positions must be [axes, N] or [axes, B, N] = ({plan.axes}, {B}, {N}), got {tuple(positions.shape)}")
+    outs, live = [], []
+    for x in xs:
+        xshape = x.shape
+        if x.dtype != dt or len(xshape) != 4 or xshape[0] != B or xshape[1] != N or xshape[3] != dh:
+            raise L.HsError("q and k must be [B, N, heads, columns] of one type, equal in B, N and columns")
+        stride = x.stride()
+        if stride[3] != 1 and dh > 1:
+            if inplace:
+                raise L.HsError("a tensor that is turned in place must have its columns side by side")
+            x = x.contiguous()
+            stride = x.stride()
+        if inplace:
+            if any(n > 1 and s == 0 for n, s in zip(xshape, stride)):
                 raise L.HsError("a broadcast tensor cannot be turned in place")
-            ins.append(x)
-        outs = ins if inplace else [torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in ins]
-        if B * N == 0 or all(x.numel() == 0 for x in ins):
-            return outs
-        live = [(x, y) for x, y in zip(ins, outs) if x.shape[2]]
-        d = O.RotaryDesc(B, N, dh, plan.pairs, plan.axes)
-        d.interleaved, d.inverse, d.dtype, d.pos_dtype = plan.interleaved, inverse, O.DTYPE[x0.dtype], _POS[positions.dtype]
-        for i, (x, y) in enumerate(live):
-            d.heads[i] = x.shape[2]
-            d.x_b[i], d.x_n[i], d.x_h[i] = O.bnh(x)
-            d.y_b[i], d.y_n[i], d.y_h[i] = O.bnh(y)
-        d.pos_a, d.pos_b, d.pos_n = pa, pb, pn
-        ptr = [p.data_ptr() for xy in live for p in xy] + [None, None]
-        O.call("hs_rotary_axes", C.byref(d), *ptr[:4], positions.data_ptr(), plan.freq.data_ptr(), plan.axis.data_ptr(), O.stream())
-        return outs
+            y, ystride = x, stride
+        else:
+            y = torch.empty(xshape, dtype=dt, device=x.device)
+            ystride = y.stride()
+        outs.append(y)
+        if y.numel():
+            live.append((xshape[2], x, O.bnh(xshape, stride), y, O.bnh(xshape, ystride)))
+    if live:
+        h0, x0, s0, y0, t0 = live[0]
+        h1, x1, s1, y1, t1 = live[1] if len(live) > 1 else (0, None, (0, 0, 0), None, (0, 0, 0))
+        desc = O.ROTARY_PACK.pack(O.ROTARY_PACK.size, B, N, dh, plan.pairs, plan.axes, h0, h1, plan.interleaved, inverse, dtype, pos_dtype,
+                                  s0[0], s1[0], s0[1], s1[1], s0[2], s1[2], t0[0], t1[0], t0[1], t1[1], t0[2], t1[2], *pos)
+        O.call(dev, "hs_rotary_axes", desc, x0.data_ptr(), y0.data_ptr(), None if x1 is None else x1.data_ptr(), None if y1 is None else y1.data_ptr(),
+               positions.data_ptr(), plan.freq.data_ptr(), plan.axis.data_ptr())
+    return outs
 
 
 class RotaryAxesFn(torch.autograd.Function):
