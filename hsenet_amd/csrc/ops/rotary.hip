@@ -5,9 +5,12 @@
 // The angle is a product in 64 bits, reduced to a fraction of a turn there (a position of 10^6 would leave an fp32 angle 0.06 rad off);
 // the fraction, at most 1/2, is rounded to 32 bits and goes through sincospi.
 #include "../common.h"
+#include <algorithm>
 #include "../../../include/hsenet_ops.h"
 
 namespace {
+
+constexpr int MOST_TOKENS = 16, TARGET = 1024;     // of a block: tokens, vectors
 
 struct RotaryArgs {
     const void* x[2];
@@ -38,14 +41,18 @@ template <> struct Elem<HS_PREC_F32> {
     static __device__ __forceinline__ T put(float f) { return f; }
 };
 
-// A row (one head of one token) is cut into items of VEC columns that one thread moves: with split halves, P / VEC items take VEC columns of
-// the first half and the VEC facing them; interleaved, 2 P / VEC items take VEC / 2 neighbouring pairs; the columns behind follow as plain
-// copies (none where a tensor is turned in place).
-template <int DT, int VEC, bool INTER>
+enum { SPLIT, LINE, PAIRS };
+
+// A row (one head of one token) is cut into items of VEC columns that one thread moves.  SPLIT (halves, j and j + P): P / VEC items take VEC columns of
+// the first half and the VEC facing them.  LINE (the same halves, where a row is a power of two of 16-byte vectors and turned whole): an item is one
+// vector, so that a wave reads and writes whole lines, and the facing vector comes from the lane that holds it: 89 us against 95 for 16 x 4097 tokens of 24
+// heads of 64 in bf16, 71 against 78 for 8 x 4097 of 20 heads of 128.  PAIRS (neighbours): an item is VEC / 2 pairs.  Columns behind the pairs follow as plain copies (none where a tensor is turned in place).
+template <int DT, int VEC, int MODE>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
     typedef typename Elem<DT>::T T;
     typedef __attribute__((ext_vector_type(VEC))) T V;
     extern __shared__ float2 cs[];                       // [tpb][P]: cosine, sine
+    __shared__ long at[MOST_TOKENS][4];                  // where each token's heads begin: x0, x1, y0, y1
     const int tok0 = blockIdx.x * a.tpb, ntok = min(a.tpb, a.tokens - tok0);
     const float inv_p = 1.0f / a.P;
     for (int i = threadIdx.x; i < ntok * a.P; i += 256) {
@@ -61,65 +68,99 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
         sincospif(2.0f * (float)turns, &s, &c);
         cs[i] = make_float2(c, s * a.inverse);
     }
+    if (threadIdx.x < (unsigned)ntok) {
+        const long tok = tok0 + threadIdx.x, b = tok / a.N, n = tok - b * a.N;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            at[threadIdx.x][i] = b * a.x_b[i] + n * a.x_n[i];
+            at[threadIdx.x][2 + i] = b * a.y_b[i] + n * a.y_n[i];
+        }
+    }
     __syncthreads();
-    constexpr bool SINGLE = INTER && VEC == 1;           // rows of odd length: a pair is two single accesses
-    const int turned = SINGLE ? a.P : INTER ? 2 * a.P / VEC : a.P / VEC;
+    constexpr bool SINGLE = MODE == PAIRS && VEC == 1;           // rows of odd length: a pair is two single accesses
+    const int turned = SINGLE ? a.P : MODE == SPLIT ? a.P / VEC : 2 * a.P / VEC;
     const int tail = (a.dh - 2 * a.P) / VEC, items = turned + tail;
     const int total = ntok * a.heads * items;
     const float inv_items = 1.0f / items;
-    for (int i = threadIdx.x; i < total; i += 256) {
-        const int row = (int)((i + 0.5f) * inv_items), it = i - row * items;
-        const int t = (int)((row + 0.5f) * a.inv_heads);
-        int h = row - t * a.heads;
-        const int which = h >= a.heads0;
-        h -= which ? a.heads0 : 0;
-        const int tok = tok0 + t, b = tok / a.N, n = tok - b * a.N;
-        const T* x = (const T*)a.x[which] + b * a.x_b[which] + n * a.x_n[which] + h * a.x_h[which];
-        T* y = (T*)a.y[which] + b * a.y_b[which] + n * a.y_n[which] + h * a.y_h[which];
-        const float2* w = cs + t * a.P;
-        if (it >= turned) {
-            const int col = 2 * a.P + (it - turned) * VEC;
-            if (x != y) *(V*)(y + col) = *(const V*)(x + col);
-        } else if constexpr (SINGLE) {
-            const float2 r = w[it];
-            const float p = Elem<DT>::get(x[2 * it]), q = Elem<DT>::get(x[2 * it + 1]);
-            y[2 * it] = Elem<DT>::put(p * r.x - q * r.y);
-            y[2 * it + 1] = Elem<DT>::put(p * r.y + q * r.x);
-        } else if constexpr (INTER) {
-            const V u = *(const V*)(x + it * VEC);
-            V o;
+    // AT items of a thread at a time: their loads are all on the way before the first is used
+    constexpr int AT = 2, W = SINGLE || MODE == SPLIT ? 2 : 1;                // vectors that an item reads
+    for (int i0 = threadIdx.x; i0 < total; i0 += 256 * AT) {
+        V u[AT][W];
+        T* y[AT];
+        int kind[AT], first[AT], second[AT];                              // 0: no item, 1: turned, 2: copied; columns; the angles' place
+        const float2* w[AT];
 #pragma unroll
-            for (int e = 0; e < VEC; e += 2) {
-                const float2 r = w[(it * VEC + e) >> 1];
-                const float p = Elem<DT>::get(u[e]), q = Elem<DT>::get(u[e + 1]);
-                o[e] = Elem<DT>::put(p * r.x - q * r.y);
-                o[e + 1] = Elem<DT>::put(p * r.y + q * r.x);
-            }
-            *(V*)(y + it * VEC) = o;
-        } else {
-            const V u = *(const V*)(x + it * VEC), v = *(const V*)(x + a.P + it * VEC);
+        for (int k = 0; k < AT; ++k) {
+            const int i = i0 + k * 256;
+            kind[k] = 0;
+            if (i >= total) continue;
+            const int row = (int)((i + 0.5f) * inv_items), it = i - row * items;
+            const int t = (int)((row + 0.5f) * a.inv_heads);
+            int h = row - t * a.heads;
+            const int which = h >= a.heads0;
+            h -= which ? a.heads0 : 0;
+            const T* x = (const T*)(which ? a.x[1] : a.x[0]) + at[t][which] + h * (which ? a.x_h[1] : a.x_h[0]);
+            y[k] = (T*)(which ? a.y[1] : a.y[0]) + at[t][2 + which] + h * (which ? a.y_h[1] : a.y_h[0]);
+            kind[k] = it < turned ? 1 : x != y[k] ? 2 : 0;
+            first[k] = it < turned ? (SINGLE ? 2 * it : it * VEC) : 2 * a.P + (it - turned) * VEC;
+            second[k] = SINGLE ? first[k] + 1 : a.P + first[k];
+            w[k] = cs + t * a.P + (SINGLE ? it : MODE == PAIRS ? it * VEC / 2 : MODE == LINE ? (it & (turned / 2 - 1)) * VEC : it * VEC);
+            if (kind[k]) u[k][0] = *(const V*)(x + first[k]);
+            if (W == 2 && kind[k] == 1) u[k][W - 1] = *(const V*)(x + second[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < AT; ++k) {
             V o, z;
+            if constexpr (MODE == LINE) {
+                typedef __attribute__((ext_vector_type(4))) int I;
+                I v = __builtin_bit_cast(I, u[k][0]);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                const float2 r = w[it * VEC + e];
-                const float p = Elem<DT>::get(u[e]), q = Elem<DT>::get(v[e]);
-                o[e] = Elem<DT>::put(p * r.x - q * r.y);
-                z[e] = Elem<DT>::put(p * r.y + q * r.x);
+                for (int e = 0; e < 4; ++e) v[e] = __shfl_xor(v[e], turned / 2, 64);       // (a row's lanes take part together or not at all)
+                z = __builtin_bit_cast(V, v);
             }
-            *(V*)(y + it * VEC) = o;
-            *(V*)(y + a.P + it * VEC) = z;
+            if (kind[k] == 2) *(V*)(y[k] + first[k]) = u[k][0];
+            if (kind[k] != 1) continue;
+            if constexpr (MODE == LINE) {
+                const float side = first[k] < a.P ? -1.0f : 1.0f;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    const float2 r = w[k][e];
+                    o[e] = Elem<DT>::put(Elem<DT>::get(u[k][0][e]) * r.x + Elem<DT>::get(z[e]) * (side * r.y));
+                }
+            } else if constexpr (W == 1) {
+#pragma unroll
+                for (int e = 0; e < VEC; e += 2) {
+                    const float2 r = w[k][e >> 1];
+                    const float p = Elem<DT>::get(u[k][0][e]), q = Elem<DT>::get(u[k][0][e + 1]);
+                    o[e] = Elem<DT>::put(p * r.x - q * r.y);
+                    o[e + 1] = Elem<DT>::put(p * r.y + q * r.x);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    const float2 r = w[k][e];
+                    const float p = Elem<DT>::get(u[k][0][e]), q = Elem<DT>::get(u[k][W - 1][e]);
+                    o[e] = Elem<DT>::put(p * r.x - q * r.y);
+                    z[e] = Elem<DT>::put(p * r.y + q * r.x);
+                }
+                *(V*)(y[k] + second[k]) = z;
+            }
+            *(V*)(y[k] + first[k]) = o;
         }
     }
 }
 
-template <int DT, bool INTER>
-void launch(const RotaryArgs& a, int vec, hipStream_t s) {
+template <int DT>
+void launch(const RotaryArgs& a, int vec, bool pairs, bool line, hipStream_t s) {
     const dim3 grid((a.tokens + a.tpb - 1) / a.tpb), block(256);
     const size_t lds = (size_t)a.tpb * a.P * sizeof(float2);
     constexpr int FULL = DT == HS_PREC_F32 ? 4 : 8;
-    if (vec == FULL) hipLaunchKernelGGL((rotary_kernel<DT, FULL, INTER>), grid, block, lds, s, a);
-    else if (vec == 2) hipLaunchKernelGGL((rotary_kernel<DT, 2, INTER>), grid, block, lds, s, a);
-    else hipLaunchKernelGGL((rotary_kernel<DT, 1, INTER>), grid, block, lds, s, a);
+#define HS_ROT(VEC, MODE) hipLaunchKernelGGL((rotary_kernel<DT, VEC, MODE>), grid, block, lds, s, a)
+    if (line) HS_ROT(FULL, LINE);
+    else if (vec == FULL) { if (pairs) HS_ROT(FULL, PAIRS); else HS_ROT(FULL, SPLIT); }
+    else if (vec == 2) { if (pairs) HS_ROT(2, PAIRS); else HS_ROT(2, SPLIT); }
+    else { if (pairs) HS_ROT(1, PAIRS); else HS_ROT(1, SPLIT); }
+#undef HS_ROT
 }
 
 }  // namespace
@@ -156,11 +197,15 @@ extern "C" int hs_rotary_axes(const hs_rotary_desc* d, const void* x0, void* y0,
     a.pos_a = d->pos_a; a.pos_b = d->pos_b; a.pos_n = d->pos_n;
     a.N = d->N; a.tokens = d->B * d->N; a.heads0 = d->heads[0]; a.heads = heads; a.P = d->pairs; a.dh = d->dh; a.pos_dtype = d->pos_dtype;
     a.inv_heads = 1.0f / heads; a.inverse = d->inverse ? -1.0f : 1.0f;
-    a.tpb = 1;
+    const int vectors = d->dh / full;
+    const bool pairs = d->interleaved, line = !pairs && vec == full && d->dh == 2 * d->pairs && vectors >= 2 && vectors <= 64 && !(vectors & (vectors - 1));
+    // tokens of a block: about TARGET vectors, while the grid still gives every CU several blocks
+    const int tail = (d->dh - 2 * d->pairs) / vec, turned = line || pairs ? std::max(2 * d->pairs / vec, 1) : 2 * (d->pairs / vec);
+    a.tpb = std::max(1, std::min({TARGET / (heads * (turned + tail)), a.tokens / 2048, MOST_TOKENS}));
     hipStream_t s = (hipStream_t)stream;
-    if (d->dtype == HS_PREC_BF16) d->interleaved ? launch<HS_PREC_BF16, true>(a, vec, s) : launch<HS_PREC_BF16, false>(a, vec, s);
-    else if (d->dtype == HS_PREC_F16) d->interleaved ? launch<HS_PREC_F16, true>(a, vec, s) : launch<HS_PREC_F16, false>(a, vec, s);
-    else d->interleaved ? launch<HS_PREC_F32, true>(a, vec, s) : launch<HS_PREC_F32, false>(a, vec, s);
+    if (d->dtype == HS_PREC_BF16) launch<HS_PREC_BF16>(a, vec, pairs, line, s);
+    else if (d->dtype == HS_PREC_F16) launch<HS_PREC_F16>(a, vec, pairs, line, s);
+    else launch<HS_PREC_F32>(a, vec, pairs, line, s);
     HS_CHECK_LAUNCH();
     return HS_OK;
 }
