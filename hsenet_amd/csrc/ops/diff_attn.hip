@@ -19,6 +19,8 @@ constexpr float NONE = -1e30f;                 // running maximum before the fir
 constexpr float HEADROOM = 8.0f;               // a running maximum is kept until a score passes it by this many powers of two
 constexpr int SHIFT16 = 4;                     // fp16: P and dS of the backward pass are held times 2^4
 
+constexpr int MOST_CHUNKS = 512;             // of a row's keys
+
 struct Args {
     const bf16_t *q, *k, *v, *go;
     const float* lam;
@@ -83,10 +85,12 @@ template <int D, int VC, int ROWS, int NW> struct Dma {
         const unsigned long long a = (unsigned long long)p;
         return u32x4{(unsigned)__builtin_amdgcn_readfirstlane((unsigned)a), (unsigned)__builtin_amdgcn_readfirstlane((unsigned)(a >> 32)), HS_MAX_RECORDS, 0x00020000u};
     }
-    __device__ __forceinline__ void issue(unsigned lds) const {           // rows at or behind `end` become zeros, and are not touched
+    __device__ __forceinline__ void issue(unsigned lds) const { send<0, PER>(lds); }
+    // pieces FROM to TO of the tile; rows at or behind `end` become zeros, and are not touched
+    template <int FROM, int TO> __device__ __forceinline__ void send(unsigned lds) const {
         const u32x4 rx = resource(x), ry = resource(y);
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
+        for (int i = FROM; i < TO; ++i) {
             const int g = i * NW + wave, image = g / GROUPS, group = g % GROUPS, more = NW == 1 ? group * 8 : 0;
             const bool pair = image < PAIRS;
             const int im = pair ? image : image - PAIRS;
@@ -413,38 +417,30 @@ __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void d
 }
 
 // ---- split forward: few queries against many keys ------------------------------------------------------------------------------------------
-// HBM-bound: K and V are read once for all query heads of a key head.  A wave's 32 rows are (head of the group, query) pairs; a block takes one
-// chunk of the keys, each of its waves every NW-th tile of 32 keys through two LDS buffers of its own (no barrier in the loop).  The waves' numerators are
-// joined in LDS, and the chunks' by diff_join_kernel; with one chunk the result is written at once.
-template <int D, bool F16, bool KEEP, int NW>
-__global__ __launch_bounds__(NW * 64, 1) void diff_split_kernel(Args a) {
-    typedef Sweep<D> S;
-    constexpr int ROWS = 32, VC = S::VC, TILE = ROWS * (2 * D + VC) * 2, NB = VC / 32, NT = NW * 64, PER = 32 * VC / NT;
-    extern __shared__ __attribute__((aligned(16))) char smem[];           // 2 NW tiles; then the waves' numerators of one map
+// HBM-bound: K and V are read once for all query heads of a key head.  The 32 columns of a wave's matrix products are 16 rows, (head of the group, query)
+// pairs, under both maps: column c is map c / 16 of row c % 16.  q K^T is made of both maps for all columns, and each column keeps its own; the softmax and
+// the products with V then go over both maps at once.  A block takes one chunk of the keys, each of its waves every NW-th tile of 32 keys through LDS of
+// its own (no barrier in the loop): the next tile's keys are sent for when the scores have been read, its values behind the products with V, so that
+// half a tile a wave is always on its way.  The waves' numerators are joined in LDS, and the chunks' by diff_join_kernel; with one chunk the result is
+// written at once.
+template <int D> struct SplitOf { static constexpr int NW = D == 128 ? 2 : 4, TILE = 32 * 4 * D * 2; };
+
+template <int D, bool F16, bool KEEP>
+__global__ __launch_bounds__(SplitOf<D>::NW * 64, D == 128 ? 1 : 2) void diff_split_kernel(Args a) {
+    constexpr int ROWS = 32, NW = SplitOf<D>::NW, TILE = SplitOf<D>::TILE, W = 2 * D, NB = W / 32, NT = NW * 64, PER = 4 * W / NT;
+    extern __shared__ __attribute__((aligned(16))) char smem[];           // a tile a wave; then the waves' numerators
     constexpr int SUMS = KEEP ? 2 : 1;
-    __shared__ float wm[2][NW][32], wl[2][SUMS][NW][32];
+    __shared__ float wm[NW][32], wl[SUMS][NW][32], total[32];
     const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, c = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int id = blockIdx.x;
-    const int half = id % S::HALVES; id /= S::HALVES;
     const int split = id % a.nsplit; id /= a.nsplit;
     const int tile = id % a.tiles; id /= a.tiles;
     const int kvh = id % a.Hkv, b = id / a.Hkv;
-    const int len = key_count(a, b), start = first_pos(a, b), rows = a.G * a.Nq;
+    const int len = key_count(a, b), start = first_pos(a, b), rows = a.G * a.Nq, here = min(16, rows - tile * 16), RT = min(16, rows);
     const int k0 = split * a.chunk;
     if (k0 >= len && a.nsplit > 1) return;                                // (the join reads the chunks that begin inside len alone)
-    const int R = tile * 32 + c, Rc = min(R, rows - 1);
-    const int head = kvh * a.G + Rc / a.Nq, query = Rc % a.Nq;
-    const int lim = visible(a, len, start, query);
-    int k1 = min(lim, k0 + a.chunk);                                      // end of the chunk's keys that some row of the tile sees
-#pragma unroll
-    for (int i = 16; i > 0; i >>= 1) k1 = max(k1, __shfl_xor(k1, i, 64));
-    k1 = __builtin_amdgcn_readfirstlane(k1);
-    int lim_lo = lim;                                                     // keys that every row sees
-#pragma unroll
-    for (int i = 16; i > 0; i >>= 1) lim_lo = min(lim_lo, __shfl_xor(lim_lo, i, 64));
-    lim_lo = __builtin_amdgcn_readfirstlane(lim_lo);
-
+    const int R = min(tile * 16 + (c & 15), rows - 1), head = kvh * a.G + R / a.Nq, query = R % a.Nq;
     bf16x8 qf[2][D / 16];
     {
         const bf16_t* qp = a.q + b * a.q_b + query * a.q_n + 2 * head * a.q_h + 8 * h;
@@ -453,137 +449,187 @@ __global__ __launch_bounds__(NW * 64, 1) void diff_split_kernel(Args a) {
 #pragma unroll
             for (int ks = 0; ks < D / 16; ++ks) qf[i][ks] = load8(qp + i * a.q_h + ks * 16);
     }
-    float m[2] = {NONE, NONE}, l[2][SUMS] = {};
-    f32x16 o[2][NB];
-    clear(o[0]); clear(o[1]);
-    char* const own = smem + wave * (2 * TILE);
-    Lane fl;
-    fl.init(own, lane);
-    Dma<D, VC, ROWS, 1> dma;
-    dma.init(0, lane, a.k + b * a.k_b + 2 * kvh * a.k_h, a.k_n, a.k_h, a.v + b * a.v_b + kvh * a.v_h + half * VC, a.v_n, k0 + wave * ROWS, len);
+    const int lim = visible(a, len, start, query);
+    int k1 = min(lim, k0 + a.chunk), lim_lo = lim;                        // end of the chunk's keys that some row sees; keys that every row sees
+#pragma unroll
+    for (int i = 8; i > 0; i >>= 1) {
+        k1 = max(k1, __shfl_xor(k1, i, 64));
+        lim_lo = min(lim_lo, __shfl_xor(lim_lo, i, 64));
+    }
+    k1 = __builtin_amdgcn_readfirstlane(k1);
+    lim_lo = __builtin_amdgcn_readfirstlane(lim_lo);
+
+    typedef Dma<D, W, ROWS, 1> Tiles;
+    constexpr int KEYS = Tiles::PAIRS * Tiles::GROUPS, ALL = Tiles::PER;  // a tile's pieces: keys, then values
+    char* const own = smem + wave * TILE;
+    const unsigned at = lds_addr(own);
+    Lane f;
+    f.init(own, lane);
+    Tiles dma;
+    dma.init(0, lane, a.k + b * a.k_b + 2 * kvh * a.k_h, a.k_n, a.k_h, a.v + b * a.v_b + kvh * a.v_h, a.v_n, k0 + wave * ROWS, k1);
+    dma.issue(at);
+    float m = NONE, l[SUMS] = {};
+    f32x16 o[NB];
+    clear(o);
     arrived();
-    int t = k0 + wave * ROWS, buf = 0;
-    if (t < k1) dma.issue(lds_addr(own));
-    for (; t < k1; t += NW * ROWS) {
-        if (t + NW * ROWS < k1) {
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");            // (the last step's reads of that buffer are over)
-            dma.skip(NW * ROWS);
-            dma.issue(lds_addr(own) + (buf ^ 1) * TILE);
-            dma.template landed<Dma<D, VC, ROWS, 1>::PER>();
-        } else {
-            dma.landed();
-        }
-        const Lane f = fl.at(buf * TILE);
-        buf ^= 1;
+    for (int t = k0 + wave * ROWS; t < k1; t += NW * ROWS) {
         f32x16 s[2];
-        bf16x8 p[2][2];
+        Tiles::template landed<ALL - KEYS>();
         scores<D, F16, ROWS>(f, qf, s);
-        if (t + ROWS > lim_lo) mask_keys(s, lim - t, h);
-        follow_max(s[0], a.c2, m[0], l[0], o[0]);
-        follow_max(s[1], a.c2, m[1], l[1], o[1]);
-        softmax_weights<F16>(s[0], a.c2, m[0], l[0], p[0]);
-        softmax_weights<F16>(s[1], a.c2, m[1], l[1], p[1]);
-        values<D, F16, ROWS>(f, p, o[0], o[1]);
-    }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                // (the reads of the keys are over)
+        dma.skip(NW * ROWS);
+        dma.template send<0, KEYS>(at);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        if (h == 0) wm[i][wave][c] = m[i];
+        for (int r = 0; r < 16; ++r) s[0][r] = c < 16 ? s[0][r] : s[1][r];
+        if (t + ROWS > lim_lo)
 #pragma unroll
-        for (int k = 0; k < SUMS; ++k) {
-            l[i][k] += __shfl_xor(l[i][k], 32, 64);
-            if (h == 0) wl[i][k][wave][c] = l[i][k];
+            for (int r = 0; r < 16; ++r) s[0][r] = acc_row(r, h) < lim - t ? s[0][r] : -__builtin_inff();
+        bf16x8 p[2];
+        follow_max(s[0], a.c2, m, l, o);
+        softmax_weights<F16>(s[0], a.c2, m, l, p);
+        Tiles::template landed<KEYS>();
+        constexpr int N = 2 * NB, AHEAD = 4;
+        bf16x8 x[AHEAD];
+#pragma unroll
+        for (int n = 0; n < AHEAD; ++n) x[n] = f.template cols32<ROWS>(16 * (n / NB), W + n % NB * 32);
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            o[n % NB] = mfma32<F16>(x[n % AHEAD], p[n / NB], o[n % NB]);
+            if (n + AHEAD < N) x[n % AHEAD] = f.template cols32<ROWS>(16 * ((n + AHEAD) / NB), W + (n + AHEAD) % NB * 32);
         }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                // (and of the values)
+        dma.template send<KEYS, ALL>(at);
     }
-    float first[PER];
-    // a thread joins PER columns of one row: row = tid % 32, columns from (tid / 32) PER
-    const int jr = tid & 31, jc = (tid >> 5) * PER, JR = tile * 32 + jr;
-    const long slot = (((long)(b * a.Hkv + kvh) * a.tiles + tile) * a.nsplit + split) * 2;
-    float* stats = a.part + (long)a.B * a.Hkv * a.tiles * a.nsplit * 2 * 32 * (2 * D);
-    float* num = (float*)smem;                                            // [wave][VC][32]
+    Tiles::landed();                                                      // (the numerators go where the tiles were)
+    if (h == 0) wm[wave][c] = m;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        __syncthreads();
-        float M = NONE;
+    for (int k = 0; k < SUMS; ++k) {
+        l[k] += __shfl_xor(l[k], 32, 64);
+        if (h == 0) wl[k][wave][c] = l[k];
+    }
+    __syncthreads();
+    const long slot = ((long)(b * a.Hkv + kvh) * a.tiles + tile) * a.nsplit + split;
+    f32x4* num = (f32x4*)smem;                                            // [wave][32][W / 4], vectors exchanged within 8 by the row's number
+    float M = NONE;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) M = fmaxf(M, wm[i][w][c]);
-        const float f = __builtin_amdgcn_exp2f(m[i] - M);
+    for (int w = 0; w < NW; ++w) M = fmaxf(M, wm[w][c]);
+    const float mine = __builtin_amdgcn_exp2f(m - M);
+    if ((c & 15) < here) {
 #pragma unroll
         for (int db = 0; db < NB; ++db)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) num[(wave * VC + db * 32 + acc_row(r, h)) * 32 + c] = o[i][db][r] * f;
-        __syncthreads();
-        M = NONE;
-        float L[SUMS] = {};
+            for (int g = 0; g < 4; ++g)
+                num[(wave * 32 + c) * (W / 4) + ((db * 8 + 2 * g + h) ^ (c & 7))] =
+                    f32x4{o[db][4 * g] * mine, o[db][4 * g + 1] * mine, o[db][4 * g + 2] * mine, o[db][4 * g + 3] * mine};
+        if (tid < 32) {
+            float L[SUMS] = {};
 #pragma unroll
-        for (int w = 0; w < NW; ++w) M = fmaxf(M, wm[i][w][jr]);
+            for (int k = 0; k < SUMS; ++k)
 #pragma unroll
-        for (int k = 0; k < SUMS; ++k)
+                for (int w = 0; w < NW; ++w) L[k] += wl[k][w][c] * __builtin_amdgcn_exp2f(wm[w][c] - M);
+            total[c] = L[0];
+            if (a.nsplit > 1) ((f32x4*)a.part)[(slot * 2 + (c >> 4)) * RT + (c & 15)] = f32x4{M, L[0], L[SUMS - 1], 0.f};
+            else if (KEEP) put_lse(a.lse + (((long)b * a.H + head) * 4 + (c >> 4)) * a.Nq + query, 2 * a.Nq, M, L[SUMS - 1]);
+        }
+    }
+    __syncthreads();
+    f32x4* part = (f32x4*)a.part + (long)a.B * a.Hkv * a.tiles * a.nsplit * 2 * RT;
 #pragma unroll
-            for (int w = 0; w < NW; ++w) L[k] += wl[i][k][w][jr] * __builtin_amdgcn_exp2f(wm[i][w][jr] - M);
-        const float inv = L[0] > 0.f ? 1.0f / L[0] : L[0] == 0.f ? 0.f : L[0];
-        if (JR < rows && a.nsplit > 1 && jc == 0 && half == 0) *(f32x4*)(stats + ((slot + i) * 32 + jr) * 4) = f32x4{M, L[0], L[SUMS - 1], 0.f};
-        const int jh = kvh * a.G + min(JR, rows - 1) / a.Nq, jq = min(JR, rows - 1) % a.Nq;
+    for (int e = 0; e < PER; ++e) {
+        const int r = (e * NT + tid) / (W / 4), at4 = (e * NT + tid) % (W / 4);
+        if (r >= here) continue;
+        f32x4 x[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            x[i] = num[(i * 16 + r) * (W / 4) + (at4 ^ (r & 7))];
+#pragma unroll
+            for (int w = 1; w < NW; ++w) x[i] += num[(w * 32 + i * 16 + r) * (W / 4) + (at4 ^ (r & 7))];
+        }
+        if (a.nsplit > 1) {
+            part[((slot * 2 + 0) * RT + r) * (W / 4) + at4] = x[0];
+            part[((slot * 2 + 1) * RT + r) * (W / 4) + at4] = x[1];
+            continue;
+        }
+        const int jh = kvh * a.G + (tile * 16 + r) / a.Nq, jq = (tile * 16 + r) % a.Nq;
         const long row = ((long)b * a.Nq + jq) * a.H + jh;
         const float jl = a.lam[jh * a.lam_stride];
 #pragma unroll
-        for (int e = 0; e < PER; ++e) {
-            float x = 0.f;
-#pragma unroll
-            for (int w = 0; w < NW; ++w) x += num[(w * VC + jc + e) * 32 + jr];
-            if (JR >= rows) continue;
-            if (a.nsplit > 1) a.part[((slot + i) * 32 + jr) * (2 * D) + half * VC + jc + e] = x;
-            else {
-                x *= inv;
-                if (KEEP) a.maps[(i * (long)a.B * a.Nq * a.H + row) * 2 * D + half * VC + jc + e] = f2h<F16>(x);
-                if (i == 0) first[e] = x; else a.o[row * 2 * D + half * VC + jc + e] = f2h<F16>(first[e] - jl * x);
-            }
+        for (int i = 0; i < 2; ++i) {
+            const float L = total[i * 16 + r];
+            x[i] *= L > 0.f ? 1.0f / L : L == 0.f ? 0.f : L;              // (a NaN stays one)
+            if (KEEP) store4<F16>(a.maps + (i * (long)a.B * a.Nq * a.H + row) * W + at4 * 4, x[i][0], x[i][1], x[i][2], x[i][3]);
         }
-        if (KEEP && JR < rows && a.nsplit == 1 && jc == 0 && half == 0) put_lse(a.lse + (((long)b * a.H + jh) * 4 + i) * a.Nq + jq, 2 * a.Nq, M, L[SUMS - 1]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[0][k] = __builtin_fmaf(-jl, x[1][k], x[0][k]);
+        store4<F16>(a.o + row * W + at4 * 4, x[0][0], x[0][1], x[0][2], x[0][3]);
     }
 }
 
-// joins the chunks of a row: a wave each
+// Joins the chunks of a row, a block each: the chunks' weights first, then their numerators, D threads for the 4 D numbers of one chunk.
 template <int D, bool F16>
 __global__ __launch_bounds__(256) void diff_join_kernel(Args a) {
-    constexpr int PER = 2 * D / 64;
-    const int lane = threadIdx.x & 63;
-    const long id = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (id >= (long)a.B * a.H * a.Nq) return;
-    const int query = id % a.Nq, head = id / a.Nq % a.H, b = id / a.Nq / a.H;
-    const int kvh = head / a.G, R = (head % a.G) * a.Nq + query;
+    constexpr int W = 2 * D, TOGETHER = 256 / D;
+    __shared__ float weight[2][MOST_CHUNKS], top[2][4], sum[2][2][4];
+    __shared__ f32x4 num[256];
+    const int tid = threadIdx.x, wave = tid >> 6;
+    const int query = blockIdx.x % a.Nq, head = blockIdx.x / a.Nq % a.H, b = blockIdx.x / a.Nq / a.H;
+    const int kvh = head / a.G, R = (head % a.G) * a.Nq + query, RT = min(16, a.G * a.Nq);
     const int n = (key_count(a, b) + a.chunk - 1) / a.chunk;              // <= nsplit
-    const long slot = (((long)(b * a.Hkv + kvh) * a.tiles + (R >> 5)) * a.nsplit) * 2;
-    const float* stats = a.part + (long)a.B * a.Hkv * a.tiles * a.nsplit * 2 * 32 * (2 * D) + (slot * 32 + (R & 31)) * 4;
-    const float* num = a.part + (slot * 32 + (R & 31)) * (2 * D) + lane * PER;
-    float out[2][PER];
-    const long row = ((long)b * a.Nq + query) * a.H + head;
+    const long slot = ((long)(b * a.Hkv + kvh) * a.tiles + (R >> 4)) * a.nsplit, slots = (long)a.B * a.Hkv * a.tiles * a.nsplit;
+    const f32x4* stats = (const f32x4*)a.part + slot * 2 * RT + (R & 15);
+    const f32x4* part = (const f32x4*)a.part + slots * 2 * RT + (slot * 2 * RT + (R & 15)) * (W / 4);
+    float M[2] = {NONE, NONE};
+    for (int s = tid; s < n; s += 256)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) M[i] = fmaxf(M[i], weight[i][s] = stats[(s * 2 + i) * RT][0]);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        float M = NONE, L = 0.f, Lx = 0.f;
-        for (int s = lane; s < n; s += 64) M = fmaxf(M, stats[(s * 2 + i) * 128]);
-        M = wave_max(M);
-#pragma unroll
-        for (int e = 0; e < PER; ++e) out[i][e] = 0.f;
-        for (int s = 0; s < n; ++s) {
-            const f32x4 st = *(const f32x4*)(stats + (s * 2 + i) * 128);
-            const float w = __builtin_amdgcn_exp2f(st[0] - M);
-            L += w * st[1];
-            Lx += w * st[2];
-            const float* x = num + (long)(s * 2 + i) * 32 * (2 * D);
-#pragma unroll
-            for (int e = 0; e < PER; ++e) out[i][e] += w * x[e];
-        }
-        const float inv = L > 0.f ? 1.0f / L : L == 0.f ? 0.f : L;
-#pragma unroll
-        for (int e = 0; e < PER; ++e) {
-            out[i][e] *= inv;
-            if (a.maps) a.maps[(i * (long)a.B * a.Nq * a.H + row) * 2 * D + lane * PER + e] = f2h<F16>(out[i][e]);
-        }
-        if (a.maps && lane == 0) put_lse(a.lse + (((long)b * a.H + head) * 4 + i) * a.Nq + query, 2 * a.Nq, M, Lx);
+        M[i] = wave_max(M[i]);
+        if ((tid & 63) == 0) top[i][wave] = M[i];
     }
-    const float lam = a.lam[head * a.lam_stride];
+    __syncthreads();
+    float L[2][2] = {};
 #pragma unroll
-    for (int e = 0; e < PER; ++e) a.o[row * 2 * D + lane * PER + e] = f2h<F16>(out[0][e] - lam * out[1][e]);
+    for (int i = 0; i < 2; ++i) M[i] = fmaxf(fmaxf(top[i][0], top[i][1]), fmaxf(top[i][2], top[i][3]));
+    for (int s = tid; s < n; s += 256)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const float w = __builtin_amdgcn_exp2f(weight[i][s] - M[i]);
+            const f32x4 st = stats[(s * 2 + i) * RT];
+            weight[i][s] = w;
+            L[i][0] += w * st[1];
+            L[i][1] += w * st[2];
+        }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            L[i][k] = wave_sum(L[i][k]);
+            if ((tid & 63) == 0) sum[i][k][wave] = L[i][k];
+        }
+    __syncthreads();
+    const int item = tid % D, map = item / (D / 2), first = tid / D;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    const f32x4* x = part + map * RT * (W / 4) + item % (D / 2);
+#pragma unroll 4
+    for (int s = first; s < n; s += TOGETHER) acc += weight[map][s] * x[(long)s * 2 * RT * (W / 4)];
+    num[tid] = acc;
+    __syncthreads();
+    if (tid >= W) return;
+    const long row = ((long)b * a.Nq + query) * a.H + head;
+    float out[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        out[i] = 0.f;
+#pragma unroll
+        for (int g = 0; g < TOGETHER; ++g) out[i] += ((const float*)num)[g * 4 * D + i * W + tid];
+        const float S = (sum[i][0][0] + sum[i][0][1]) + (sum[i][0][2] + sum[i][0][3]);
+        out[i] *= S > 0.f ? 1.0f / S : S == 0.f ? 0.f : S;                // (a NaN stays one)
+        if (a.maps) a.maps[(i * (long)a.B * a.Nq * a.H + row) * W + tid] = f2h<F16>(out[i]);
+        if (a.maps && tid == 0)
+            put_lse(a.lse + (((long)b * a.H + head) * 4 + i) * a.Nq + query, 2 * a.Nq, M[i], (sum[i][1][0] + sum[i][1][1]) + (sum[i][1][2] + sum[i][1][3]));
+    }
+    a.o[row * W + tid] = f2h<F16>(__builtin_fmaf(-a.lam[head * a.lam_stride], out[1], out[0]));
 }
 
 // ---- backward ----------------------------------------------------------------------------------------------------------------------------------
@@ -960,18 +1006,23 @@ int check(const hs_diff_attn_desc* d, bool backward) {
 bool misaligned(const void* p, unsigned n = 16) { return !p || (uintptr_t)p % n; }
 
 struct Split { int tiles, nsplit, chunk; };
-// Whether the split forward runs, and how it cuts the keys
+constexpr int WANT = 1024;
+// Whether the split forward runs, and how it cuts the keys.  The whole forward needs the time of one block over all keys for each round of its blocks on
+// the 256 CUs, full or not; the split forward's time goes with its tiles, wherever they come from.  Measured with 16 query heads on 4 key heads of 64, 8192
+// keys, whole / split in us: 1 entry, 16 queries 277 / 20, 256 queries 282 / 72; 16 entries, 16 queries 327 / 108, 32 (512 tiles) 311 / 197, 64 (1024 tiles)
+// 319 / 341, 128 339 / 494.  8 on 2 of 128, 16 entries, 512 / 2048 keys: 32 queries (256 tiles) 33, 100 / 35, 68, 64 (512 tiles) 32, 101 / 54, 86.
 Split split_of(const hs_diff_attn_desc* d) {
-    const int64_t rows = (int64_t)(d->H / d->Hkv) * d->Nq, tiles = (rows + 31) / 32;
-    if (rows > 32) return {0, 0, 0};
-    const int64_t blocks = (int64_t)d->B * d->Hkv * tiles;
-    int64_t want = (1024 + blocks - 1) / blocks;
-    int64_t chunk = ((d->Nk + want - 1) / want + 127) / 128 * 128;
-    if (chunk < 256) chunk = 256;
+    const int64_t rows = (int64_t)(d->H / d->Hkv) * d->Nq, tiles = (rows + 15) / 16, blocks = (int64_t)d->B * d->Hkv * tiles;
+    const int own = d->d == 128 ? Sweep<128>::OWN : Sweep<64>::OWN, halves = d->d == 128 ? Sweep<128>::HALVES : 1;
+    const int64_t rounds = ((int64_t)d->B * d->H * ((d->Nq + own - 1) / own) * halves + 255) / 256;
+    if (blocks > rounds * (d->d == 128 ? 256 : 512)) return {0, 0, 0};
+    const int64_t want = std::min<int64_t>((WANT + blocks - 1) / blocks, MOST_CHUNKS);
+    const int64_t chunk = std::max<int64_t>(((d->Nk + want - 1) / want + 127) / 128 * 128, d->d == 128 ? 256 : 512);
     return {(int)tiles, (int)((d->Nk + chunk - 1) / chunk), (int)chunk};
 }
 size_t split_bytes(const hs_diff_attn_desc* d, const Split& s) {
-    return s.nsplit > 1 ? (size_t)d->B * d->Hkv * s.tiles * s.nsplit * 2 * 32 * (2 * d->d + 4) * 4 : 0;
+    const size_t rows = std::min<int64_t>(16, (int64_t)(d->H / d->Hkv) * d->Nq);
+    return s.nsplit > 1 ? (size_t)d->B * d->Hkv * s.tiles * s.nsplit * 2 * rows * (2 * d->d + 4) * 4 : 0;
 }
 Args args_of(const hs_diff_attn_desc* d) {
     Args a = {};
@@ -990,9 +1041,9 @@ template <int D, bool F16, bool KEEP> void forward(const Args& a, const Split& s
     typedef Sweep<D> S;
     constexpr int TILE = S::ROWS * (2 * D + S::VC) * 2;
     if (sp.nsplit) {
-        constexpr int NW = D == 128 ? 2 : 4;
-        launch(diff_split_kernel<D, F16, KEEP, NW>, (int64_t)a.B * a.Hkv * sp.tiles * sp.nsplit * S::HALVES, NW * 64, (size_t)NW * 2 * TILE, s, a);
-        if (sp.nsplit > 1) launch(diff_join_kernel<D, F16>, ((int64_t)a.B * a.H * a.Nq + 3) / 4, 256, 0, s, a);
+        typedef SplitOf<D> P;
+        launch(diff_split_kernel<D, F16, KEEP>, (int64_t)a.B * a.Hkv * sp.tiles * sp.nsplit, P::NW * 64, (size_t)P::NW * P::TILE, s, a);
+        if (sp.nsplit > 1) launch(diff_join_kernel<D, F16>, (int64_t)a.B * a.H * a.Nq, 256, 0, s, a);
         return;
     }
     launch(diff_fwd_kernel<D, F16, KEEP>, (int64_t)a.B * a.H * ((a.Nq + S::OWN - 1) / S::OWN) * S::HALVES, S::NW * 64, (size_t)S::BUFS * TILE, s, a);

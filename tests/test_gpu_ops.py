@@ -217,14 +217,29 @@ def test_diff_attention_values_and_gradients(dev, case):
     assert all(torch.equal(got[n], again[n]) for n in got)                    # no atomics
 
 
+@pytest.mark.parametrize("case", [                             # so many rows that the keys are not cut
+    dict(B=4, Nq=65, Nk=63, Hq=32, Hkv=32, d=64, dtype=F16, causal=True), dict(B=1, Nq=257, Nk=257, Hq=32, Hkv=32, d=64, dtype=BF, causal=True),
+    dict(B=1, Nq=1025, Nk=1030, Hq=8, Hkv=8, d=32, dtype=BF, causal=True), dict(B=1, Nq=130, Nk=300, Hq=32, Hkv=32, d=128, dtype=BF, causal=True),
+    dict(B=3, Nq=40, Nk=200, Hq=32, Hkv=32, d=128, dtype=F16, lens=[0, 1, 200], lam="one"),
+    dict(B=3, Nq=97, Nk=97, Hq=32, Hkv=8, d=32, dtype=BF, causal=True, lens=[0, 50, 97], start=[0, -20, 3]),
+    dict(B=2, Nq=300, Nk=129, Hq=32, Hkv=16, d=64, dtype=BF, causal=True, start=[-40, 100], lam="none"),
+    dict(B=1, Nq=300, Nk=200, Hq=32, Hkv=32, d=64, dtype=BF, grow=36.0), dict(B=4, Nq=70, Nk=333, Hq=32, Hkv=32, d=32, dtype=F16, grow=36.0),
+    dict(B=1, Nq=140, Nk=150, Hq=32, Hkv=32, d=128, dtype=F16, grow=20.0, causal=True), dict(B=2, Nq=300, Nk=190, Hq=16, Hkv=16, d=64, dtype=BF, size=12.0),
+    dict(B=70, Nq=70, Nk=31, Hq=2, Hkv=2, d=64, dtype=F16, scale=0.3)],
+    ids=lambda c: f"{c['B']}x{c['Nq']}x{c['Nk']}-{c['Hq']}/{c['Hkv']}x{c['d']}")
+def test_diff_attention_of_many_rows(dev, case):
+    test_diff_attention_values_and_gradients(dev, case)
+
+
 @pytest.mark.parametrize("d", [32, 64, 128])
 @pytest.mark.parametrize("Nq", [1, 200])
-def test_diff_one_visible_key_gives_its_value(dev, d, Nq):
+@pytest.mark.parametrize("B", [2, 64])
+def test_diff_one_visible_key_gives_its_value(dev, d, Nq, B):
     """softmax of one key is 1, and of two equal keys a half, whatever the scores: no rounding of P may show"""
     g = torch.Generator("cuda").manual_seed(d + Nq)
-    q, k, v = rnd(g, 2, Nq, 4, d, dtype=BF), rnd(g, 2, 300, 4, d, dtype=BF), rnd(g, 2, 300, 2, 2 * d, dtype=BF)
-    k[1, 1], v[1, 1] = k[1, 0], v[1, 0]
-    o = H.diff_attention(q, k, v, torch.tensor([0.5, 0.0], device="cuda"), kv_len=torch.tensor([1, 2], dtype=torch.int32, device="cuda"))
+    q, k, v = rnd(g, B, Nq, 4, d, dtype=BF), rnd(g, B, 300, 4, d, dtype=BF), rnd(g, B, 300, 2, 2 * d, dtype=BF)
+    k[1::2, 1], v[1::2, 1] = k[1::2, 0], v[1::2, 0]
+    o = H.diff_attention(q, k, v, torch.tensor([0.5, 0.0], device="cuda"), kv_len=torch.tensor([1, 2] * (B // 2), dtype=torch.int32, device="cuda"))
     assert torch.equal(o[:, :, 0], (0.5 * v[:, :1, 0]).expand_as(o[:, :, 0])) and torch.equal(o[:, :, 1], v[:, :1, 1].expand_as(o[:, :, 1]))
 
 
