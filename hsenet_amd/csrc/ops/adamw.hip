@@ -3,14 +3,14 @@
 // Bound: HBM.  Per element: p read and written, g read, both moments read and written: 28 bytes with fp32 everywhere, 16 (+ 16 bytes a block of
 // 256 for the scales) with 8-bit moments.  The tensors' addresses travel in the kernel's arguments (no table in device memory that a later
 // call could overwrite while an earlier one still reads it); a block finds its tensor by comparing its number with the tensors' first blocks, a lane
-// each.  One wave owns one block of 256 elements, 4 a lane, so a block's scale is a maximum over the wave and never leaves its registers.
+// each.  Half a wave owns one block of 256 elements, 8 a lane, so a block's scale is a maximum over 32 lanes and never leaves their registers.
 #include "../common.h"
 #include "../../../include/hsenet_ops.h"
 
 namespace {
 
 constexpr int BLOCK = HS_ADAMW_BLOCK;      // elements that share an 8-bit scale
-constexpr int CHUNK = 16 * BLOCK;          // elements of a thread block: 4 waves, 4 blocks of 256 each
+constexpr int CHUNK = 16 * BLOCK;          // elements of a thread block
 constexpr int TENSORS = 56;                // of one launch: 56 * 68 bytes + the rest stay under the 4 KiB of kernel arguments
 constexpr int STEPS = 480;                 // step counters of one launch of the first kernel
 
@@ -48,124 +48,164 @@ template <int DT> __device__ __forceinline__ float get1(const void* p, long i) {
 template <int DT> __device__ __forceinline__ void put1(void* p, long i, float f) {
     if constexpr (DT == HS_PREC_F32) ((float*)p)[i] = f; else ((bf16_t*)p)[i] = f2h<DT == HS_PREC_F16>(f);
 }
-// elements [i, i + 4) of a tensor of n: whole where the tensor's four arrays are aligned for it, else one by one
-template <int DT> __device__ __forceinline__ f32x4 get4(const void* p, long i, long n, bool whole) {
-    f32x4 r = {0.f, 0.f, 0.f, 0.f};
+template <int GAP> __device__ __forceinline__ long nth(long i, int e) { return i + (e >> 2) * GAP + (e & 3); }
+// A lane's 8 elements of a tensor of n: two stretches of 4 that begin at i and GAP further, whole where its arrays are aligned for it, else one by one.
+// In 16 bits they are side by side, one access of 16 bytes; in 32 bits each access of 16 bytes has its neighbours in the lanes beside it.
+template <int DT, int GAP> __device__ __forceinline__ void get8(float (&r)[8], const void* p, long i, long n, bool whole) {
     if (whole) {
-        if constexpr (DT == HS_PREC_F32) r = *(const f32x4*)((const float*)p + i);
-        else {
-            const u32x2 u = *(const u32x2*)((const bf16_t*)p + i);
-            constexpr bool F = DT == HS_PREC_F16;
-            r[0] = unpack_lo<F>(u[0]); r[1] = unpack_hi<F>(u[0]); r[2] = unpack_lo<F>(u[1]); r[3] = unpack_hi<F>(u[1]);
+        if constexpr (DT == HS_PREC_F32) {
+            const f32x4 x = *(const f32x4*)((const float*)p + i), y = *(const f32x4*)((const float*)p + i + GAP);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { r[e] = x[e]; r[4 + e] = y[e]; }
+        } else {
+            static_assert(GAP == 4, "one access");
+            const u32x4 u = *(const u32x4*)((const bf16_t*)p + i);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { r[2 * e] = unpack_lo<DT == HS_PREC_F16>(u[e]); r[2 * e + 1] = unpack_hi<DT == HS_PREC_F16>(u[e]); }
         }
     } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) if (i + e < n) r[e] = get1<DT>(p, i + e);
+        for (int e = 0; e < 8; ++e) r[e] = nth<GAP>(i, e) < n ? get1<DT>(p, nth<GAP>(i, e)) : 0.f;
     }
-    return r;
 }
-template <int DT> __device__ __forceinline__ void put4(void* p, long i, long n, bool whole, f32x4 r) {
+template <int DT, int GAP> __device__ __forceinline__ void put8(void* p, long i, long n, bool whole, const float (&r)[8]) {
     if (whole) {
-        if constexpr (DT == HS_PREC_F32) *(f32x4*)((float*)p + i) = r;
-        else {
-            u32x2 u;
-            u[0] = pack2h<DT == HS_PREC_F16>(r[0], r[1]); u[1] = pack2h<DT == HS_PREC_F16>(r[2], r[3]);
-            *(u32x2*)((bf16_t*)p + i) = u;
+        if constexpr (DT == HS_PREC_F32) {
+            *(f32x4*)((float*)p + i) = f32x4{r[0], r[1], r[2], r[3]};
+            *(f32x4*)((float*)p + i + GAP) = f32x4{r[4], r[5], r[6], r[7]};
+        } else {
+            u32x4 u;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) u[e] = pack2h<DT == HS_PREC_F16>(r[2 * e], r[2 * e + 1]);
+            *(u32x4*)((bf16_t*)p + i) = u;
         }
     } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) if (i + e < n) put1<DT>(p, i + e, r[e]);
+        for (int e = 0; e < 8; ++e) if (nth<GAP>(i, e) < n) put1<DT>(p, nth<GAP>(i, e), r[e]);
     }
 }
-__device__ __forceinline__ unsigned get_codes(const void* p, long i, long n, bool whole) {
-    if (whole) return *(const unsigned*)((const unsigned char*)p + i);
-    unsigned r = 0;
+template <int GAP> __device__ __forceinline__ u32x2 get_codes(const void* p, long i, long n, bool whole) {
+    const unsigned char* c = (const unsigned char*)p;
+    if (whole) return GAP == 4 ? *(const u32x2*)(c + i) : u32x2{*(const unsigned*)(c + i), *(const unsigned*)(c + i + GAP)};
+    u32x2 r = {0, 0};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) if (i + e < n) r |= (unsigned)((const unsigned char*)p)[i + e] << (8 * e);
+    for (int e = 0; e < 8; ++e) if (nth<GAP>(i, e) < n) r[e >> 2] |= (unsigned)c[nth<GAP>(i, e)] << (8 * (e & 3));
     return r;
 }
-__device__ __forceinline__ void put_codes(void* p, long i, long n, bool whole, unsigned c) {
-    if (whole) { *(unsigned*)((unsigned char*)p + i) = c; return; }
+template <int GAP> __device__ __forceinline__ void put_codes(void* p, long i, long n, bool whole, u32x2 r) {
+    unsigned char* c = (unsigned char*)p;
+    if (whole) {
+        if (GAP == 4) *(u32x2*)(c + i) = r;
+        else { *(unsigned*)(c + i) = r[0]; *(unsigned*)(c + i + GAP) = r[1]; }
+        return;
+    }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) if (i + e < n) ((unsigned char*)p)[i + e] = (unsigned char)(c >> (8 * e));
+    for (int e = 0; e < 8; ++e) if (nth<GAP>(i, e) < n) c[nth<GAP>(i, e)] = (unsigned char)(r[e >> 2] >> (8 * (e & 3)));
 }
-__device__ __forceinline__ float m_of(float s, unsigned codes, int e) {
-    const float r = (float)(int)(signed char)(codes >> (8 * e)) * (1.0f / 127.0f);
-    return s * (r * fabsf(r));
+__device__ __forceinline__ void moments_of(float (&m)[8], float (&v)[8], u32x2 cm, u32x2 cv, float sm, float su) {
+    sm *= 1.0f / (127 * 127);
+    su *= 1.0f / (255 * 255);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float r = (float)(int)(signed char)(cm[e >> 2] >> (8 * (e & 3))), w = (float)((cv[e >> 2] >> (8 * (e & 3))) & 255u), u = su * (w * w);
+        m[e] = sm * (r * fabsf(r));
+        v[e] = u * u;
+    }
 }
-__device__ __forceinline__ float u_of(float s, unsigned codes, int e) {
-    const float r = (float)((codes >> (8 * e)) & 255u) * (1.0f / 255.0f);
-    return s * (r * r);
+// square root to a last place: the instruction takes what is below the normal numbers for 0
+__device__ __forceinline__ float root(float x) {
+    const bool tiny = x < 0x1p-96f;
+    return __builtin_amdgcn_sqrtf(x * (tiny ? 0x1p64f : 1.0f)) * (tiny ? 0x1p-32f : 1.0f);
 }
-// largest of a block's values (all >= 0, or NaN) over the wave, and NaN where one of them is not finite
-__device__ __forceinline__ float block_scale(f32x4 a) {
-    const float s = wave_max(fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])));
-    const float sum = (a[0] + a[1]) + (a[2] + a[3]);       // NaN exactly where one of them is (they are >= 0)
-    return __builtin_amdgcn_ballot_w64(sum != sum) || !(s < __builtin_inff()) ? __builtin_nanf("") : s;
+template <int CTRL> __device__ __forceinline__ unsigned moved(unsigned x) { return (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xf, 0xf, true); }
+// Largest of a block's values (all >= 0, or NaN) over its 32 lanes, and NaN where one of them is not finite: as whole numbers, the bits of what is not
+// finite are larger than all others.
+__device__ __forceinline__ float block_scale(const float (&a)[8]) {
+    unsigned s = __builtin_bit_cast(unsigned, a[0]);
+#pragma unroll
+    for (int e = 1; e < 8; ++e) s = max(s, __builtin_bit_cast(unsigned, a[e]));
+    s = max(s, moved<0xB1>(s));                                           // lanes that differ in bit 0, bit 1; the other 4 of 8; the other 8 of 16
+    s = max(s, moved<0x4E>(s));
+    s = max(s, moved<0x141>(s));
+    s = max(s, moved<0x140>(s));
+    s = max(s, (unsigned)__shfl_xor((int)s, 16, 64));
+    return s < 0x7f800000u ? __builtin_bit_cast(float, s) : __builtin_nanf("");
+}
+// The nearest whole number of x f, below 2^22, in the low bits (two's complement) of a float whose last place is 1; and the low bytes of four of these.
+__device__ __forceinline__ unsigned whole_bits(float x, float f) { return __builtin_bit_cast(unsigned, __builtin_fmaf(x, f, 12582912.0f)); }
+__device__ __forceinline__ unsigned low_bytes(unsigned a, unsigned b, unsigned c, unsigned d) {
+    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, 0x0c0c0400u), __builtin_amdgcn_perm(b, a, 0x0c0c0400u), 0x05040100u);
+}
+
+// A thread block's elements: two blocks of 256 for each half of a wave.
+constexpr int TURNS = CHUNK / (256 * 8);
+template <int DT> constexpr int GAP_OF = DT == HS_PREC_F32 ? BLOCK / 2 : 4;
+struct Place { long i, blk; };
+template <int GAP> __device__ __forceinline__ Place place_of(const Table& a, int k, int turn) {
+    const long blk = (long)(blockIdx.x - a.first[k]) * (CHUNK / BLOCK) + turn * 8 + (threadIdx.x >> 5);
+    return {blk * BLOCK + (threadIdx.x & 31) * (GAP == 4 ? 8 : 4), blk};
 }
 
 template <int DT, bool BITS8>
 __global__ __launch_bounds__(256) void adamw_kernel(Table a) {
     const int k = find_tensor(a);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     void* p = a.p[k];
     const void* g = a.g[k];
     void *m = a.m[k], *v = a.v[k];
     const long n = a.n[k];
-    const float c1 = ((const float*)a.step[k])[1], c2 = ((const float*)a.step[k])[2];
-    constexpr unsigned PA = DT == HS_PREC_F32 ? 15 : 7, SA = BITS8 ? 3 : 15;
-    const bool aligned = !((((uintptr_t)p | (uintptr_t)g) & PA) | (((uintptr_t)m | (uintptr_t)v) & SA));
-    const float step_size = a.lr * c1;
-    const long base = (long)(blockIdx.x - a.first[k]) * CHUNK;
+    constexpr int GAP = GAP_OF<DT>;
+    const bool aligned = !((((uintptr_t)p | (uintptr_t)g) & 15) | (((uintptr_t)m | (uintptr_t)v) & (BITS8 ? 7 : 15)));
+    float pv[TURNS][8], gv[TURNS][8], mv[TURNS][8], vv[TURNS][8], sm[TURNS], su[TURNS];
+    u32x2 cm[TURNS], cv[TURNS];
 #pragma unroll
-    for (int it = 0; it < CHUNK / (4 * BLOCK); ++it) {
-        const long blk = base / BLOCK + it * 4 + wave, i = blk * BLOCK + lane * 4;
-        if (blk * BLOCK >= n) break;
-        const bool whole = aligned && i + 4 <= n;
-        f32x4 pv = get4<DT>(p, i, n, whole);
-        const f32x4 gv = get4<DT>(g, i, n, whole);
-        f32x4 mv, vv;
+    for (int t = 0; t < TURNS; ++t) {                                     // everything is sent for before anything is used
+        const Place at = place_of<GAP>(a, k, t);
+        const bool whole = aligned && at.i + GAP + 4 <= n, some = at.blk * BLOCK < n;
+        get8<DT, GAP>(pv[t], p, at.i, n, whole);
+        get8<DT, GAP>(gv[t], g, at.i, n, whole);
         if constexpr (BITS8) {
-            const float sm = a.ms[k][blk], su = a.vs[k][blk];
-            const unsigned cm = get_codes(m, i, n, whole), cv = get_codes(v, i, n, whole);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                mv[e] = m_of(sm, cm, e);
-                const float u = u_of(su, cv, e);
-                vv[e] = u * u;
-            }
+            cm[t] = get_codes<GAP>(m, at.i, n, whole);
+            cv[t] = get_codes<GAP>(v, at.i, n, whole);
+            sm[t] = some ? a.ms[k][at.blk] : 0.f;
+            su[t] = some ? a.vs[k][at.blk] : 0.f;
         } else {
-            mv = get4<HS_PREC_F32>(m, i, n, whole);
-            vv = get4<HS_PREC_F32>(v, i, n, whole);
+            get8<HS_PREC_F32, GAP>(mv[t], m, at.i, n, whole);
+            get8<HS_PREC_F32, GAP>(vv[t], v, at.i, n, whole);
         }
-        f32x4 am, uv;
+    }
+    const float step_size = a.lr * ((const float*)a.step[k])[1], c2 = ((const float*)a.step[k])[2];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            mv[e] = mv[e] * a.beta1 + gv[e] * a.rest1;
-            vv[e] = vv[e] * a.beta2 + gv[e] * gv[e] * a.rest2;
-            uv[e] = sqrtf(vv[e]);
-            am[e] = fabsf(mv[e]);
-            pv[e] = pv[e] * a.keep - step_size * mv[e] / (uv[e] * c2 + a.eps);
+    for (int t = 0; t < TURNS; ++t) {
+        const Place at = place_of<GAP>(a, k, t);
+        const bool whole = aligned && at.i + GAP + 4 <= n;
+        float am[8], uv[8];
+        if constexpr (BITS8) moments_of(mv[t], vv[t], cm[t], cv[t], sm[t], su[t]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            mv[t][e] = mv[t][e] * a.beta1 + gv[t][e] * a.rest1;
+            vv[t][e] = vv[t][e] * a.beta2 + gv[t][e] * gv[t][e] * a.rest2;
+            uv[e] = root(vv[t][e]);
+            am[e] = fabsf(mv[t][e]);
+            pv[t][e] = pv[t][e] * a.keep - step_size * mv[t][e] * __builtin_amdgcn_rcpf(uv[e] * c2 + a.eps);      // (to a last place)
         }
-        put4<DT>(p, i, n, whole, pv);
+        put8<DT, GAP>(p, at.i, n, whole, pv[t]);
         if constexpr (BITS8) {
-            const float sm = block_scale(am), su = block_scale(uv);
-            const float im = sm > 0.f ? 1.0f / sm : 0.f, iu = su > 0.f ? 1.0f / su : 0.f;
-            unsigned cm = 0, cv = 0;
+            const float Sm = block_scale(am), Su = block_scale(uv);
+            const float im = Sm >= 0x1p-126f ? 1.0f / Sm : 0.f, iu = Su > 0.f ? 255.0f * 255 / Su : 0.f;      // (Su: 0 or at least 2^-75)
+            unsigned wm[8], wv[8];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int c = (int)fminf(rintf(sqrtf(am[e] * im) * 127.0f), 127.0f);
-                cm |= (unsigned)((mv[e] < 0.f ? -c : c) & 255) << (8 * e);
-                int u = (int)fminf(rintf(sqrtf(uv[e] * iu) * 255.0f), 255.0f);
-                u = uv[e] > 0.f ? max(u, 1) : u;
-                cv |= (unsigned)(u & 255) << (8 * e);
+            for (int e = 0; e < 8; ++e) {                                 // (roots to a last place; what is not 0 is not taken for 0 in the second moment)
+                wm[e] = whole_bits(copysignf(__builtin_amdgcn_sqrtf(am[e] * im), mv[t][e]), 127.0f);
+                wv[e] = whole_bits(fmaxf(__builtin_amdgcn_sqrtf(uv[e] * iu), __builtin_amdgcn_fmed3f(uv[e] * 0x1p100f, 0.f, 1.0f)), 1.0f);
             }
-            put_codes(m, i, n, whole, cm);
-            put_codes(v, i, n, whole, cv);
-            if (lane == 0) { a.ms[k][blk] = sm; a.vs[k][blk] = su; }
+            const u32x2 nm = {low_bytes(wm[0], wm[1], wm[2], wm[3]), low_bytes(wm[4], wm[5], wm[6], wm[7])};
+            const u32x2 nv = {low_bytes(wv[0], wv[1], wv[2], wv[3]), low_bytes(wv[4], wv[5], wv[6], wv[7])};
+            put_codes<GAP>(m, at.i, n, whole, nm);
+            put_codes<GAP>(v, at.i, n, whole, nv);
+            if ((threadIdx.x & 31) == 0 && at.i < n) { a.ms[k][at.blk] = Sm; a.vs[k][at.blk] = Su; }
         } else {
-            put4<HS_PREC_F32>(m, i, n, whole, mv);
-            put4<HS_PREC_F32>(v, i, n, whole, vv);
+            put8<HS_PREC_F32, GAP>(m, at.i, n, whole, mv[t]);
+            put8<HS_PREC_F32, GAP>(v, at.i, n, whole, vv[t]);
         }
     }
 }
@@ -174,28 +214,29 @@ __global__ __launch_bounds__(256) void adamw_kernel(Table a) {
 template <int DT>
 __global__ __launch_bounds__(256) void adamw_moments_kernel(Table a) {
     const int k = find_tensor(a);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     void *om = a.p[k], *ov = (void*)a.g[k];
     const long n = a.n[k];
-    constexpr unsigned PA = DT == HS_PREC_F32 ? 15 : 7;
-    const bool aligned = !((((uintptr_t)om | (uintptr_t)ov) & PA) | (((uintptr_t)a.m[k] | (uintptr_t)a.v[k]) & 3));
-    const long base = (long)(blockIdx.x - a.first[k]) * CHUNK;
+    constexpr int GAP = GAP_OF<DT>;
+    const bool aligned = !((((uintptr_t)om | (uintptr_t)ov) & 15) | (((uintptr_t)a.m[k] | (uintptr_t)a.v[k]) & 7));
+    u32x2 cm[TURNS], cv[TURNS];
+    float sm[TURNS], su[TURNS];
 #pragma unroll
-    for (int it = 0; it < CHUNK / (4 * BLOCK); ++it) {
-        const long blk = base / BLOCK + it * 4 + wave, i = blk * BLOCK + lane * 4;
-        if (blk * BLOCK >= n) break;
-        const bool whole = aligned && i + 4 <= n;
-        const float sm = a.ms[k][blk], su = a.vs[k][blk];
-        const unsigned cm = get_codes(a.m[k], i, n, whole), cv = get_codes(a.v[k], i, n, whole);
-        f32x4 mv, vv;
+    for (int t = 0; t < TURNS; ++t) {
+        const Place at = place_of<GAP>(a, k, t);
+        const bool whole = aligned && at.i + GAP + 4 <= n, some = at.blk * BLOCK < n;
+        cm[t] = get_codes<GAP>(a.m[k], at.i, n, whole);
+        cv[t] = get_codes<GAP>(a.v[k], at.i, n, whole);
+        sm[t] = some ? a.ms[k][at.blk] : 0.f;
+        su[t] = some ? a.vs[k][at.blk] : 0.f;
+    }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            mv[e] = m_of(sm, cm, e);
-            const float u = u_of(su, cv, e);
-            vv[e] = u * u;
-        }
-        put4<DT>(om, i, n, whole, mv);
-        put4<DT>(ov, i, n, whole, vv);
+    for (int t = 0; t < TURNS; ++t) {
+        const Place at = place_of<GAP>(a, k, t);
+        const bool whole = aligned && at.i + GAP + 4 <= n;
+        float mv[8], vv[8];
+        moments_of(mv, vv, cm[t], cv[t], sm[t], su[t]);
+        put8<DT, GAP>(om, at.i, n, whole, mv);
+        put8<DT, GAP>(ov, at.i, n, whole, vv);
     }
 }
 
