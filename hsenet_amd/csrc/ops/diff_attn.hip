@@ -19,7 +19,8 @@ constexpr float NONE = -1e30f;                 // running maximum before the fir
 constexpr float HEADROOM = 8.0f;               // a running maximum is kept until a score passes it by this many powers of two
 constexpr int SHIFT16 = 4;                     // fp16: P and dS of the backward pass are held times 2^4
 
-constexpr int MOST_CHUNKS = 512;             // of a row's keys
+typedef __attribute__((ext_vector_type(2))) float f32x2;
+constexpr int MOST_CHUNKS = 512;               // of a row's keys
 
 struct Args {
     const bf16_t *q, *k, *v, *go;
@@ -209,6 +210,25 @@ __device__ __forceinline__ void softmax_weights(f32x16& s, float c2, float m, fl
         for (int e = 0; e < 4; ++e) part[e & 1] = add2<F16>(w[e], part[e & 1]);
     }
     l[0] += part[0] + part[1];
+}
+// numerators in two numbers of 16 bits, value and what its rounding left, and their sum
+template <bool F16>
+__device__ __forceinline__ void two_part_weights(f32x16& s, float c2, float m, float& l, bf16x8 (&p)[2], bf16x8 (&rest)[2]) {
+    float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c2, -m));
+        part[r & 3] += s[r];
+    }
+    l += (part[0] + part[1]) + (part[2] + part[3]);
+#pragma unroll
+    for (int sp = 0; sp < 2; ++sp) {
+        p[sp] = pack8<F16>(s, sp);
+        const u32x4 w = __builtin_bit_cast(u32x4, p[sp]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[8 * sp + e] -= e & 1 ? unpack_hi<F16>(w[e >> 1]) : unpack_lo<F16>(w[e >> 1]);
+        rest[sp] = pack8<F16>(s, sp);
+    }
 }
 // What the backward pass needs of a row's softmax: P = 2^(c2 s - hi - lo), hi whole (the reference m is), 0 <= lo < 1.  One fp32 number of their sum's
 // size would put a common error of 5e-7 on all of a row's P, which the sum that is lam's gradient would keep.
@@ -421,7 +441,8 @@ __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void d
 // pairs, under both maps: column c is map c / 16 of row c % 16.  q K^T is made of both maps for all columns, and each column keeps its own; the softmax and
 // the products with V then go over both maps at once.  A block takes one chunk of the keys, each of its waves every NW-th tile of 32 keys through LDS of
 // its own (no barrier in the loop): the next tile's keys are sent for when the scores have been read, its values behind the products with V, so that
-// half a tile a wave is always on its way.  The waves' numerators are joined in LDS, and the chunks' by diff_join_kernel; with one chunk the result is
+// half a tile a wave is always on its way.  Bandwidth leaves the matrix pipe room enough to take P in two numbers of 16 bits, value and what its rounding
+// left, so that o is rounded once, at its end.  The waves' numerators are joined in LDS, and the chunks' by diff_join_kernel; with one chunk the result is
 // written at once.
 template <int D> struct SplitOf { static constexpr int NW = D == 128 ? 2 : 4, TILE = 32 * 4 * D * 2; };
 
@@ -429,8 +450,7 @@ template <int D, bool F16, bool KEEP>
 __global__ __launch_bounds__(SplitOf<D>::NW * 64, D == 128 ? 1 : 2) void diff_split_kernel(Args a) {
     constexpr int ROWS = 32, NW = SplitOf<D>::NW, TILE = SplitOf<D>::TILE, W = 2 * D, NB = W / 32, NT = NW * 64, PER = 4 * W / NT;
     extern __shared__ __attribute__((aligned(16))) char smem[];           // a tile a wave; then the waves' numerators
-    constexpr int SUMS = KEEP ? 2 : 1;
-    __shared__ float wm[NW][32], wl[SUMS][NW][32], total[32];
+    __shared__ float wm[NW][32], wl[NW][32], total[32];
     const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, c = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int id = blockIdx.x;
@@ -468,7 +488,7 @@ __global__ __launch_bounds__(SplitOf<D>::NW * 64, D == 128 ? 1 : 2) void diff_sp
     Tiles dma;
     dma.init(0, lane, a.k + b * a.k_b + 2 * kvh * a.k_h, a.k_n, a.k_h, a.v + b * a.v_b + kvh * a.v_h, a.v_n, k0 + wave * ROWS, k1);
     dma.issue(at);
-    float m = NONE, l[SUMS] = {};
+    float m = NONE, l[1] = {0.f};
     f32x16 o[NB];
     clear(o);
     arrived();
@@ -484,9 +504,9 @@ __global__ __launch_bounds__(SplitOf<D>::NW * 64, D == 128 ? 1 : 2) void diff_sp
         if (t + ROWS > lim_lo)
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[0][r] = acc_row(r, h) < lim - t ? s[0][r] : -__builtin_inff();
-        bf16x8 p[2];
+        bf16x8 p[2], rest[2];
         follow_max(s[0], a.c2, m, l, o);
-        softmax_weights<F16>(s[0], a.c2, m, l, p);
+        two_part_weights<F16>(s[0], a.c2, m, l[0], p, rest);
         Tiles::template landed<KEYS>();
         constexpr int N = 2 * NB, AHEAD = 4;
         bf16x8 x[AHEAD];
@@ -495,6 +515,7 @@ __global__ __launch_bounds__(SplitOf<D>::NW * 64, D == 128 ? 1 : 2) void diff_sp
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             o[n % NB] = mfma32<F16>(x[n % AHEAD], p[n / NB], o[n % NB]);
+            o[n % NB] = mfma32<F16>(x[n % AHEAD], rest[n / NB], o[n % NB]);
             if (n + AHEAD < N) x[n % AHEAD] = f.template cols32<ROWS>(16 * ((n + AHEAD) / NB), W + (n + AHEAD) % NB * 32);
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                // (and of the values)
@@ -502,11 +523,8 @@ __global__ __launch_bounds__(SplitOf<D>::NW * 64, D == 128 ? 1 : 2) void diff_sp
     }
     Tiles::landed();                                                      // (the numerators go where the tiles were)
     if (h == 0) wm[wave][c] = m;
-#pragma unroll
-    for (int k = 0; k < SUMS; ++k) {
-        l[k] += __shfl_xor(l[k], 32, 64);
-        if (h == 0) wl[k][wave][c] = l[k];
-    }
+    l[0] += __shfl_xor(l[0], 32, 64);
+    if (h == 0) wl[wave][c] = l[0];
     __syncthreads();
     const long slot = ((long)(b * a.Hkv + kvh) * a.tiles + tile) * a.nsplit + split;
     f32x4* num = (f32x4*)smem;                                            // [wave][32][W / 4], vectors exchanged within 8 by the row's number
@@ -522,18 +540,16 @@ __global__ __launch_bounds__(SplitOf<D>::NW * 64, D == 128 ? 1 : 2) void diff_sp
                 num[(wave * 32 + c) * (W / 4) + ((db * 8 + 2 * g + h) ^ (c & 7))] =
                     f32x4{o[db][4 * g] * mine, o[db][4 * g + 1] * mine, o[db][4 * g + 2] * mine, o[db][4 * g + 3] * mine};
         if (tid < 32) {
-            float L[SUMS] = {};
+            float L = 0.f;
 #pragma unroll
-            for (int k = 0; k < SUMS; ++k)
-#pragma unroll
-                for (int w = 0; w < NW; ++w) L[k] += wl[k][w][c] * __builtin_amdgcn_exp2f(wm[w][c] - M);
-            total[c] = L[0];
-            if (a.nsplit > 1) ((f32x4*)a.part)[(slot * 2 + (c >> 4)) * RT + (c & 15)] = f32x4{M, L[0], L[SUMS - 1], 0.f};
-            else if (KEEP) put_lse(a.lse + (((long)b * a.H + head) * 4 + (c >> 4)) * a.Nq + query, 2 * a.Nq, M, L[SUMS - 1]);
+            for (int w = 0; w < NW; ++w) L += wl[w][c] * __builtin_amdgcn_exp2f(wm[w][c] - M);
+            total[c] = L;
+            if (a.nsplit > 1) ((f32x2*)a.part)[(slot * 2 + (c >> 4)) * RT + (c & 15)] = f32x2{M, L};
+            else if (KEEP) put_lse(a.lse + (((long)b * a.H + head) * 4 + (c >> 4)) * a.Nq + query, 2 * a.Nq, M, L);
         }
     }
     __syncthreads();
-    f32x4* part = (f32x4*)a.part + (long)a.B * a.Hkv * a.tiles * a.nsplit * 2 * RT;
+    f32x4* part = (f32x4*)a.part + (long)a.B * a.Hkv * a.tiles * a.nsplit * RT;
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
         const int r = (e * NT + tid) / (W / 4), at4 = (e * NT + tid) % (W / 4);
@@ -569,15 +585,15 @@ __global__ __launch_bounds__(SplitOf<D>::NW * 64, D == 128 ? 1 : 2) void diff_sp
 template <int D, bool F16>
 __global__ __launch_bounds__(256) void diff_join_kernel(Args a) {
     constexpr int W = 2 * D, TOGETHER = 256 / D;
-    __shared__ float weight[2][MOST_CHUNKS], top[2][4], sum[2][2][4];
+    __shared__ float weight[2][MOST_CHUNKS], top[2][4], sum[2][4];
     __shared__ f32x4 num[256];
     const int tid = threadIdx.x, wave = tid >> 6;
     const int query = blockIdx.x % a.Nq, head = blockIdx.x / a.Nq % a.H, b = blockIdx.x / a.Nq / a.H;
     const int kvh = head / a.G, R = (head % a.G) * a.Nq + query, RT = min(16, a.G * a.Nq);
     const int n = (key_count(a, b) + a.chunk - 1) / a.chunk;              // <= nsplit
     const long slot = ((long)(b * a.Hkv + kvh) * a.tiles + (R >> 4)) * a.nsplit, slots = (long)a.B * a.Hkv * a.tiles * a.nsplit;
-    const f32x4* stats = (const f32x4*)a.part + slot * 2 * RT + (R & 15);
-    const f32x4* part = (const f32x4*)a.part + slots * 2 * RT + (slot * 2 * RT + (R & 15)) * (W / 4);
+    const f32x2* stats = (const f32x2*)a.part + slot * 2 * RT + (R & 15);
+    const f32x4* part = (const f32x4*)a.part + slots * RT + (slot * 2 * RT + (R & 15)) * (W / 4);
     float M[2] = {NONE, NONE};
     for (int s = tid; s < n; s += 256)
 #pragma unroll
@@ -588,25 +604,21 @@ __global__ __launch_bounds__(256) void diff_join_kernel(Args a) {
         if ((tid & 63) == 0) top[i][wave] = M[i];
     }
     __syncthreads();
-    float L[2][2] = {};
+    float L[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < 2; ++i) M[i] = fmaxf(fmaxf(top[i][0], top[i][1]), fmaxf(top[i][2], top[i][3]));
     for (int s = tid; s < n; s += 256)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const float w = __builtin_amdgcn_exp2f(weight[i][s] - M[i]);
-            const f32x4 st = stats[(s * 2 + i) * RT];
             weight[i][s] = w;
-            L[i][0] += w * st[1];
-            L[i][1] += w * st[2];
+            L[i] += w * stats[(s * 2 + i) * RT][1];
         }
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            L[i][k] = wave_sum(L[i][k]);
-            if ((tid & 63) == 0) sum[i][k][wave] = L[i][k];
-        }
+    for (int i = 0; i < 2; ++i) {
+        L[i] = wave_sum(L[i]);
+        if ((tid & 63) == 0) sum[i][wave] = L[i];
+    }
     __syncthreads();
     const int item = tid % D, map = item / (D / 2), first = tid / D;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
@@ -623,11 +635,10 @@ __global__ __launch_bounds__(256) void diff_join_kernel(Args a) {
         out[i] = 0.f;
 #pragma unroll
         for (int g = 0; g < TOGETHER; ++g) out[i] += ((const float*)num)[g * 4 * D + i * W + tid];
-        const float S = (sum[i][0][0] + sum[i][0][1]) + (sum[i][0][2] + sum[i][0][3]);
+        const float S = (sum[i][0] + sum[i][1]) + (sum[i][2] + sum[i][3]);
         out[i] *= S > 0.f ? 1.0f / S : S == 0.f ? 0.f : S;                // (a NaN stays one)
         if (a.maps) a.maps[(i * (long)a.B * a.Nq * a.H + row) * W + tid] = f2h<F16>(out[i]);
-        if (a.maps && tid == 0)
-            put_lse(a.lse + (((long)b * a.H + head) * 4 + i) * a.Nq + query, 2 * a.Nq, M[i], (sum[i][1][0] + sum[i][1][1]) + (sum[i][1][2] + sum[i][1][3]));
+        if (a.maps && tid == 0) put_lse(a.lse + (((long)b * a.H + head) * 4 + i) * a.Nq + query, 2 * a.Nq, M[i], S);
     }
     a.o[row * W + tid] = f2h<F16>(__builtin_fmaf(-a.lam[head * a.lam_stride], out[1], out[0]));
 }
@@ -1022,7 +1033,7 @@ Split split_of(const hs_diff_attn_desc* d) {
 }
 size_t split_bytes(const hs_diff_attn_desc* d, const Split& s) {
     const size_t rows = std::min<int64_t>(16, (int64_t)(d->H / d->Hkv) * d->Nq);
-    return s.nsplit > 1 ? (size_t)d->B * d->Hkv * s.tiles * s.nsplit * 2 * rows * (2 * d->d + 4) * 4 : 0;
+    return s.nsplit > 1 ? (size_t)d->B * d->Hkv * s.tiles * s.nsplit * 2 * rows * (2 * d->d + 2) * 4 : 0;
 }
 Args args_of(const hs_diff_attn_desc* d) {
     Args a = {};
