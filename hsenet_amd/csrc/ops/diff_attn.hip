@@ -28,11 +28,12 @@ struct Args {
     const int *q_start, *kv_len;
     bf16_t *o, *maps;
     float* lse;                                // [B][H][hi of both maps, lo of both][Nq] (put_lse); hi = +inf: no visible key
+    f32x4* sums;                               // backward: parts of dk and dv
     float *D, *x2, *rc;                        // backward: D_m [B][H][2][Nq], D_2 in full precision [B][H][Nq], constants of the rows (diff_rows_kernel)
     bf16_t *dq, *dk, *dv;
     float* part;                               // split forward: numerators, then (maximum, sum)
     long q_b, q_n, q_h, k_b, k_n, k_h, v_b, v_n, v_h, go_b, go_n, go_h;
-    int B, Nq, Nk, H, Hkv, G, causal, q_start0, lam_stride, nsplit, chunk, tiles;
+    int B, Nq, Nk, H, Hkv, G, causal, q_start0, lam_stride, nsplit, chunk, tiles, parts;
     float c2, scale;                           // scale * log2(e), scale
 };
 
@@ -829,7 +830,7 @@ __device__ __forceinline__ void mask_queries(f32x16 (&s)[2], int vis, int h) {
 
 // At d = 64 the wave's keys lie in LDS and its values in registers: all of both would leave the fragments no room in the 256 registers of two waves
 // a SIMD.
-template <int D, bool F16>
+template <int D, bool F16, bool CUT>
 __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void diff_dkv_kernel(Args a) {
     typedef Sweep<D> S;
     constexpr int ROWS = S::ROWS, TILE = S::TILE, NW = S::NW, KEYS = S::OWN, NBUF = S::BUFS, NEVER = 0x7fffffff, NQ = D / 32;
@@ -841,12 +842,17 @@ __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void d
     int id = block_order();
     const int blk = id % nblk;                                            // under a causal mask the first keys have most to do: first
     id /= nblk;
-    const int kvh = id % a.Hkv, b = id / a.Hkv;
+    const int kvh = id % a.Hkv;
+    id /= a.Hkv;
+    const int b = CUT ? id % a.B : id, part = CUT ? id / a.B : 0;
     const int len = key_count(a, b), start = first_pos(a, b);
     const int kb = blk * KEYS, k0 = kb + wave * 32, key = k0 + c;
     // first query that sees the block's first key; the tiles of a head begin at its tile
     const int t0 = (a.causal ? max(0, kb - start) : 0) / ROWS, qt = (a.Nq + ROWS - 1) / ROWS;
-    const int per = kb < len ? max(0, qt - t0) : 0, nj = per * a.G;
+    // the block's list of tiles, head by head, and its part of it
+    const int per = kb < len ? max(0, qt - t0) : 0, all = per * a.G;
+    const int j0 = CUT ? (int)((long)all * part / a.parts) : 0, nj = CUT ? (int)((long)all * (part + 1) / a.parts) - j0 : all;
+    const int g0 = CUT && per ? j0 / per : 0, first = CUT && per ? t0 + j0 % per : t0;
     // first query row that sees a key (NEVER: the key does not count)
     auto sees = [&](int key) { return key >= len ? NEVER : a.causal ? key - start : -(1 << 30); };
     const int vis = sees(key), vis_all = sees(k0 + 31);
@@ -858,16 +864,15 @@ __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void d
     fl.init(smem, lane);
     ol.init(own, lane);
     Dma<D, 2 * D, ROWS, NW> dma;
-    // the block's list of tiles, head by head: what is sent next
-    int sg = 0, st = t0, sbuf = 0;
+    int sg = g0, st = first, sbuf = 0;                                    // what is sent next
     const char* srow = nullptr;                                           // the tile's row constants
     auto head_start = [&]() {
         const int head = kvh * a.G + sg;
-        dma.start(a.q + b * a.q_b + 2 * head * a.q_h, a.go + b * a.go_b + head * a.go_h, t0 * ROWS, a.Nq);
-        srow = (const char*)(a.rc + (((long)b * a.H + head) * qt + t0) * 128) + wave * 256;
+        dma.start(a.q + b * a.q_b + 2 * head * a.q_h, a.go + b * a.go_b + head * a.go_h, st * ROWS, a.Nq);
+        srow = (const char*)(a.rc + (((long)b * a.H + head) * qt + st) * 128) + wave * 256;
     };
     dma.init(wave, lane, a.q, a.q_n, a.q_h, a.go, a.go_n, 0, 0);
-    head_start();
+    if (!CUT || nj > 0) head_start();
     auto send = [&]() {
         dma.issue(lds0 + sbuf * TILE);
         if (wave < 2) {
@@ -934,8 +939,8 @@ __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void d
     __syncthreads();
     next_scores(0);                                                       // (without a tile, or behind the last: of what lies there, not used)
     S::fall_behind(wave);
-    int buf = 0, g = 0, tq = t0;
-    float sign = copysignf(1.0f, a.lam[kvh * a.G * a.lam_stride]);
+    int buf = 0, g = g0, tq = first;
+    float sign = copysignf(1.0f, a.lam[(kvh * a.G + (CUT && nj > 0 ? g0 : 0)) * a.lam_stride]);
     for (int j = 0; j < nj; ++j) {
         S::template before_vector<decltype(dma)>();
         if (j + S::LEAD < nj) send();
@@ -972,12 +977,47 @@ __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void d
         __syncthreads();
     }
     S::wait_for_late(wave);
+    if (CUT) {                                                            // [part][32 keys][32 columns][a lane's 4 at a time], for diff_dkv_join_kernel
+        f32x4* to = a.sums + ((((long)part * a.B + b) * a.Hkv + kvh) * nblk * NW + blk * NW + wave) * (4 * NQ * 256) + lane;
+#pragma unroll
+        for (int n = 0; n < 4 * NQ; ++n) {
+            const f32x16& x = n < 2 * NQ ? dk[n / NQ % 2][n % NQ] : dv[n < 2 * NQ ? 0 : n - 2 * NQ];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) to[n * 256 + i * 64] = f32x4{x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]};
+        }
+        return;
+    }
     if (key >= a.Nk) return;
     const float down = F16 ? 1.0f / (1 << SHIFT16) : 1.0f;
     const long row = ((long)b * a.Nk + key) * a.Hkv + kvh;
     store_rows<F16>(a.dv + row * 2 * D, dv, down, h);
     store_rows<F16>(a.dk + row * 2 * D, dk[0], a.scale * down, h);
     store_rows<F16>(a.dk + row * 2 * D + D, dk[1], a.scale * down, h);
+}
+
+// the sum of the parts of dk and dv, in their order: a wave 32 keys by 32 columns of [dk1 | dk2 | dv]
+template <int D, bool F16>
+__global__ __launch_bounds__(256) void diff_dkv_join_kernel(Args a) {
+    constexpr int NQ = D / 32, PER = 4 * NQ;
+    const int lane = threadIdx.x & 63, h = lane >> 5, nk = (a.Nk + Sweep<D>::OWN - 1) / Sweep<D>::OWN * Sweep<D>::NW;
+    const long piece = (long)blockIdx.x * 4 + (threadIdx.x >> 6), pieces = (long)a.B * a.Hkv * nk * PER;
+    if (piece >= pieces) return;
+    const int n = piece % PER, key = (int)(piece / PER % nk) * 32 + (lane & 31), kvh = piece / PER / nk % a.Hkv;
+    const long b = piece / PER / nk / a.Hkv;
+    if (key >= a.Nk) return;
+    const f32x4* from = a.sums + piece * 256 + lane;
+    f32x16 x[1] = {zero16()};
+    for (int p = 0; p < a.parts; ++p)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const f32x4 t = from[p * pieces * 256 + i * 64];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[0][4 * i + e] += t[e];
+        }
+    const float down = F16 ? 1.0f / (1 << SHIFT16) : 1.0f;
+    const long row = ((b * a.Nk + key) * a.Hkv + kvh) * 2 * D;
+    if (n < 2 * NQ) store_rows<F16>(a.dk + row + n * 32, x, a.scale * down, h);
+    else store_rows<F16>(a.dv + row + n * 32 - 2 * D, x, down, h);
 }
 
 // dlam[h] = - sum over entries and queries of D_2 (all heads for one shared lam): a block each, in a fixed order, summed in 64 bits
@@ -1035,6 +1075,24 @@ size_t split_bytes(const hs_diff_attn_desc* d, const Split& s) {
     const size_t rows = std::min<int64_t>(16, (int64_t)(d->H / d->Hkv) * d->Nq);
     return s.nsplit > 1 ? (size_t)d->B * d->Hkv * s.tiles * s.nsplit * 2 * rows * (2 * d->d + 2) * 4 : 0;
 }
+// Parts that the dk, dv sweep's list of tiles is cut into.  A round of blocks (one a CU) takes 1.4 us a tile; cutting costs each block another start (4
+// tiles' time), a second kernel, and 0.1 us for a part's sums of a block written and read: blocks over so few keys or so long lists that a cut pays.
+int parts_of(const hs_diff_attn_desc* d) {
+    const int64_t own = d->d == 128 ? Sweep<128>::OWN : Sweep<64>::OWN, blocks = (int64_t)d->B * d->Hkv * ((d->Nk + own - 1) / own);
+    const double tiles = (double)(d->H / d->Hkv) * ((d->Nq + 31) / 32);
+    int best = 1;
+    double least = 0;
+    for (int p = 1; p <= 16; ++p) {
+        const double time = (double)((blocks * p + 255) / 256) * (tiles / p + 4) + (p > 1 ? 6 + 0.07 * (double)blocks * p : 0);
+        if (p == 1 || time < least) { best = p; least = time; }
+    }
+    return best;
+}
+size_t sums_at(const hs_diff_attn_desc* d) { return ((size_t)d->B * d->H * (d->Nq * 12 + (size_t)((d->Nq + 31) / 32) * 512) + 255) / 256 * 256; }
+size_t backward_bytes(const hs_diff_attn_desc* d) {
+    const size_t own = d->d == 128 ? Sweep<128>::OWN : Sweep<64>::OWN, p = parts_of(d);
+    return sums_at(d) + (p > 1 ? p * d->B * d->Hkv * ((d->Nk + own - 1) / own) * own * d->d * 16 : 0);
+}
 Args args_of(const hs_diff_attn_desc* d) {
     Args a = {};
     a.q_b = d->q_b; a.q_n = d->q_n; a.q_h = d->q_h; a.k_b = d->k_b; a.k_n = d->k_n; a.k_h = d->k_h;
@@ -1064,8 +1122,11 @@ template <int D, bool F16> void backward(const Args& a, hipStream_t s) {
     constexpr int LANES = D / 4;
     launch(diff_rows_kernel<D, F16>, ((int64_t)a.B * ((a.Nq + 31) / 32 * 32) * a.H * LANES + 255) / 256, 256, 0, s, a);
     launch(diff_dq_kernel<D, F16>, (int64_t)a.B * a.H * ((a.Nq + S::OWN - 1) / S::OWN), S::NW * 64, (size_t)S::BUFS * S::TILE, s, a);
-    launch(diff_dkv_kernel<D, F16>, (int64_t)a.B * a.Hkv * ((a.Nk + S::OWN - 1) / S::OWN), S::NW * 64,
-           (size_t)S::BUFS * (S::TILE + 512) + (D == 64 ? S::OWN * D * 4 : 0), s, a);
+    const int64_t blocks = (int64_t)a.B * a.Hkv * ((a.Nk + S::OWN - 1) / S::OWN);
+    const size_t lds = (size_t)S::BUFS * (S::TILE + 512) + (D == 64 ? S::OWN * D * 4 : 0);
+    if (a.parts == 1) return launch(diff_dkv_kernel<D, F16, false>, blocks, S::NW * 64, lds, s, a);
+    launch(diff_dkv_kernel<D, F16, true>, blocks * a.parts, S::NW * 64, lds, s, a);
+    launch(diff_dkv_join_kernel<D, F16>, blocks * S::NW * (D / 32), 256, 0, s, a);
 }
 #define HS_BY_TYPE(call)                                                               \
     do {                                                                               \
@@ -1078,7 +1139,7 @@ template <int D, bool F16> void backward(const Args& a, hipStream_t s) {
 }  // namespace
 
 extern "C" size_t hs_diff_attn_fwd_ws_bytes(const hs_diff_attn_desc* d) { return check(d, false) == HS_OK ? split_bytes(d, split_of(d)) : 0; }
-extern "C" size_t hs_diff_attn_bwd_ws_bytes(const hs_diff_attn_desc* d) { return check(d, false) == HS_OK ? (size_t)d->B * d->H * (d->Nq * 12 + (size_t)((d->Nq + 31) / 32) * 512) : 0; }
+extern "C" size_t hs_diff_attn_bwd_ws_bytes(const hs_diff_attn_desc* d) { return check(d, false) == HS_OK ? backward_bytes(d) : 0; }
 
 extern "C" int hs_diff_attn_fwd(const hs_diff_attn_desc* d, const void* q, const void* k, const void* v, const float* lam, const int32_t* q_start,
                                 const int32_t* kv_len, void* o, void* maps, float* lse, void* ws, size_t ws_bytes, void* stream) {
@@ -1109,12 +1170,13 @@ extern "C" int hs_diff_attn_bwd(const hs_diff_attn_desc* d, const void* q, const
     if (!q || !k || !v || !lam || !d_o || !maps || !lse || !dq || !dk || !dv || !dlam || !ws) return HS_ERR_ARG;
     for (const void* p : {q, k, v, d_o, maps, (const void*)dq, (const void*)dk, (const void*)dv, (const void*)ws})
         if (misaligned(p)) return HS_ERR_SHAPE;
-    if (ws_bytes < hs_diff_attn_bwd_ws_bytes(d)) return HS_ERR_SHAPE;
+    if (ws_bytes < backward_bytes(d)) return HS_ERR_SHAPE;
     Args a = args_of(d);
     a.q = (const bf16_t*)q; a.k = (const bf16_t*)k; a.v = (const bf16_t*)v; a.go = (const bf16_t*)d_o; a.lam = lam;
     a.q_start = q_start; a.kv_len = kv_len; a.maps = (bf16_t*)maps; a.lse = (float*)lse;
     a.D = (float*)ws; a.x2 = a.D + (size_t)d->B * d->H * 2 * d->Nq;
     a.rc = a.x2 + (size_t)d->B * d->H * d->Nq;
+    a.parts = parts_of(d); a.sums = (f32x4*)((char*)ws + sums_at(d));
     a.dq = (bf16_t*)dq; a.dk = (bf16_t*)dk; a.dv = (bf16_t*)dv;
     hipStream_t s = (hipStream_t)stream;
 #define CALL(D, F) backward<D, F>(a, s)

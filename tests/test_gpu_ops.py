@@ -231,6 +231,15 @@ def test_diff_attention_of_many_rows(dev, case):
     test_diff_attention_values_and_gradients(dev, case)
 
 
+@pytest.mark.parametrize("case", [                             # many queries for each key: the gradients of keys and values come in parts
+    dict(B=1, Nq=300, Nk=260, Hq=8, Hkv=1, d=64, dtype=BF, causal=True), dict(B=2, Nq=290, Nk=140, Hq=6, Hkv=1, d=128, dtype=F16, lens=[0, 139]),
+    dict(B=2, Nq=200, Nk=300, Hq=6, Hkv=2, d=64, dtype=F16, causal=True, start=[-150, 90]), dict(B=1, Nq=900, Nk=1, Hq=2, Hkv=1, d=32, dtype=BF, lam="one"),
+    dict(B=3, Nq=500, Nk=33, Hq=4, Hkv=2, d=128, dtype=BF, causal=True, lens=[1, 33, 20], start=[-499, -300, 0])],
+    ids=lambda c: f"{c['B']}x{c['Nq']}x{c['Nk']}-{c['Hq']}/{c['Hkv']}x{c['d']}")
+def test_diff_attention_of_few_keys(dev, case):
+    test_diff_attention_values_and_gradients(dev, case)
+
+
 @pytest.mark.parametrize("d", [32, 64, 128])
 @pytest.mark.parametrize("Nq", [1, 200])
 @pytest.mark.parametrize("B", [2, 64])
