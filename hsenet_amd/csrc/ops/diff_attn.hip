@@ -1088,10 +1088,11 @@ int parts_of(const hs_diff_attn_desc* d) {
     }
     return best;
 }
-size_t sums_at(const hs_diff_attn_desc* d) { return ((size_t)d->B * d->H * (d->Nq * 12 + (size_t)((d->Nq + 31) / 32) * 512) + 255) / 256 * 256; }
+size_t rows_bytes(const hs_diff_attn_desc* d) { return (size_t)d->B * d->H * (d->Nq * 12 + (size_t)((d->Nq + 31) / 32) * 512); }
+size_t sums_at(const hs_diff_attn_desc* d) { return (rows_bytes(d) + 255) / 256 * 256; }
 size_t backward_bytes(const hs_diff_attn_desc* d) {
     const size_t own = d->d == 128 ? Sweep<128>::OWN : Sweep<64>::OWN, p = parts_of(d);
-    return sums_at(d) + (p > 1 ? p * d->B * d->Hkv * ((d->Nk + own - 1) / own) * own * d->d * 16 : 0);
+    return p == 1 ? rows_bytes(d) : sums_at(d) + p * d->B * d->Hkv * ((d->Nk + own - 1) / own) * own * d->d * 16;
 }
 Args args_of(const hs_diff_attn_desc* d) {
     Args a = {};

@@ -28,7 +28,8 @@ def _dense(t: torch.Tensor) -> bool:
 class AdamW(torch.optim.Optimizer):
     """p *= 1 - lr * weight_decay; m, v the moments of the gradient; p -= lr m^ / (sqrt(v^) + eps), with all tensors of a group in a launch per 56.
 
-    Parameters: bf16, fp16 or fp32 (arithmetic in fp32, one rounding at the end), dense in any order of their axes, gradients of the same type.
+    Parameters: bf16, fp16 or fp32 (arithmetic in fp32, one rounding at the end), dense in any order of their axes, no two in the same memory (they are
+    updated side by side), gradients of the same type.
     state_bits 32: moments in fp32.  state_bits 8: int8 and uint8 codes with an fp32 scale per 256 elements of a tensor, in its order in memory
     (include/hsenet_ops.h has the formula): 2.03 bytes an element instead of 8.  The step is taken with the new moments before they are rounded.
     A gradient that is not finite makes its element, and with 8 bits its block's moments, NaN: skip such a step, as torch.amp.GradScaler does.
@@ -53,6 +54,8 @@ class AdamW(torch.optim.Optimizer):
             for p in g["params"]:
                 if p.dtype not in O.DTYPE:
                     raise ValueError(f"parameters must be bf16, fp16 or fp32, got {p.dtype}")
+            if len(set(g["params"])) != len(g["params"]):
+                raise ValueError("a parameter stands twice in a group")
         except ValueError:
             self.param_groups.pop()
             raise
@@ -131,25 +134,28 @@ class AdamW(torch.optim.Optimizer):
                 if g.dtype is not dtype or g.get_device() != dev or g.is_sparse:
                     raise L.HsError("a gradient must be dense, of its parameter's type and on its device")
                 st = state.get(p) or self._init_state(p, bits)
-                stride = p.stride()
-                if not (p.is_contiguous() or _dense(p)):
-                    raise L.HsError("a parameter's elements must fill one stretch of memory")
-                if g.stride() != stride:
-                    g = torch.empty_like(p).copy_(g)
-                m, v = st["exp_avg"], st["exp_avg_sq"]
-                if m.stride() != stride or v.stride() != stride:
+                m, v, n = st["exp_avg"], st["exp_avg_sq"], p.numel()
+                if not (p.is_contiguous() and g.is_contiguous() and m.is_contiguous() and v.is_contiguous()):
+                    if not _dense(p):
+                        raise L.HsError("a parameter's elements must fill one stretch of memory")
+                    if g.stride() != p.stride():
+                        g = torch.empty_like(p).copy_(g)
+                    self._check_state(p, st, bits)
+                elif m.numel() != n or m.get_device() != dev:  # (the parameter has been moved or given other data)
                     self._check_state(p, st, bits)
                 if key != (dev, dtype):
                     key = (dev, dtype)
                     if key not in tables:
+                        if dtype not in O.DTYPE:
+                            raise L.HsError(f"parameters must be bf16, fp16 or fp32, got {dtype}")
                         tables[key] = (array("q"), [])
                     words, held = tables[key]
                 held.append(g)                                 # (a gradient that was copied lives until the launch)
                 if bits == 8:
                     words.extend((p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), st["exp_avg_scale"].data_ptr(),
-                                  st["exp_avg_sq_scale"].data_ptr(), st["step"].data_ptr(), p.numel()))
+                                  st["exp_avg_sq_scale"].data_ptr(), st["step"].data_ptr(), n))
                 else:
-                    words.extend((p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), 0, 0, st["step"].data_ptr(), p.numel()))
+                    words.extend((p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), 0, 0, st["step"].data_ptr(), n))
                 changed.append(p)
             for (dev, dtype), (words, _) in tables.items():
                 O.call(dev, "hs_adamw_multi", words.buffer_info()[0], len(words) // 8, O.DTYPE[dtype], bits, *numbers)

@@ -564,6 +564,19 @@ def test_adamw_refusals(dev):
                dict(exp_avg=c, exp_avg_sq=c.byte(), exp_avg_scale=s.double()), dict(exp_avg=c.cpu(), exp_avg_sq=c.byte())):
         with pytest.raises(L.HsError):
             opt.set_state(p, step=0, **{"exp_avg_scale": s, "exp_avg_sq_scale": s, **kw})
+    q = torch.zeros(6, 4, device="cuda", requires_grad=True)
+    other = H.AdamW([q], state_bits=8)
+    q.grad = torch.ones_like(q)
+    other.step()
+    held = other.state[q]["exp_avg"]
+    other.state[q]["exp_avg"] = held.cpu()                    # a state that was moved, a parameter that was given other data
+    with pytest.raises(L.HsError, match="device"):
+        other.step()
+    other.state[q]["exp_avg"], q.grad = held, None
+    q.data = torch.zeros(60, 40, device="cuda")
+    q.grad = torch.ones_like(q)
+    with pytest.raises(L.HsError, match="shape"):
+        other.step()
     m = torch.zeros(8, 8, device="cuda")
     for bad in (([m], []), ([m.half()], [m.half()]), ([m[:4]], [m[:4]]), ([m.t()[:, :4]], [m]), ([m], [m.bfloat16()])):
         with pytest.raises(L.HsError):

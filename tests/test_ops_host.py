@@ -95,6 +95,13 @@ def test_diff_attention_pointers_and_workspace():
     assert lib.hs_diff_attn_fwd(C.byref(long), P, P, P, P, None, None, P, None, None, None, 0, None) == L.HS_ERR_SHAPE
 
 
+@pytest.mark.filterwarnings("ignore:optimizer contains a parameter group with duplicate")
+def test_adamw_takes_a_parameter_once():
+    p = torch.zeros(3, requires_grad=True)
+    with pytest.raises(ValueError, match="twice"):
+        H.AdamW([p, p])
+
+
 @no_gpu_only
 def test_adamw_refusals():
     lib = O.load()
