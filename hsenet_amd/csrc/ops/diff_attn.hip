@@ -445,7 +445,7 @@ __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void d
 // half a tile a wave is always on its way.  Bandwidth leaves the matrix pipe room enough to take P in two numbers of 16 bits, value and what its rounding
 // left, so that o is rounded once, at its end.  The waves' numerators are joined in LDS, and the chunks' by diff_join_kernel; with one chunk the result is
 // written at once.
-template <int D> struct SplitOf { static constexpr int NW = D == 128 ? 2 : 4, TILE = 32 * 4 * D * 2; };
+template <int D> struct SplitOf { static constexpr int NW = 4, TILE = 32 * 4 * D * 2; };
 
 template <int D, bool F16, bool KEEP>
 __global__ __launch_bounds__(SplitOf<D>::NW * 64, D == 128 ? 1 : 2) void diff_split_kernel(Args a) {
@@ -1057,7 +1057,7 @@ int check(const hs_diff_attn_desc* d, bool backward) {
 bool misaligned(const void* p, unsigned n = 16) { return !p || (uintptr_t)p % n; }
 
 struct Split { int tiles, nsplit, chunk; };
-constexpr int WANT = 1024;
+constexpr int WANT = 1024, LEAST = 512;       // blocks (two rounds even out ragged entries: 70 us against 78 with one); keys of a chunk (4 tiles a wave)
 // Whether the split forward runs, and how it cuts the keys.  The whole forward needs the time of one block over all keys for each round of its blocks on
 // the 256 CUs, full or not; the split forward's time goes with its tiles, wherever they come from.  Measured with 16 query heads on 4 key heads of 64, 8192
 // keys, whole / split in us: 1 entry, 16 queries 277 / 20, 256 queries 282 / 72; 16 entries, 16 queries 327 / 108, 32 (512 tiles) 311 / 197, 64 (1024 tiles)
@@ -1068,7 +1068,7 @@ Split split_of(const hs_diff_attn_desc* d) {
     const int64_t rounds = ((int64_t)d->B * d->H * ((d->Nq + own - 1) / own) * halves + 255) / 256;
     if (blocks > rounds * (d->d == 128 ? 256 : 512)) return {0, 0, 0};
     const int64_t want = std::min<int64_t>((WANT + blocks - 1) / blocks, MOST_CHUNKS);
-    const int64_t chunk = std::max<int64_t>(((d->Nk + want - 1) / want + 127) / 128 * 128, d->d == 128 ? 256 : 512);
+    const int64_t chunk = std::max<int64_t>(((d->Nk + want - 1) / want + 127) / 128 * 128, LEAST);
     return {(int)tiles, (int)((d->Nk + chunk - 1) / chunk), (int)chunk};
 }
 size_t split_bytes(const hs_diff_attn_desc* d, const Split& s) {
