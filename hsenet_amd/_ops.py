@@ -21,6 +21,14 @@ ROTARY_MAX_PAIRS = 512
 _vp, _i, _i64, _sz, _d, _i64x2 = C.c_void_p, C.c_int, C.c_int64, C.c_size_t, C.c_double, C.c_int64 * 2
 
 
+class _Packed(struct.Struct):
+    def pack(self, *numbers) -> bytes:
+        try:
+            return super().pack(*numbers)
+        except struct.error as e:
+            raise L.HsError(f"a size does not fit 32 bits: {e}") from e
+
+
 class RotaryDesc(L._Desc):
     _fields_ = [("struct_size", C.c_uint32), ("B", _i), ("N", _i), ("dh", _i), ("pairs", _i), ("axes", _i), ("heads", _i * 2), ("interleaved", _i),
                 ("inverse", _i), ("dtype", _i), ("pos_dtype", _i), ("x_b", _i64x2), ("x_n", _i64x2), ("x_h", _i64x2), ("y_b", _i64x2),
@@ -33,7 +41,7 @@ class DiffAttnDesc(L._Desc):
 
 
 # descriptors are packed in one go where a call builds them (setting a structure's fields one by one costs more than the launch)
-ROTARY_PACK, DIFF_PACK = struct.Struct("@I11i15q"), struct.Struct("@I10if12q")
+ROTARY_PACK, DIFF_PACK = _Packed("@I11i15q"), _Packed("@I10if12q")
 assert ROTARY_PACK.size == C.sizeof(RotaryDesc) and DIFF_PACK.size == C.sizeof(DiffAttnDesc)
 
 SIGNATURES = {

@@ -250,7 +250,7 @@ template <class F> int over_tables(const hs_adamw_tensor* t, int count, Table a,
         for (; at < count && a.count < TENSORS; ++at) {
             if (t[at].n == 0) continue;
             const uint64_t more = ((uint64_t)t[at].n + CHUNK - 1) / CHUNK;
-            if (a.count && blocks + more > 0x7fffffffu) break;
+            if (a.count && blocks + more >= 1u << 24) break;          // (256 threads each: below 2^32)
             const int k = a.count++;
             a.p[k] = t[at].p; a.g[k] = t[at].g; a.m[k] = t[at].m; a.v[k] = t[at].v;
             a.ms[k] = t[at].m_scale; a.vs[k] = t[at].v_scale; a.step[k] = t[at].step; a.n[k] = (long)t[at].n;
@@ -273,7 +273,7 @@ extern "C" int hs_adamw_multi(const hs_adamw_tensor* t, int count, int dtype, in
     if (!(beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1 && eps >= 0)) return HS_ERR_ARG;
     const unsigned size = dtype == HS_PREC_F32 ? 4 : 2;
     for (int i = 0; i < count; ++i) {
-        if (t[i].n < 0 || t[i].n > ((int64_t)1 << 42)) return HS_ERR_SHAPE;
+        if (t[i].n < 0 || t[i].n >= ((int64_t)CHUNK << 24) - CHUNK) return HS_ERR_SHAPE;
         if (bad(t[i].step, 16)) return HS_ERR_ARG;
         if (!t[i].n) continue;
         if (bad(t[i].p, size) || bad(t[i].g, size) || bad(t[i].m, state_bits / 8) || bad(t[i].v, state_bits / 8)) return HS_ERR_ARG;
@@ -307,7 +307,7 @@ extern "C" int hs_adamw_moments(const hs_adamw_tensor* t, int count, int out_dty
     if (!t || count < 1 || (out_dtype != HS_PREC_BF16 && out_dtype != HS_PREC_F32)) return HS_ERR_ARG;
     const unsigned size = out_dtype == HS_PREC_F32 ? 4 : 2;
     for (int i = 0; i < count; ++i) {
-        if (t[i].n < 0 || t[i].n > ((int64_t)1 << 42)) return HS_ERR_SHAPE;
+        if (t[i].n < 0 || t[i].n >= ((int64_t)CHUNK << 24) - CHUNK) return HS_ERR_SHAPE;
         if (!t[i].n) continue;
         if (bad(t[i].p, size) || bad(t[i].g, size) || bad(t[i].m, 1) || bad(t[i].v, 1) || bad(t[i].m_scale, 4) || bad(t[i].v_scale, 4)) return HS_ERR_ARG;
     }

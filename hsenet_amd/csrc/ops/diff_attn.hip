@@ -42,10 +42,14 @@ __device__ __forceinline__ int block_order() {
     const int nb = gridDim.x, id = blockIdx.x, q = nb >> 3, r = nb & 7, x = id & 7;
     return (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (id >> 3);
 }
-__device__ __forceinline__ int key_count(const Args& a, int b) { return a.kv_len ? min(max(a.kv_len[b], 0), a.Nk) : a.Nk; }
 __device__ __forceinline__ int first_pos(const Args& a, int b) {
     const int s = a.q_start ? a.q_start[b] : a.q_start0;
     return min(max(s, -(1 << 30)), 1 << 30);
+}
+// number of leading keys that some query sees: the others are not touched (a cache may hold anything there)
+__device__ __forceinline__ int key_count(const Args& a, int b) {
+    const int len = a.kv_len ? min(max(a.kv_len[b], 0), a.Nk) : a.Nk;
+    return a.causal ? max(0, min(len, first_pos(a, b) + a.Nq)) : len;
 }
 // number of leading keys that query i sees
 __device__ __forceinline__ int visible(const Args& a, int len, int start, int i) { return a.causal ? max(0, min(len, start + i + 1)) : len; }
@@ -1044,7 +1048,10 @@ int check(const hs_diff_attn_desc* d, bool backward) {
     if (d->B < 1 || d->Nq < 1 || d->Nk < 1 || d->H < 1 || d->Hkv < 1 || d->H % d->Hkv) return HS_ERR_SHAPE;
     if (d->d != 32 && d->d != 64 && d->d != 128) return HS_ERR_SHAPE;
     if (d->Nq > (1 << 28) || d->Nk > (1 << 28) || d->H > (1 << 16) || (int64_t)d->B * d->H * ((int64_t)d->Nq + d->Nk) > ((int64_t)1 << 36)) return HS_ERR_SHAPE;
-    if ((int64_t)d->B * d->H * (((int64_t)(d->Nq > d->Nk ? d->Nq : d->Nk) + 127) / 128) > (1 << 30)) return HS_ERR_SHAPE;
+    // every launch stays under 2^32 threads: the sweeps have 512 for 256 rows or 256 for 64 or 128, the split forward 256 for 16, twice as many at most as
+    // the whole forward, and the rows' constants d / 4 for one
+    if ((int64_t)d->B * d->H * (((int64_t)(d->Nq > d->Nk ? d->Nq : d->Nk) + 127) / 128) >= (1 << 22)) return HS_ERR_SHAPE;
+    if (backward && (int64_t)d->B * d->H * (((int64_t)d->Nq + 31) / 32) * 8 * d->d >= (int64_t)1 << 32) return HS_ERR_SHAPE;
     for (int64_t s : {d->q_b, d->q_n, d->q_h, d->k_b, d->k_n, d->k_h, d->v_b, d->v_n, d->v_h})
         if (s < 0 || (s & 7)) return HS_ERR_SHAPE;
     for (int64_t s : {d->q_n, d->q_h, d->k_n, d->k_h, d->v_n, d->v_h, backward ? d->go_n : 0, backward ? d->go_h : 0})

@@ -202,6 +202,7 @@ extern "C" int hs_rotary_axes(const hs_rotary_desc* d, const void* x0, void* y0,
     // tokens of a block: about TARGET vectors, while the grid still gives every CU several blocks
     const int tail = (d->dh - 2 * d->pairs) / vec, turned = line || pairs ? std::max(2 * d->pairs / vec, 1) : 2 * (d->pairs / vec);
     a.tpb = std::max(1, std::min({TARGET / (heads * (turned + tail)), a.tokens / 2048, MOST_TOKENS}));
+    if (a.tokens / a.tpb >= (1 << 24) - 1) return HS_ERR_SHAPE;                          // 2^32 threads
     hipStream_t s = (hipStream_t)stream;
     if (d->dtype == HS_PREC_BF16) launch<HS_PREC_BF16>(a, vec, pairs, line, s);
     else if (d->dtype == HS_PREC_F16) launch<HS_PREC_F16>(a, vec, pairs, line, s);

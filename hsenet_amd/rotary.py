@@ -129,6 +129,8 @@ def rotary_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Ten
     ``inplace``: the tensors themselves are turned and returned, without a graph (a new token's q and k)."""
     xs = (q,) if k is None else (q, k)
     if inplace:
+        if k is not None and k.numel() and k.data_ptr() == q.data_ptr():
+            raise L.HsError("one tensor cannot be turned in place twice in a call")
         if torch.is_grad_enabled() and any(x.requires_grad for x in xs):
             raise L.HsError("turning in place is not differentiable: call it under no_grad, or without inplace")
         out = _turn(xs, positions, plan, False, True)

@@ -106,6 +106,8 @@ def test_rotary_refusals(dev):
             H.rotary_axes(*args)
     with pytest.raises(L.HsError, match="not differentiable"):
         H.rotary_axes(q.requires_grad_(), None, pos, plan, inplace=True)
+    with pytest.raises(L.HsError, match="twice"), torch.no_grad():
+        H.rotary_axes(q, q, pos, plan, inplace=True)
     with pytest.raises(L.HsError, match="broadcast"):
         H.rotary_axes(q.detach()[:, :, :1].expand(2, 6, 3, 32), None, pos, plan, inplace=True)
 
@@ -299,6 +301,23 @@ def test_diff_caches_views_and_what_lies_behind(dev):
         over = H.diff_attention(q, k, v, lam, kv_len=torch.tensor([-5, 1000], dtype=torch.int32, device="cuda"))
         assert not over[0].any() and torch.equal(over[1], H.diff_attention(q, k, v, lam)[1])
         assert H.diff_attention(q[:, :0], k, v, lam).shape == (B, 0, Hq, 2 * d) and not H.diff_attention(q, k[:, :0], v[:, :0], lam).any()
+
+
+@pytest.mark.parametrize("B,Nq,Hq,Hkv,d", [(2, 1, 4, 2, 64), (2, 5, 8, 2, 128), (3, 40, 2, 2, 32), (8, 70, 16, 16, 64), (4, 100, 16, 16, 128)])
+def test_diff_causal_cache_filled_to_its_queries(dev, B, Nq, Hq, Hkv, d):
+    """a cache that holds NaN behind the last query's own position: the causal mask alone says that nothing there counts"""
+    g = torch.Generator("cuda").manual_seed(Nq)
+    S = Nq + 90
+    q, k, v = rnd(g, B, Nq, 2 * Hq, d, dtype=BF), rnd(g, B, S, 2 * Hkv, d, dtype=BF), rnd(g, B, S, Hkv, 2 * d, dtype=BF)
+    lam, go = torch.full((Hq,), 0.3, device="cuda"), rnd(g, B, Nq, Hq, 2 * d, dtype=BF)
+    start = torch.tensor([0, 61, -3, 40][:B] * 2, dtype=torch.int32, device="cuda")[:B].contiguous()
+    kw = dict(causal=True, q_start=start)
+    want = run_diff(q, k, v, lam, go, dict(kw, kv_len=(start + Nq).clamp_(0, S).to(torch.int32)))
+    gap = torch.arange(S, device="cuda")[None, :] >= (start + Nq)[:, None]
+    got = run_diff(q, k.masked_fill(gap[..., None, None], math.nan), v.masked_fill(gap[..., None, None], math.nan), lam, go, kw)
+    for n in want:
+        assert torch.equal(got[n], want[n]), n
+    assert not got["k"][gap].any() and not got["v"][gap].any()
 
 
 def test_diff_shared_and_broadcast_weight(dev):

@@ -102,6 +102,11 @@ def test_adamw_takes_a_parameter_once():
         H.AdamW([p, p])
 
 
+def test_sizes_that_do_not_fit_are_errors():
+    with pytest.raises(L.HsError, match="32 bits"):
+        O.DIFF_PACK.pack(O.DIFF_PACK.size, 1, 1 << 31, *[1] * 8, 1.0, *[0] * 12)
+
+
 @no_gpu_only
 def test_adamw_refusals():
     lib = O.load()
