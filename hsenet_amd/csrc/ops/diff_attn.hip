@@ -1024,16 +1024,26 @@ __global__ __launch_bounds__(256) void diff_dkv_join_kernel(Args a) {
     else store_rows<F16>(a.dv + row + n * 32 - 2 * D, x, down, h);
 }
 
-// dlam[h] = - sum over entries and queries of D_2 (all heads for one shared lam): a block each, in a fixed order, summed in 64 bits
-__global__ __launch_bounds__(256) void diff_dlam_kernel(Args a, float* dlam) {
-    __shared__ double red[256];
-    const int h0 = a.lam_stride ? blockIdx.x : 0, nh = a.lam_stride ? 1 : a.H;
+// dlam[h] = - sum over entries and queries of D_2 (all heads for one shared lam): a block each, in a fixed order, summed in 64 bits; a thread has
+// eight loads on their way at a time
+__global__ __launch_bounds__(1024) void diff_dlam_kernel(Args a, float* dlam) {
+    __shared__ double red[1024];
+    const int h0 = a.lam_stride ? blockIdx.x : 0;
+    const long run = (long)(a.lam_stride ? 1 : a.H) * a.Nq, n = run * a.B;                   // an entry's stretch of D_2; all of them
     double s = 0;
-    for (int b = 0; b < a.B; ++b)
-        for (long i = threadIdx.x; i < (long)nh * a.Nq; i += 256) s += a.x2[((long)b * a.H + h0) * a.Nq + i];
+    for (long i0 = threadIdx.x; i0 < n; i0 += 8 * 1024) {
+        float x[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const long i = i0 + k * 1024, b = i / run;
+            x[k] = i < n ? a.x2[(b * a.H + h0) * a.Nq + (i - b * run)] : 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) s += x[k];
+    }
     red[threadIdx.x] = s;
     __syncthreads();
-    for (int w = 128; w > 0; w >>= 1) {
+    for (int w = 512; w > 0; w >>= 1) {
         if ((int)threadIdx.x < w) red[threadIdx.x] += red[threadIdx.x + w];
         __syncthreads();
     }
@@ -1191,7 +1201,7 @@ extern "C" int hs_diff_attn_bwd(const hs_diff_attn_desc* d, const void* q, const
     HS_BY_TYPE(CALL);
 #undef CALL
     HS_CHECK_LAUNCH();
-    hipLaunchKernelGGL(diff_dlam_kernel, dim3(a.lam_stride ? a.H : 1), dim3(256), 0, s, a, dlam);
+    hipLaunchKernelGGL(diff_dlam_kernel, dim3(a.lam_stride ? a.H : 1), dim3(1024), 0, s, a, dlam);
     HS_CHECK_LAUNCH();
     return HS_OK;
 }
