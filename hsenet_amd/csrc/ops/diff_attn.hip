@@ -195,26 +195,12 @@ template <bool F16> __device__ __forceinline__ float add2(unsigned pair, float s
     if constexpr (F16) return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, pair), h2{(_Float16)1.f, (_Float16)1.f}, sum, false);
     else return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, pair), b2{(__bf16)1.f, (__bf16)1.f}, sum, false);
 }
-// p = 2^(c2 s - m) rounded for the product; l += their sums (short ones first: they run over thousands of keys)
-template <bool F16, int SUMS>
-__device__ __forceinline__ void softmax_weights(f32x16& s, float c2, float m, float (&l)[SUMS], bf16x8 (&p)[2]) {
-    float part[4] = {0.f, 0.f, 0.f, 0.f};
+// numerators, in s as they are and in p rounded for the product
+template <bool F16>
+__device__ __forceinline__ void softmax_weights(f32x16& s, float c2, float m, bf16x8 (&p)[2]) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c2, -m));
-    if (SUMS == 2) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) part[r & 3] += s[r];
-        l[SUMS - 1] += (part[0] + part[1]) + (part[2] + part[3]);
-        part[0] = part[1] = 0.f;
-    }
-#pragma unroll
-    for (int sp = 0; sp < 2; ++sp) {
-        p[sp] = pack8<F16>(s, sp);
-        const u32x4 w = __builtin_bit_cast(u32x4, p[sp]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) part[e & 1] = add2<F16>(w[e], part[e & 1]);
-    }
-    l[0] += part[0] + part[1];
+    p[0] = pack8<F16>(s, 0); p[1] = pack8<F16>(s, 1);
 }
 // numerators in two numbers of 16 bits, value and what its rounding left, and their sum
 template <bool F16>
@@ -289,13 +275,40 @@ template <bool F16> __device__ __forceinline__ void pack2maps(const f32x16 (&s)[
 #pragma unroll
         for (int sp = 0; sp < 2; ++sp) p[i][sp] = pack8<F16>(s[i], sp);
 }
-template <int D, bool F16, int ROWS, int NB>
-__device__ __forceinline__ void values(const Lane& f, const bf16x8 (&p)[2][2], f32x16 (&o1)[NB], f32x16 (&o2)[NB]) {
+// The sums of a step's numerators (short ones, which l takes up: it runs over thousands of keys): of the rounded ones, that o is divided by, and with
+// SUMS = 2 of those in s.
+template <bool F16, int SUMS> __device__ __forceinline__ void add_weights(const bf16x8 (&p)[2][2], const f32x16 (&s)[2], float (&part)[2], float (&whole)[2]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) part[i] = add2<F16>(__builtin_bit_cast(u32x4, p[i][e >> 2])[e & 3], part[i]);
+    if (SUMS == 2)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) whole[i] += s[i][r];
+}
+template <int SUMS> __device__ __forceinline__ void take_up(float (&l)[2][SUMS], const float (&part)[2], const float (&whole)[2]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        l[i][0] += part[i];
+        if (SUMS == 2) l[i][SUMS - 1] += whole[i];
+    }
+}
+// the products with V, and with PAIRED the sums, while the first fragments are on their way
+template <int D, bool F16, int ROWS, bool PAIRED, int NB, int SUMS>
+__device__ __forceinline__ void values(const Lane& f, const bf16x8 (&p)[2][2], const f32x16 (&s)[2], f32x16 (&o1)[NB], f32x16 (&o2)[NB], float (&l)[2][SUMS]) {
     constexpr int N = 2 * NB, AHEAD = 4;
     bf16x8 x[AHEAD];
+    float part[2] = {0.f, 0.f}, whole[2] = {0.f, 0.f};
 #pragma unroll
     for (int n = 0; n < AHEAD; ++n) x[n] = f.template cols32<ROWS>(16 * (n / NB), 2 * D + n % NB * 32);
     __builtin_amdgcn_sched_barrier(0);
+    if (PAIRED) {
+        add_weights<F16, SUMS>(p, s, part, whole);
+        if (SUMS == 1) take_up(l, part, whole);
+        __builtin_amdgcn_sched_barrier(0);
+    }
 #pragma unroll
     for (int n = 0; n < N; ++n) {
         const int sp = n / NB, db = n % NB, q = n + AHEAD;
@@ -304,14 +317,16 @@ __device__ __forceinline__ void values(const Lane& f, const bf16x8 (&p)[2][2], f
         if (q < N) x[n % AHEAD] = f.template cols32<ROWS>(16 * (q / NB), 2 * D + q % NB * 32);
         __builtin_amdgcn_sched_barrier(0);
     }
+    if (PAIRED && SUMS == 2) take_up(l, part, whole);                     // (here it costs fewer registers)
 }
 
 // ---- the phases of a sweep -----------------------------------------------------------------------------------------------------------------------
 // The forward, dq and dk,dv sweeps share one scheme: a wave keeps 32 rows of its own and a tile of 32 rows streams past a step.  A step is a vector phase (the
 // softmax weights of the step) and a matrix phase (the products that the weights go into, then the next step's scores), a barrier behind each.
 // At d = 32 and 64 a block has 8 waves; w and w + 4 share a SIMD, and the later four run half a step behind: while one works on the vector units, the
-// other has the matrix pipe (left to themselves both do the same thing at the same time).  At d = 128 a SIMD's registers hold one wave only, and the
-// forward pass' numerators of half of the values: two blocks then, each with the scores of all.
+// other has the matrix pipe (left to themselves both do the same thing at the same time).  The vector phase is the longer one: sums of what it made, that
+// nobody waits for, are taken in the matrix phase (forward at d = 64: 4 % faster with one sum a map, 12 % with two; at d = 128 3 % slower).  At d = 128 a
+// SIMD's registers hold one wave only, and the forward pass' numerators of half of the values: two blocks then, each with the scores of all.
 // Tile t is first read in the matrix phase of step t - 1 and left in step t's, half a step later by the later waves: it is sent for in step t - LEAD
 // into the buffer of tile t - BUFS.
 template <int D> struct Sweep {
@@ -399,12 +414,17 @@ __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void d
                 follow_max(s[1], a.c2, m[1], l[1], o2);
             }
             bf16x8 p[2][2];
-            softmax_weights<F16>(s[0], a.c2, m[0], l[0], p[0]);
-            softmax_weights<F16>(s[1], a.c2, m[1], l[1], p[1]);
+            softmax_weights<F16>(s[0], a.c2, m[0], p[0]);
+            softmax_weights<F16>(s[1], a.c2, m[1], p[1]);
+            if (!S::PAIRED) {
+                float part[2] = {0.f, 0.f}, whole[2] = {0.f, 0.f};
+                add_weights<F16, SUMS>(p, s, part, whole);
+                take_up(l, part, whole);
+            }
             S::template behind_vector<decltype(dma)>(j + S::LEAD < nj);
             __syncthreads();
             __builtin_amdgcn_s_setprio(1);
-            values<D, F16, ROWS>(fl.at(buf * TILE), p, o1, o2);
+            values<D, F16, ROWS, S::PAIRED>(fl.at(buf * TILE), p, s, o1, o2, l);
             buf = S::next(buf);
             scores<D, F16, ROWS>(fl.at(buf * TILE), qf, s);
             __builtin_amdgcn_s_setprio(0);
@@ -747,16 +767,13 @@ __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void d
         dma.skip(ROWS);
         ahead = S::next(ahead);
         if (j * 32 + 32 > lim_lo) mask_keys(s, lim - j * 32, h);
-        float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][r], a.c2, -hi0));
             const float p2 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[1][r], a.c2, -hi1));
-            part[r & 3] = __builtin_fmaf(p2, dp[r], part[r & 3]);
             s[0][r] = p1 * (dp[r] - D0);
             s[1][r] = p2 * (dp[r] - D1);
         }
-        x2 += (part[0] + part[1]) + (part[2] + part[3]);
         bf16x8 ds[2][2];
         pack2maps<F16>(s, ds);
         S::template behind_vector<decltype(dma)>(j + S::LEAD < nj);
@@ -764,6 +781,7 @@ __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void d
         __builtin_amdgcn_s_setprio(1);
         {
             const Lane f = fl.at(buf * TILE);
+            float part[2] = {0.f, 0.f};
             constexpr int N = 4 * NQ, AHEAD = 4;                          // (map, sixteen keys, 32 columns)
             auto frag = [&](int n) { return f.template cols32<ROWS>(16 * (n / NQ % 2), n / (2 * NQ) * D + n % NQ * 32); };
             bf16x8 x[AHEAD];
@@ -774,9 +792,12 @@ __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void d
             for (int n = 0; n < N; ++n) {
                 f32x16& acc = dq[n / (2 * NQ)][n % NQ];
                 acc = mfma32<F16>(x[n % AHEAD], ds[n / (2 * NQ)][n / NQ % 2], acc);
+#pragma unroll
+                for (int e = 16 / N * n; e < 16 / N * (n + 1); ++e) part[e & 1] += s[1][e];        // (beside a matrix instruction: see values())
                 if (n + AHEAD < N) x[n % AHEAD] = frag(n + AHEAD);
                 __builtin_amdgcn_sched_barrier(0);
             }
+            x2 += part[0] + part[1];
         }
         buf = S::next(buf);
         scores_dp<D, F16, ROWS>(fl.at(buf * TILE), qf, gf, s, dp);
@@ -788,7 +809,8 @@ __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void d
     const float down = F16 ? 1.0f / (1 << SHIFT16) : 1.0f, mul = a.scale * down;
     const float un0 = __builtin_amdgcn_exp2f(-ls[2 * a.Nq]), un1 = __builtin_amdgcn_exp2f(-ls[3 * a.Nq]);
     x2 += __shfl_xor(x2, 32, 64);
-    if (h == 0) a.x2[bh * a.Nq + query] = x2 * down * un1;
+    // D_2 = sum P2 dP = D_1' + sum P2 (dP - D_1'), whatever D_1' is that stands for it in the row's dS (sum P2 = 1)
+    if (h == 0) a.x2[bh * a.Nq + query] = x2 * down * un1 + D1;
     bf16_t* p = a.dq + (((long)b * a.Nq + query) * a.H + head) * 2 * D;
     store_rows<F16>(p, dq[0], mul * un0, h);
     store_rows<F16>(p + D, dq[1], -a.lam[head * a.lam_stride] * mul * un1, h);
