@@ -1,7 +1,8 @@
 // Rotary positions with several axes: point j of a head is turned by the angle positions[axis[j]] * freq[j].
 //
 // Bound: HBM.  q and k are read and written once; the angles of a token are shared by all of its heads, so a block makes the cosines and
-// sines of its few tokens once, in LDS, and then streams the heads' rows past them with 16-byte accesses.
+// sines of its few tokens once, in LDS, and then streams the heads' rows past them with 16-byte accesses: 4.4 to 5.3 TB/s over 8 to 16 volumes of 4097
+// tokens, where a plain copy reaches 5.0.
 // The angle is a product in 64 bits, reduced to a fraction of a turn there (a position of 10^6 would leave an fp32 angle 0.06 rad off);
 // the fraction, at most 1/2, is rounded to 32 bits and goes through sincospi.
 #include "../common.h"
@@ -10,7 +11,7 @@
 
 namespace {
 
-constexpr int MOST_TOKENS = 16, TARGET = 1024;     // of a block: tokens, vectors
+constexpr int MOST_TOKENS = 16, TARGET = 1024, MOST_STAGED = 512;     // of a block: tokens, vectors, vectors in LDS
 
 struct RotaryArgs {
     const void* x[2];
@@ -41,12 +42,14 @@ template <> struct Elem<HS_PREC_F32> {
     static __device__ __forceinline__ T put(float f) { return f; }
 };
 
-enum { SPLIT, LINE, PAIRS };
+enum { SPLIT, LINE, PAIRS, STAGED };
 
 // A row (one head of one token) is cut into items of VEC columns that one thread moves.  SPLIT (halves, j and j + P): P / VEC items take VEC columns of
 // the first half and the VEC facing them.  LINE (the same halves, where a row is a power of two of 16-byte vectors and turned whole): an item is one
-// vector, so that a wave reads and writes whole lines, and the facing vector comes from the lane that holds it: 89 us against 95 for 16 x 4097 tokens of 24
-// heads of 64 in bf16, 71 against 78 for 8 x 4097 of 20 heads of 128.  PAIRS (neighbours): an item is VEC / 2 pairs.  Columns behind the pairs follow as plain copies (none where a tensor is turned in place).
+// vector, so that a wave reads and writes whole lines, and the facing vector comes from the lane that holds it: 90 us against 94 for 16 x 4097 tokens of 24
+// heads of 64 in bf16, 73 against 77 for 8 x 4097 of 20 heads of 128.  PAIRS (neighbours): an item is VEC / 2 pairs, the last ones maybe not to be turned.
+// Columns behind the pairs follow as plain copies (none where a tensor is turned in place).  STAGED (halves whose P is no multiple of the vector): rows go
+// through LDS, where a column's partner is read by itself: 8 x 4097 tokens of 24 heads of 64 with P = 29 in bf16 46 us, in single columns 134.
 template <int DT, int VEC, int MODE>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
     typedef typename Elem<DT>::T T;
@@ -77,9 +80,53 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
         }
     }
     __syncthreads();
+    if constexpr (MODE == STAGED) {
+        constexpr int AT = MOST_STAGED / 256;
+        __shared__ V stage[MOST_STAGED];
+        const int items = a.dh / VEC, rows = ntok * a.heads, at_once = MOST_STAGED / items;
+        const float inv_items = 1.0f / items;
+        for (int r0 = 0; r0 < rows; r0 += at_once) {
+            const int count = min(at_once, rows - r0) * items;
+            V u[AT];
+            T* y[AT];
+            int it[AT], t[AT];
+#pragma unroll
+            for (int k = 0; k < AT; ++k) {
+                const int i = threadIdx.x + k * 256;
+                if (i >= count) continue;
+                const int r = (int)((i + 0.5f) * inv_items), row = r0 + r;
+                it[k] = i - r * items;
+                t[k] = (int)((row + 0.5f) * a.inv_heads);
+                int h = row - t[k] * a.heads;
+                const int which = h >= a.heads0;
+                h -= which ? a.heads0 : 0;
+                u[k] = *(const V*)((const T*)(which ? a.x[1] : a.x[0]) + at[t[k]][which] + h * (which ? a.x_h[1] : a.x_h[0]) + it[k] * VEC);
+                y[k] = (T*)(which ? a.y[1] : a.y[0]) + at[t[k]][2 + which] + h * (which ? a.y_h[1] : a.y_h[0]) + it[k] * VEC;
+                stage[i] = u[k];
+            }
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < AT; ++k) {
+                const int i = threadIdx.x + k * 256;
+                if (i >= count) continue;
+                const T* row = (const T*)(stage + (i - it[k]));
+                V o;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    const int c = it[k] * VEC + e, low = c < a.P;
+                    const float2 r = cs[t[k] * a.P + min(low ? c : c - a.P, a.P - 1)];
+                    const float own = Elem<DT>::get(u[k][e]), other = Elem<DT>::get(row[low ? c + a.P : c < 2 * a.P ? c - a.P : c]);
+                    o[e] = c < 2 * a.P ? Elem<DT>::put(own * r.x + other * (low ? -r.y : r.y)) : u[k][e];
+                }
+                *(V*)y[k] = o;
+            }
+            __syncthreads();                                              // (the next rows go where these are)
+        }
+        return;
+    }
     constexpr bool SINGLE = MODE == PAIRS && VEC == 1;           // rows of odd length: a pair is two single accesses
-    const int turned = SINGLE ? a.P : MODE == SPLIT ? a.P / VEC : 2 * a.P / VEC;
-    const int tail = (a.dh - 2 * a.P) / VEC, items = turned + tail;
+    const int turned = SINGLE ? a.P : MODE == SPLIT ? a.P / VEC : (2 * a.P + VEC - 1) / VEC;
+    const int items = turned + (MODE == PAIRS && !SINGLE ? a.dh / VEC - turned : (a.dh - 2 * a.P) / VEC);
     const int total = ntok * a.heads * items;
     const float inv_items = 1.0f / items;
     // AT items of a thread at a time: their loads are all on the way before the first is used
@@ -102,9 +149,9 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
             const T* x = (const T*)(which ? a.x[1] : a.x[0]) + at[t][which] + h * (which ? a.x_h[1] : a.x_h[0]);
             y[k] = (T*)(which ? a.y[1] : a.y[0]) + at[t][2 + which] + h * (which ? a.y_h[1] : a.y_h[0]);
             kind[k] = it < turned ? 1 : x != y[k] ? 2 : 0;
-            first[k] = it < turned ? (SINGLE ? 2 * it : it * VEC) : 2 * a.P + (it - turned) * VEC;
+            first[k] = it < turned || (MODE == PAIRS && !SINGLE) ? (SINGLE ? 2 * it : it * VEC) : 2 * a.P + (it - turned) * VEC;
             second[k] = SINGLE ? first[k] + 1 : a.P + first[k];
-            w[k] = cs + t * a.P + (SINGLE ? it : MODE == PAIRS ? it * VEC / 2 : MODE == LINE ? (it & (turned / 2 - 1)) * VEC : it * VEC);
+            w[k] = cs + t * a.P + (SINGLE ? it : MODE == PAIRS ? 0 : MODE == LINE ? (it & (turned / 2 - 1)) * VEC : it * VEC);
             if (kind[k]) u[k][0] = *(const V*)(x + first[k]);
             if (W == 2 && kind[k] == 1) u[k][W - 1] = *(const V*)(x + second[k]);
         }
@@ -128,12 +175,21 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
                     o[e] = Elem<DT>::put(Elem<DT>::get(u[k][0][e]) * r.x + Elem<DT>::get(z[e]) * (side * r.y));
                 }
             } else if constexpr (W == 1) {
-#pragma unroll
-                for (int e = 0; e < VEC; e += 2) {
-                    const float2 r = w[k][e >> 1];
+                const int left = a.P - (first[k] >> 1);                   // pairs from here on
+                const float2* r = w[k] + (first[k] >> 1);
+                o = u[k][0];
+                auto turn = [&](int e) {
                     const float p = Elem<DT>::get(u[k][0][e]), q = Elem<DT>::get(u[k][0][e + 1]);
-                    o[e] = Elem<DT>::put(p * r.x - q * r.y);
-                    o[e + 1] = Elem<DT>::put(p * r.y + q * r.x);
+                    o[e] = Elem<DT>::put(p * r[e >> 1].x - q * r[e >> 1].y);
+                    o[e + 1] = Elem<DT>::put(p * r[e >> 1].y + q * r[e >> 1].x);
+                };
+                if (left >= VEC / 2) {
+#pragma unroll
+                    for (int e = 0; e < VEC; e += 2) turn(e);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < VEC - 2; e += 2)
+                        if ((e >> 1) < left) turn(e);
                 }
             } else {
 #pragma unroll
@@ -151,15 +207,16 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
 }
 
 template <int DT>
-void launch(const RotaryArgs& a, int vec, bool pairs, bool line, hipStream_t s) {
+void launch(const RotaryArgs& a, int vec, int mode, hipStream_t s) {
     const dim3 grid((a.tokens + a.tpb - 1) / a.tpb), block(256);
     const size_t lds = (size_t)a.tpb * a.P * sizeof(float2);
     constexpr int FULL = DT == HS_PREC_F32 ? 4 : 8;
 #define HS_ROT(VEC, MODE) hipLaunchKernelGGL((rotary_kernel<DT, VEC, MODE>), grid, block, lds, s, a)
-    if (line) HS_ROT(FULL, LINE);
-    else if (vec == FULL) { if (pairs) HS_ROT(FULL, PAIRS); else HS_ROT(FULL, SPLIT); }
-    else if (vec == 2) { if (pairs) HS_ROT(2, PAIRS); else HS_ROT(2, SPLIT); }
-    else { if (pairs) HS_ROT(1, PAIRS); else HS_ROT(1, SPLIT); }
+    if (mode == LINE) HS_ROT(FULL, LINE);
+    else if (mode == STAGED) HS_ROT(FULL, STAGED);
+    else if (vec == FULL) { if (mode == PAIRS) HS_ROT(FULL, PAIRS); else HS_ROT(FULL, SPLIT); }
+    else if (vec == 2) { if (mode == PAIRS) HS_ROT(2, PAIRS); else HS_ROT(2, SPLIT); }
+    else { if (mode == PAIRS) HS_ROT(1, PAIRS); else HS_ROT(1, SPLIT); }
 #undef HS_ROT
 }
 
@@ -176,9 +233,8 @@ extern "C" int hs_rotary_axes(const hs_rotary_desc* d, const void* x0, void* y0,
     if (heads > 4096 || (int64_t)heads * d->dh > (1 << 18)) return HS_ERR_SHAPE;      // a block's item numbers stay far inside fp32's whole numbers
     const int size = d->dtype == HS_PREC_F32 ? 4 : 2, full = 16 / size;
     RotaryArgs a = {};
-    auto fits = [&](int vec) {
-        if (d->interleaved ? (2 * d->pairs) % vec : d->pairs % vec) return false;
-        if ((d->dh - 2 * d->pairs) % vec) return false;
+    auto aligned = [&](int vec) {                                         // rows of whole vectors at whole vectors' places
+        if (d->dh % vec) return false;
         for (int i = 0; i < (d->heads[1] ? 2 : 1); ++i) {
             const void *x = i ? x1 : x0, *y = i ? y1 : y0;
             if (((uintptr_t)x | (uintptr_t)y) % (vec * size)) return false;
@@ -187,7 +243,11 @@ extern "C" int hs_rotary_axes(const hs_rotary_desc* d, const void* x0, void* y0,
         }
         return true;
     };
-    const int vec = fits(full) ? full : fits(2) ? 2 : 1;
+    const int P = d->pairs, vectors = d->dh / full;
+    int vec = aligned(full) ? full : aligned(2) ? 2 : 1, mode = d->interleaved ? PAIRS : SPLIT;
+    if (mode == SPLIT && vec == full && P % full == 0 && d->dh == 2 * P && vectors >= 2 && vectors <= 64 && !(vectors & (vectors - 1))) mode = LINE;
+    if (mode == SPLIT && vec == full && P % full && vectors <= MOST_STAGED) mode = STAGED;
+    if (mode == SPLIT && P % vec) vec = P % 2 == 0 ? 2 : 1;
     for (int i = 0; i < 2; ++i) {
         a.x[i] = i ? x1 : x0; a.y[i] = i ? y1 : y0;
         a.x_b[i] = d->x_b[i]; a.x_n[i] = d->x_n[i]; a.x_h[i] = d->x_h[i];
@@ -197,16 +257,14 @@ extern "C" int hs_rotary_axes(const hs_rotary_desc* d, const void* x0, void* y0,
     a.pos_a = d->pos_a; a.pos_b = d->pos_b; a.pos_n = d->pos_n;
     a.N = d->N; a.tokens = d->B * d->N; a.heads0 = d->heads[0]; a.heads = heads; a.P = d->pairs; a.dh = d->dh; a.pos_dtype = d->pos_dtype;
     a.inv_heads = 1.0f / heads; a.inverse = d->inverse ? -1.0f : 1.0f;
-    const int vectors = d->dh / full;
-    const bool pairs = d->interleaved, line = !pairs && vec == full && d->dh == 2 * d->pairs && vectors >= 2 && vectors <= 64 && !(vectors & (vectors - 1));
     // tokens of a block: about TARGET vectors, while the grid still gives every CU several blocks
-    const int tail = (d->dh - 2 * d->pairs) / vec, turned = line || pairs ? std::max(2 * d->pairs / vec, 1) : 2 * (d->pairs / vec);
-    a.tpb = std::max(1, std::min({TARGET / (heads * (turned + tail)), a.tokens / 2048, MOST_TOKENS}));
+    const int items = mode == SPLIT ? (d->dh - 2 * P) / vec + 2 * (P / vec) : std::max(d->dh / vec, 1);
+    a.tpb = std::max(1, std::min({TARGET / (heads * items), a.tokens / 2048, MOST_TOKENS}));
     if (a.tokens / a.tpb >= (1 << 24) - 1) return HS_ERR_SHAPE;                          // 2^32 threads
     hipStream_t s = (hipStream_t)stream;
-    if (d->dtype == HS_PREC_BF16) launch<HS_PREC_BF16>(a, vec, pairs, line, s);
-    else if (d->dtype == HS_PREC_F16) launch<HS_PREC_F16>(a, vec, pairs, line, s);
-    else launch<HS_PREC_F32>(a, vec, pairs, line, s);
+    if (d->dtype == HS_PREC_BF16) launch<HS_PREC_BF16>(a, vec, mode, s);
+    else if (d->dtype == HS_PREC_F16) launch<HS_PREC_F16>(a, vec, mode, s);
+    else launch<HS_PREC_F32>(a, vec, mode, s);
     HS_CHECK_LAUNCH();
     return HS_OK;
 }

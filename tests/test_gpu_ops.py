@@ -55,7 +55,10 @@ def turned(x, pos, plan, sign=1.0):
 @pytest.mark.parametrize("B,N,Hq,Hk,dh,sections,inter,dtype,pos", [
     (1, 1, 1, 0, 2, (1,), False, F32, "i32"), (2, 5, 3, 1, 64, (8, 12, 12), False, BF, "i32"), (2, 65, 12, 12, 64, (10, 11, 11), True, BF, "i64"),
     (3, 33, 4, 2, 80, (8, 13, 15), True, F32, "f32"), (1, 130, 2, 2, 33, (3, 0, 4), False, F16, "i32"), (1, 7, 2, 1, 33, (5, 11), True, F16, "i32"),
-    (2, 9, 5, 2, 96, (20, 13), False, F16, "i32"), (1, 4099, 3, 1, 128, (16, 24, 24), False, BF, "i32"), (4, 17, 2, 2, 34, (4, 9, 4), False, BF, "f32")])
+    (2, 9, 5, 2, 96, (20, 13), False, F16, "i32"), (1, 4099, 3, 1, 128, (16, 24, 24), False, BF, "i32"), (4, 17, 2, 2, 34, (4, 9, 4), False, BF, "f32"),
+    (1, 4100, 12, 12, 64, (7, 11, 11), False, BF, "i32"), (2, 31, 3, 2, 80, (9, 13, 9), False, F32, "f32"), (1, 6, 1, 0, 4096, (100, 203), False, F16, "i64"),
+    (1, 4100, 5, 3, 64, (7, 11, 11), True, BF, "i32"), (2, 31, 3, 1, 72, (9, 13, 9), True, F32, "f32"), (1, 9, 2, 1, 2080, (1,), False, F32, "i32"),
+    (2, 5, 40, 8, 8, (1, 1, 1), False, BF, "i32"), (2, 5, 40, 8, 8, (1, 1, 1), True, F16, "i32")])
 def test_rotary_values_and_gradient(dev, B, N, Hq, Hk, dh, sections, inter, dtype, pos):
     g = torch.Generator("cuda").manual_seed(B * 1000 + N)
     plan = H.RotaryAxes(sections, theta=5000.0, ladder="shared" if N % 2 else "per_axis", interleaved=inter)
