@@ -1,7 +1,9 @@
 // AdamW over many tensors in one launch, moments in fp32 or in 8 bits.
 //
 // Bound: HBM.  Per element: p read and written, g read, both moments read and written: 28 bytes with fp32 everywhere, 16 (+ 16 bytes a block of
-// 256 for the scales) with 8-bit moments.  The tensors' addresses travel in the kernel's arguments (no table in device memory that a later
+// 256 for the scales) with 8-bit moments.  125.8 M elements: fp32 659 us with fp32 moments, 388 with 8 bits; bf16 544 and 247: 5.1 to 5.3 TB/s (a plain
+// copy: 5.0).  With 8-bit moments in bf16 the vector instructions come near the bytes: 4 elements a lane and correctly rounded roots, quotients and
+// conversions took 394 us.  Accesses of 16 bytes, all of a block's in flight before the first is used.  The tensors' addresses travel in the kernel's arguments (no table in device memory that a later
 // call could overwrite while an earlier one still reads it); a block finds its tensor by comparing its number with the tensors' first blocks, a lane
 // each.  Half a wave owns one block of 256 elements, 8 a lane, so a block's scale is a maximum over 32 lanes and never leaves their registers.
 #include "../common.h"

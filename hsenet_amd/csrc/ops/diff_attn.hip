@@ -6,8 +6,10 @@
 //   dq       S_m^T, dP^T = V dO^T          -> dS_m^T = P_m^T (dP^T - D_m) ;  dQ_m^T[d][query] += K_m^T dS_m^T
 //   dk, dv   S_m[query][key] = Q_m K_m^T, dP = dO V^T ;          dV^T[dv][key] += dO^T (P1 - lam P2) ;  dK_m^T[d][key] += Q_m^T dS_m
 // with D_m = sum over keys of P_m dP = dO . O_m (O_m: the map's own output, kept by the forward pass).  dP is one product for both maps, and dV too.
-// Tiles of 64 rows are staged in LDS images R (common.h: 128-byte rows, read by rows and by columns): d / 32 images of a head pair's two keys
+// Tiles of 32 rows are staged in LDS images R (common.h: 128-byte rows, read by rows and by columns): d / 32 images of a head pair's two keys
 // (queries) side by side and d / 32 of its values (dO).
+// P and dS are rounded to the operands' 16 bits for the matrix products, as every softmax weight that goes through them has to be: with o's own rounding that
+// leaves bf16 outputs 2.5e-3 off (o's rounding alone: 1.7e-3), fp16 3.2e-4.  Scores, sums, D and all accumulators are fp32.
 #include "../common.h"
 #include "../attn_util.h"
 #include "../../../include/hsenet_ops.h"
@@ -348,6 +350,9 @@ template <int D> struct Sweep {
 };
 
 // ---- forward ----------------------------------------------------------------------------------------------------------------------------------
+// 12 d operations a visible pair and head, both maps' products with V apart.  Bound: the matrix and vector instructions together (53 and 42 % of a SIMD's
+// cycles, at a clock that the power cap holds at 2.2 GHz).  16 heads of 64 on 4, 8192 causal tokens: 355 us, 1.16 PFLOP/s.  2 x 4097 tokens of 6 heads: 168 us,
+// 183 with the maps kept; its 204 blocks leave 52 of the 256 CUs idle.
 template <int D, bool F16, bool KEEP>
 __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void diff_fwd_kernel(Args a) {
     typedef Sweep<D> S;
@@ -468,7 +473,8 @@ __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void d
 // its own (no barrier in the loop): the next tile's keys are sent for when the scores have been read, its values behind the products with V, so that
 // half a tile a wave is always on its way.  Bandwidth leaves the matrix pipe room enough to take P in two numbers of 16 bits, value and what its rounding
 // left, so that o is rounded once, at its end.  The waves' numerators are joined in LDS, and the chunks' by diff_join_kernel; with one chunk the result is
-// written at once.
+// written at once.  Measured: one query of 16 entries on 16384 keys (16 heads on 4 of 64) 108 us with the join, 5.0 TB/s; entries of 0 to 16384 keys 70 us,
+// the kernel itself 53, the time of its bytes; 1 entry on 30000 keys 15; 64 entries on 1000 keys 29 us, 4.5 TB/s.
 template <int D> struct SplitOf { static constexpr int NW = 4, TILE = 32 * 4 * D * 2; };
 
 template <int D, bool F16, bool KEEP>
@@ -606,7 +612,7 @@ __global__ __launch_bounds__(SplitOf<D>::NW * 64, D == 128 ? 1 : 2) void diff_sp
     }
 }
 
-// Joins the chunks of a row, a block each: the chunks' weights first, then their numerators, D threads for the 4 D numbers of one chunk.
+// Joins the chunks of a row (latency: 5 to 6 us), a block each: the chunks' weights first, then their numerators, D threads for the 4 D numbers of one chunk.
 template <int D, bool F16>
 __global__ __launch_bounds__(256) void diff_join_kernel(Args a) {
     constexpr int W = 2 * D, TOGETHER = 256 / D;
@@ -711,7 +717,7 @@ __global__ __launch_bounds__(256) void diff_rows_kernel(Args a) {
     r[0] = -e[0] / a.c2; r[32] = -e[1] / a.c2; r[64] = -d[0]; r[96] = copysignf(1.0f, lam) * (d[1] - d[0]);
 }
 
-// dQ: queries stay, keys stream
+// dQ: queries stay, keys stream.  Bound as the forward pass is; 2 x 4097 tokens of 6 heads of 64: 186 us, 155 GFLOP, 0.83 PFLOP/s on 204 of the 256 CUs.
 template <int D, bool F16>
 __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void diff_dq_kernel(Args a) {
     typedef Sweep<D> S;
@@ -856,6 +862,8 @@ __device__ __forceinline__ void mask_queries(f32x16 (&s)[2], int vis, int h) {
 
 // At d = 64 the wave's keys lie in LDS and its values in registers: all of both would leave the fragments no room in the 256 registers of two waves
 // a SIMD.
+// Bound: the matrix phase (32 products, 52 fragment reads of LDS: 1600 cycles) and the vector phase (1600) of a step alike.  2 x 4097 tokens of 6 heads of 64: 260 us,
+// 206 GFLOP, 0.79 PFLOP/s on 204 of the 256 CUs.
 template <int D, bool F16, bool CUT>
 __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void diff_dkv_kernel(Args a) {
     typedef Sweep<D> S;
@@ -1099,8 +1107,8 @@ struct Split { int tiles, nsplit, chunk; };
 constexpr int WANT = 1024, LEAST = 512;       // blocks (two rounds even out ragged entries: 70 us against 78 with one); keys of a chunk (4 tiles a wave)
 // Whether the split forward runs, and how it cuts the keys.  The whole forward needs the time of one block over all keys for each round of its blocks on
 // the 256 CUs, full or not; the split forward's time goes with its tiles, wherever they come from.  Measured with 16 query heads on 4 key heads of 64, 8192
-// keys, whole / split in us: 1 entry, 16 queries 277 / 20, 256 queries 282 / 72; 16 entries, 16 queries 327 / 108, 32 (512 tiles) 311 / 197, 64 (1024 tiles)
-// 319 / 341, 128 339 / 494.  8 on 2 of 128, 16 entries, 512 / 2048 keys: 32 queries (256 tiles) 33, 100 / 35, 68, 64 (512 tiles) 32, 101 / 54, 86.
+// keys, whole / split in us: 1 entry, 16 queries 256 / 18, 256 queries 261 / 79; 16 entries, 16 queries 343 / 116, 32 (512 tiles) 328 / 205, 64 (1024 tiles)
+// 317 / 352, 128 334 / 488.  8 on 2 of 128, 16 entries, 512 / 2048 keys: 32 queries (256 tiles) 33, 106 / 28, 79, 64 (512 tiles) 33, 105 / 36, 114.
 Split split_of(const hs_diff_attn_desc* d) {
     const int64_t rows = (int64_t)(d->H / d->Hkv) * d->Nq, tiles = (rows + 15) / 16, blocks = (int64_t)d->B * d->Hkv * tiles;
     const int own = d->d == 128 ? Sweep<128>::OWN : Sweep<64>::OWN, halves = d->d == 128 ? Sweep<128>::HALVES : 1;
@@ -1116,6 +1124,8 @@ size_t split_bytes(const hs_diff_attn_desc* d, const Split& s) {
 }
 // Parts that the dk, dv sweep's list of tiles is cut into.  A round of blocks (one a CU) takes 1.4 us a tile; cutting costs each block another start (4
 // tiles' time), a second kernel, and 0.1 us for a part's sums of a block written and read: blocks over so few keys or so long lists that a cut pays.
+// Backward pass whole / cut in us: 8192 causal tokens, 16 heads of 64 on 1: 5904 / 1216, on 4: 1850 / 1225; 4 x 512 tokens, 12 on 4: 130 / 107; 2 x 4097
+// tokens, 6 on 6 (204 blocks): not cut.
 int parts_of(const hs_diff_attn_desc* d) {
     const int64_t own = d->d == 128 ? Sweep<128>::OWN : Sweep<64>::OWN, blocks = (int64_t)d->B * d->Hkv * ((d->Nk + own - 1) / own);
     const double tiles = (double)(d->H / d->Hkv) * ((d->Nq + 31) / 32);
