@@ -1104,7 +1104,7 @@ int check(const hs_diff_attn_desc* d, bool backward) {
 bool misaligned(const void* p, unsigned n = 16) { return !p || (uintptr_t)p % n; }
 
 struct Split { int tiles, nsplit, chunk; };
-constexpr int WANT = 1024, LEAST = 512;       // blocks (two rounds even out ragged entries: 70 us against 78 with one); keys of a chunk (4 tiles a wave)
+constexpr int SPARSE = 128, WANT = 1024, LEAST = 512;       // blocks (two rounds even out ragged entries: 70 us against 78 with one); keys of a chunk (4 tiles a wave)
 // Whether the split forward runs, and how it cuts the keys.  The whole forward needs the time of one block over all keys for each round of its blocks on
 // the 256 CUs, full or not; the split forward's time goes with its tiles, wherever they come from.  Measured with 16 query heads on 4 key heads of 64, 8192
 // keys, whole / split in us: 1 entry, 16 queries 256 / 18, 256 queries 261 / 79; 16 entries, 16 queries 343 / 116, 32 (512 tiles) 328 / 205, 64 (1024 tiles)
@@ -1115,7 +1115,9 @@ Split split_of(const hs_diff_attn_desc* d) {
     const int64_t rounds = ((int64_t)d->B * d->H * ((d->Nq + own - 1) / own) * halves + 255) / 256;
     if (blocks > rounds * (d->d == 128 ? 256 : 512)) return {0, 0, 0};
     const int64_t want = std::min<int64_t>((WANT + blocks - 1) / blocks, MOST_CHUNKS);
-    const int64_t chunk = std::max<int64_t>(((d->Nk + want - 1) / want + 127) / 128 * 128, LEAST);
+    // (a grid that leaves most CUs idle anyway takes half as long chunks, unless one would do without the join: 1 entry, 2000 keys 12 -> 11 us)
+    const int64_t least = d->Nk > LEAST && blocks * ((d->Nk + LEAST - 1) / LEAST) <= SPARSE ? LEAST / 2 : LEAST;
+    const int64_t chunk = std::max<int64_t>(((d->Nk + want - 1) / want + 127) / 128 * 128, least);
     return {(int)tiles, (int)((d->Nk + chunk - 1) / chunk), (int)chunk};
 }
 size_t split_bytes(const hs_diff_attn_desc* d, const Split& s) {

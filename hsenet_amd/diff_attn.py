@@ -61,8 +61,8 @@ def _forward(q, k, v, lam, scale, causal, q_start, kv_len, keep):
     """-> (o, and for a backward pass the descriptor's numbers, the operands as they were read, the maps' outputs and statistics)"""
     dev, numbers, q, k, v, lam = _prepare(q, k, v, lam, scale, causal, q_start, kv_len)
     _, B, Nq, Nk, H, _, d = numbers[:7]
-    o = torch.empty(B, Nq, H, 2 * d, dtype=q.dtype, device=q.device)
-    maps = torch.empty(2, B, Nq, H, 2 * d, dtype=q.dtype, device=q.device) if keep else None
+    o = q.new_empty((B, Nq, H, 2 * d))
+    maps = q.new_empty((2, B, Nq, H, 2 * d)) if keep else None
     lse = torch.empty(B, H, 4, Nq, dtype=torch.float32, device=q.device) if keep else None
     if B * Nq:
         if Nk == 0:
@@ -96,8 +96,7 @@ class DiffAttnFn(torch.autograd.Function):
         q, k, v, lam, q_start, kv_len, maps, lse = ctx.saved_tensors
         dev = O.device_of(q, go)
         go, sg = _placed(go)
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        dlam = torch.empty(lam.shape, dtype=torch.float32, device=q.device)
+        dq, dk, dv, dlam = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v, lam))
         if q.numel() == 0 or k.numel() == 0:
             return (*(t.zero_() for t in (dq, dk, dv, dlam)), None, None, None, None)
         desc = O.DIFF_PACK.pack(*ctx.numbers, *sg)
