@@ -64,18 +64,17 @@ def _turn(xs, positions, plan, inverse, inplace):
     pos_dtype = _POS.get(positions.dtype)
     if pos_dtype is None:
         raise L.HsError(f"positions must be int32, int64 or float32, got {positions.dtype}")
-    if tuple(positions.shape) == (plan.axes, B, N):
-        pos = positions.stride()
-    elif tuple(positions.shape) == (plan.axes, N):
-        pos = (positions.stride(0), 0, positions.stride(1))
-    else:
+    pshape, pos = positions.shape, positions.stride()
+    if pshape == (plan.axes, N):
+        pos = (pos[0], 0, pos[1])
+    elif pshape != (plan.axes, B, N):
         raise L.HsError(f"positions must be [axes, N] or [axes, B, N] = ({plan.axes}, {B}, {N}), got {tuple(positions.shape)}")
     outs, live = [], []
     for x in xs:
         xshape = x.shape
-        if x.dtype != dt or len(xshape) != 4 or xshape[0] != B or xshape[1] != N or xshape[3] != dh:
+        if x.dtype is not dt or len(xshape) != 4 or xshape[0] != B or xshape[1] != N or xshape[3] != dh:
             raise L.HsError("q and k must be [B, N, heads, columns] of one type, equal in B, N and columns")
-        stride = x.stride()
+        stride, h = x.stride(), xshape[2]
         if stride[3] != 1 and dh > 1:
             if inplace:
                 raise L.HsError("a tensor that is turned in place must have its columns side by side")
@@ -86,11 +85,11 @@ def _turn(xs, positions, plan, inverse, inplace):
                 raise L.HsError("a broadcast tensor cannot be turned in place")
             y, ystride = x, stride
         else:
-            y = torch.empty(xshape, dtype=dt, device=x.device)
-            ystride = y.stride()
+            y = torch.empty_like(x, memory_format=torch.contiguous_format)
+            ystride = (N * h * dh, h * dh, dh, 1)
         outs.append(y)
-        if y.numel():
-            live.append((xshape[2], x, O.bnh(xshape, stride), y, O.bnh(xshape, ystride)))
+        if B * N * h * dh:
+            live.append((h, x, O.bnh(xshape, stride), y, O.bnh(xshape, ystride)))
     if live:
         h0, x0, s0, y0, t0 = live[0]
         h1, x1, s1, y1, t1 = live[1] if len(live) > 1 else (0, None, (0, 0, 0), None, (0, 0, 0))
