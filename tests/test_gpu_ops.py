@@ -3,6 +3,7 @@
 Tolerances are bounds, element by element.  A rounding to a type is off by at most half a step, eps / 2 of the value (fp16 also by 2^-25, half its
 smallest step).  What is rounded on the way is the P and dS of the matrix products' operands, the maps' own outputs that D = dO . O_m is made of, and
 the result; everything else is fp32: its errors are taken as 2^-22 of the absolute sums, times 1 + the largest score for the exponents."""
+import copy
 import math
 
 import pytest
@@ -603,6 +604,30 @@ def test_adamw_refusals(dev):
     for bad in (([m], []), ([m.half()], [m.half()]), ([m[:4]], [m[:4]]), ([m.t()[:, :4]], [m]), ([m], [m.bfloat16()])):
         with pytest.raises(L.HsError):
             opt.read_moments(*bad)
+
+
+def test_adamw_steps_a_tower(dev):
+    """the framework's own encoder under this optimizer: the steps of torch's AdamW, and a forward pass that uses the new weights"""
+    torch.manual_seed(4)
+    a = H.ViT_stage1(1, (8, 32, 32), (4, 16, 16), num_layers=1, pos_embed="perceptron", classification=True).to("cuda").eval()
+    b = copy.deepcopy(a)
+    x = torch.rand(2, 1, 8, 32, 32, device="cuda")
+    kw = dict(lr=1e-2, betas=(0.9, 0.99), eps=1e-8, weight_decay=0.1)
+    mine, other = H.AdamW(a.parameters(), **kw), torch.optim.AdamW(b.parameters(), **kw)
+    old = a(x)[0].detach().clone()
+    for _ in range(2):
+        mine.zero_grad(), other.zero_grad()
+        a(x)[0].square().sum().backward()
+        for p, q in zip(a.parameters(), b.parameters()):
+            q.grad = None if p.grad is None else p.grad.clone()
+            q.data.copy_(p)
+        mine.step(), other.step()
+        for (n, p), q in zip(a.named_parameters(), b.parameters()):
+            # a step is at most lr (1 / (1 - beta1)) long; a dozen roundings of 2^-24 on it, two on the weight
+            assert ((p - q).abs() <= 12 * 2.0 ** -24 * 10 * kw["lr"] + 2.0 ** -23 * q.abs()).all(), n
+    b.load_state_dict(a.state_dict())
+    new = a(x)[0]
+    assert torch.equal(new, b(x)[0]) and not torch.equal(new, old)
 
 
 # ---- the three together ----------------------------------------------------------------------------------------------------------
