@@ -12,6 +12,7 @@
 // leaves bf16 outputs 2.5e-3 off (o's rounding alone: 1.7e-3), fp16 3.2e-4.  Scores, sums, D and all accumulators are fp32.
 #include "../common.h"
 #include "../attn_util.h"
+#include <type_traits>
 #include "../../../include/hsenet_ops.h"
 
 namespace {
@@ -191,6 +192,14 @@ __device__ __forceinline__ void follow_max(const f32x16& s, float c2, float& m, 
         m = mn;
     }
 }
+// the reference that the first 32 keys of a row give
+__device__ __forceinline__ float first_max(const f32x16& s, float c2) {
+    float mx = s[0];
+#pragma unroll
+    for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
+    mx *= c2;
+    return fmaxf(NONE, ceilf(fmaxf(mx, __shfl_xor(mx, 32, 64))));
+}
 template <bool F16> __device__ __forceinline__ float add2(unsigned pair, float sum) {      // sum + both halves, in fp32
     typedef __attribute__((ext_vector_type(2))) __bf16 b2;
     typedef __attribute__((ext_vector_type(2))) _Float16 h2;
@@ -297,8 +306,8 @@ template <int SUMS> __device__ __forceinline__ void take_up(float (&l)[2][SUMS],
         if (SUMS == 2) l[i][SUMS - 1] += whole[i];
     }
 }
-// the products with V, and with PAIRED the sums, while the first fragments are on their way
-template <int D, bool F16, int ROWS, bool PAIRED, int NB, int SUMS>
+// the products with V, and the sums while the first fragments are on their way
+template <int D, bool F16, int ROWS, int NB, int SUMS>
 __device__ __forceinline__ void values(const Lane& f, const bf16x8 (&p)[2][2], const f32x16 (&s)[2], f32x16 (&o1)[NB], f32x16 (&o2)[NB], float (&l)[2][SUMS]) {
     constexpr int N = 2 * NB, AHEAD = 4;
     bf16x8 x[AHEAD];
@@ -306,11 +315,9 @@ __device__ __forceinline__ void values(const Lane& f, const bf16x8 (&p)[2][2], c
 #pragma unroll
     for (int n = 0; n < AHEAD; ++n) x[n] = f.template cols32<ROWS>(16 * (n / NB), 2 * D + n % NB * 32);
     __builtin_amdgcn_sched_barrier(0);
-    if (PAIRED) {
-        add_weights<F16, SUMS>(p, s, part, whole);
-        if (SUMS == 1) take_up(l, part, whole);
-        __builtin_amdgcn_sched_barrier(0);
-    }
+    add_weights<F16, SUMS>(p, s, part, whole);
+    if (SUMS == 1) take_up(l, part, whole);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int n = 0; n < N; ++n) {
         const int sp = n / NB, db = n % NB, q = n + AHEAD;
@@ -319,7 +326,7 @@ __device__ __forceinline__ void values(const Lane& f, const bf16x8 (&p)[2][2], c
         if (q < N) x[n % AHEAD] = f.template cols32<ROWS>(16 * (q / NB), 2 * D + q % NB * 32);
         __builtin_amdgcn_sched_barrier(0);
     }
-    if (PAIRED && SUMS == 2) take_up(l, part, whole);                     // (here it costs fewer registers)
+    if (SUMS == 2) take_up(l, part, whole);                     // (here it costs fewer registers)
 }
 
 // ---- the phases of a sweep -----------------------------------------------------------------------------------------------------------------------
@@ -327,13 +334,13 @@ __device__ __forceinline__ void values(const Lane& f, const bf16x8 (&p)[2][2], c
 // softmax weights of the step) and a matrix phase (the products that the weights go into, then the next step's scores), a barrier behind each.
 // At d = 32 and 64 a block has 8 waves; w and w + 4 share a SIMD, and the later four run half a step behind: while one works on the vector units, the
 // other has the matrix pipe (left to themselves both do the same thing at the same time).  The vector phase is the longer one: sums of what it made, that
-// nobody waits for, are taken in the matrix phase (forward at d = 64: 4 % faster with one sum a map, 12 % with two; at d = 128 3 % slower).  At d = 128 a
-// SIMD's registers hold one wave only, and the forward pass' numerators of half of the values: two blocks then, each with the scores of all.
+// nobody waits for, are taken in the matrix phase (forward at d = 64: 4 % faster with one sum a map, 12 % with two).  At d = 128 a SIMD's registers hold one
+// wave only, and the forward pass has a kernel of its own.
 // Tile t is first read in the matrix phase of step t - 1 and left in step t's, half a step later by the later waves: it is sent for in step t - LEAD
 // into the buffer of tile t - BUFS.
 template <int D> struct Sweep {
     static constexpr bool PAIRED = D < 128;
-    static constexpr int NW = PAIRED ? 8 : 4, ROWS = 32, TILE = ROWS * D * 8, HALVES = PAIRED ? 1 : 2, VC = 2 * D / HALVES, BUFS = PAIRED ? 5 : 3, LEAD = PAIRED ? 3 : 2, OWN = NW * 32;
+    static constexpr int NW = PAIRED ? 8 : 4, ROWS = 32, TILE = ROWS * D * 8, BUFS = PAIRED ? 5 : 3, LEAD = PAIRED ? 3 : 2, OWN = NW * 32;
     static __device__ __forceinline__ void fall_behind(int wave) { if (PAIRED && wave >= NW / 2) __syncthreads(); }
     static __device__ __forceinline__ void wait_for_late(int wave) { if (PAIRED && wave < NW / 2) __syncthreads(); }
     static __device__ __forceinline__ int next(int buf) { return buf == BUFS - 1 ? 0 : buf + 1; }
@@ -356,14 +363,13 @@ template <int D> struct Sweep {
 template <int D, bool F16, bool KEEP>
 __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void diff_fwd_kernel(Args a) {
     typedef Sweep<D> S;
-    constexpr int ROWS = S::ROWS, VC = S::VC, TILE = ROWS * (2 * D + VC) * 2, NW = S::NW, NB = VC / 32;
+    static_assert(S::PAIRED, "d = 128: diff_fwd_wide_kernel");
+    constexpr int ROWS = S::ROWS, TILE = S::TILE, NW = S::NW, NB = D / 16;
     extern __shared__ __attribute__((aligned(16))) char smem[];           // BUFS tiles
     const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, c = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int nblk = (a.Nq + NW * 32 - 1) / (NW * 32);
     int id = block_order();
-    const int half = id % S::HALVES;
-    id /= S::HALVES;
     const int blk = nblk - 1 - id % nblk;                                 // under a causal mask the last queries have most to do: first
     id /= nblk;
     const int head = id % a.H, b = id / a.H, kvh = head / a.G;
@@ -376,8 +382,8 @@ __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void d
     Lane fl;
     fl.init(smem, lane);
     const unsigned lds0 = lds_addr(smem);
-    Dma<D, VC, ROWS, NW> dma;
-    const bf16_t *kp = a.k + b * a.k_b + 2 * kvh * a.k_h, *vp = a.v + b * a.v_b + kvh * a.v_h + half * VC;
+    Dma<D, 2 * D, ROWS, NW> dma;
+    const bf16_t *kp = a.k + b * a.k_b + 2 * kvh * a.k_h, *vp = a.v + b * a.v_b + kvh * a.v_h;
     dma.init(wave, lane, kp, a.k_n, a.k_h, vp, a.v_n, 0, len);
     for (int t = 0; t < min(S::LEAD, nj); ++t) { dma.issue(lds0 + t * TILE); dma.skip(ROWS); }
     bf16x8 qf[2][D / 16];
@@ -421,15 +427,10 @@ __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void d
             bf16x8 p[2][2];
             softmax_weights<F16>(s[0], a.c2, m[0], p[0]);
             softmax_weights<F16>(s[1], a.c2, m[1], p[1]);
-            if (!S::PAIRED) {
-                float part[2] = {0.f, 0.f}, whole[2] = {0.f, 0.f};
-                add_weights<F16, SUMS>(p, s, part, whole);
-                take_up(l, part, whole);
-            }
             S::template behind_vector<decltype(dma)>(j + S::LEAD < nj);
             __syncthreads();
             __builtin_amdgcn_s_setprio(1);
-            values<D, F16, ROWS, S::PAIRED>(fl.at(buf * TILE), p, s, o1, o2, l);
+            values<D, F16, ROWS>(fl.at(buf * TILE), p, s, o1, o2, l);
             buf = S::next(buf);
             scores<D, F16, ROWS>(fl.at(buf * TILE), qf, s);
             __builtin_amdgcn_s_setprio(0);
@@ -448,12 +449,12 @@ __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void d
         for (int k = 0; k < SUMS; ++k) l[i][k] += __shfl_xor(l[i][k], 32, 64);
         inv[i] = l[i][0] > 0.f ? 1.0f / l[i][0] : l[i][0] == 0.f ? 0.f : l[i][0];      // (a NaN stays one)
     }
-    const long row = ((long)b * a.Nq + query) * a.H + head, at = row * 2 * D + half * VC;
+    const long row = ((long)b * a.Nq + query) * a.H + head, at = row * 2 * D;
     if (KEEP) {
         store_rows<F16>(a.maps + at, o1, inv[0], h);
         store_rows<F16>(a.maps + (long)a.B * a.Nq * a.H * 2 * D + at, o2, inv[1], h);
         float* ls = a.lse + ((long)b * a.H + head) * 4 * a.Nq + query;
-        if (h == 0 && half == 0) {
+        if (h == 0) {
             put_lse(ls, 2 * a.Nq, m[0], l[0][SUMS - 1]);
             put_lse(ls + a.Nq, 2 * a.Nq, m[1], l[1][SUMS - 1]);
         }
@@ -464,6 +465,131 @@ __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void d
 #pragma unroll
         for (int r = 0; r < 16; ++r) o1[db][r] = __builtin_fmaf(-w2, o2[db][r], o1[db][r] * inv[0]);
     store_rows<F16>(a.o + at, o1, 1.0f, h);
+}
+
+// one map's scores at d = 128
+template <bool F16, int ROWS> __device__ __forceinline__ void one_score(const Lane& f, const bf16x8 (&qf)[8], f32x16& s) {
+    constexpr int AHEAD = 4;
+    bf16x8 x[AHEAD];
+#pragma unroll
+    for (int n = 0; n < AHEAD; ++n) x[n] = f.template rows16<ROWS>(n * 16);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+        s = mfma32<F16>(x[n % AHEAD], qf[n], n ? s : zero16());
+        if (n + AHEAD < 8) x[n % AHEAD] = f.template rows16<ROWS>((n + AHEAD) * 16);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
+// Forward pass at d = 128: one map after the other.  Both maps' numerators are half of a lane's registers; map 1's outputs wait there, finished, while map 2's
+// are made.  A SIMD holds one wave, so nothing alternates, and a step needs one barrier: the tile sent for in step j goes where tile j - 2 was, which all
+// waves have left by the barrier of step j - 1.  2 x 4096 tokens of 4 heads: 241 us, 252 with the maps kept,
+// 0.86 PFLOP/s (both maps at once in two blocks of half the values, each with all scores: 390 and 412).
+struct Wide { static constexpr int D = 128, W = 256, ROWS = 32, NW = Sweep<128>::NW, OWN = Sweep<128>::OWN, BUFS = 4, LEAD = 2, TILE = ROWS * (D + W) * 2; };
+template <bool F16, bool KEEP>
+__global__ __launch_bounds__(Wide::NW * 64, 1) void diff_fwd_wide_kernel(Args a) {
+    typedef Wide S;
+    constexpr int ROWS = S::ROWS, TILE = S::TILE, NB = S::W / 32, SUMS = KEEP ? 2 : 1;
+    extern __shared__ __attribute__((aligned(16))) char smem[];           // BUFS tiles: a map's keys, two images, and the values, four
+    const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, c = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int nblk = (a.Nq + S::OWN - 1) / S::OWN;
+    int id = block_order();
+    const int blk = nblk - 1 - id % nblk;
+    id /= nblk;
+    const int head = id % a.H, b = id / a.H, kvh = head / a.G;
+    const int len = key_count(a, b), start = first_pos(a, b);
+    const int q0 = blk * S::OWN + wave * 32, query = q0 + c;
+    const int kend = visible(a, len, start, min(blk * S::OWN + S::OWN, a.Nq) - 1);
+    const int lim = visible(a, len, start, query), lim_lo = visible(a, len, start, q0);
+    const int nj = (kend + ROWS - 1) / ROWS;
+    Lane fl;
+    fl.init(smem, lane);
+    const unsigned lds0 = lds_addr(smem);
+    typedef Dma<64, S::W, ROWS, S::NW> Tiles;                             // (128 columns of one map: two images of 64, 64 columns apart)
+    Tiles dma;
+    const bf16_t *kp = a.k + b * a.k_b + 2 * kvh * a.k_h, *vp = a.v + b * a.v_b + kvh * a.v_h;
+    dma.init(wave, lane, kp, a.k_n, 64, vp, a.v_n, 0, len);
+    const float lam = a.lam[head * a.lam_stride];
+    const long row = ((long)b * a.Nq + query) * a.H + head, at = row * S::W;
+    f32x16 done[NB];
+#pragma unroll
+    for (int map = 0; map < 2; ++map) {
+        bf16x8 qf[S::D / 16];
+        const bf16_t* qp = a.q + b * a.q_b + (long)min(query, a.Nq - 1) * a.q_n + (2 * head + map) * a.q_h + 8 * h;
+#pragma unroll
+        for (int ks = 0; ks < S::D / 16; ++ks) qf[ks] = load8(qp + ks * 16);
+        float m, l[SUMS];
+        f32x16 o[NB], s;
+        // With a fixed reference of a row's scores or a running one (see diff_fwd_kernel).  Two loops: numerators that a step may have to rescale do not
+        // stay in the accumulation registers, which costs 128 copies a step.
+        auto sweep = [&](auto kind) {
+            constexpr bool RUNNING = decltype(kind)::value;
+            dma.start(kp + map * a.k_h, vp, 0, len);
+            for (int t = 0; t < min(S::LEAD, nj); ++t) { dma.issue(lds0 + t * TILE); dma.skip(ROWS); }
+            m = NONE;
+            l[0] = l[SUMS - 1] = 0.f;
+            clear(o);
+            arrived();
+            dma.landed();
+            __syncthreads();
+            one_score<F16, ROWS>(fl, qf, s);                              // (without a tile, or behind the last: of what lies there, not used)
+            int buf = 0, ahead = S::LEAD;
+            for (int j = 0; j < nj; ++j) {
+                if (j + S::LEAD < nj) dma.issue(lds0 + ahead * TILE);
+                dma.skip(ROWS);
+                ahead = (ahead + 1) & (S::BUFS - 1);
+                if (j * 32 + 32 > lim_lo)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[r] = acc_row(r, h) < lim - j * 32 ? s[r] : -__builtin_inff();
+                if (RUNNING) follow_max(s, a.c2, m, l, o);
+                else if (j == 0) m = first_max(s, a.c2);
+                bf16x8 p[2];
+                softmax_weights<F16>(s, a.c2, m, p);
+                float part[2] = {0.f, 0.f}, whole[2] = {0.f, 0.f};
+#pragma unroll
+                for (int e = 0; e < 8; ++e) part[e & 1] = add2<F16>(__builtin_bit_cast(u32x4, p[e >> 2])[e & 3], part[e & 1]);
+                l[0] += part[0] + part[1];
+                if (KEEP) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) whole[r & 1] += s[r];
+                    l[SUMS - 1] += whole[0] + whole[1];
+                }
+                Sweep<128>::behind_vector<Tiles>(j + S::LEAD < nj);
+                __syncthreads();
+                const Lane f = fl.at(buf * TILE);
+                buf = (buf + 1) & (S::BUFS - 1);
+                constexpr int N = 2 * NB, AHEAD = 4;
+                bf16x8 x[AHEAD];
+#pragma unroll
+                for (int n = 0; n < AHEAD; ++n) x[n] = f.template cols32<ROWS>(16 * (n / NB), S::D + n % NB * 32);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int n = 0; n < N; ++n) {
+                    o[n % NB] = mfma32<F16>(x[n % AHEAD], p[n / NB], o[n % NB]);
+                    if (n + AHEAD < N) x[n % AHEAD] = f.template cols32<ROWS>(16 * ((n + AHEAD) / NB), S::D + (n + AHEAD) % NB * 32);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                one_score<F16, ROWS>(fl.at(buf * TILE), qf, s);
+            }
+            return __syncthreads_or(!(l[0] < (F16 ? 32768.f : 1.0995116e12f)));
+        };
+        if (sweep(std::false_type())) sweep(std::true_type());
+#pragma unroll
+        for (int k = 0; k < SUMS; ++k) l[k] += __shfl_xor(l[k], 32, 64);
+        const float inv = l[0] > 0.f ? 1.0f / l[0] : l[0] == 0.f ? 0.f : l[0];      // (a NaN stays one)
+        if (KEEP && query < a.Nq) {
+            store_rows<F16>(a.maps + map * (long)a.B * a.Nq * a.H * S::W + at, o, inv, h);
+            if (h == 0) put_lse(a.lse + (((long)b * a.H + head) * 4 + map) * a.Nq + query, 2 * a.Nq, m, l[SUMS - 1]);
+        }
+        const float w2 = lam * inv;
+#pragma unroll
+        for (int db = 0; db < NB; ++db)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) done[db][r] = map ? __builtin_fmaf(-w2, o[db][r], done[db][r]) : o[db][r] * inv;
+    }
+    if (query < a.Nq) store_rows<F16>(a.o + at, done, 1.0f, h);
 }
 
 // ---- split forward: few queries against many keys ------------------------------------------------------------------------------------------
@@ -1108,12 +1234,12 @@ constexpr int SPARSE = 128, WANT = 1024, LEAST = 512;       // blocks (two round
 // Whether the split forward runs, and how it cuts the keys.  The whole forward needs the time of one block over all keys for each round of its blocks on
 // the 256 CUs, full or not; the split forward's time goes with its tiles, wherever they come from.  Measured with 16 query heads on 4 key heads of 64, 8192
 // keys, whole / split in us: 1 entry, 16 queries 256 / 18, 256 queries 261 / 79; 16 entries, 16 queries 343 / 116, 32 (512 tiles) 328 / 205, 64 (1024 tiles)
-// 317 / 352, 128 334 / 488.  8 on 2 of 128, 16 entries, 512 / 2048 keys: 32 queries (256 tiles) 33, 106 / 28, 79, 64 (512 tiles) 33, 105 / 36, 114.
+// 317 / 352, 128 334 / 488.  8 on 2 of 128, 16 entries, 512 / 2048 keys: 32 queries (256 tiles) 36, 116 / 27, 74, 64 (512 tiles) 37, 117 / 36, 107.
 Split split_of(const hs_diff_attn_desc* d) {
     const int64_t rows = (int64_t)(d->H / d->Hkv) * d->Nq, tiles = (rows + 15) / 16, blocks = (int64_t)d->B * d->Hkv * tiles;
-    const int own = d->d == 128 ? Sweep<128>::OWN : Sweep<64>::OWN, halves = d->d == 128 ? Sweep<128>::HALVES : 1;
-    const int64_t rounds = ((int64_t)d->B * d->H * ((d->Nq + own - 1) / own) * halves + 255) / 256;
-    if (blocks > rounds * (d->d == 128 ? 256 : 512)) return {0, 0, 0};
+    const int own = d->d == 128 ? Sweep<128>::OWN : Sweep<64>::OWN;
+    const int64_t rounds = ((int64_t)d->B * d->H * ((d->Nq + own - 1) / own) + 255) / 256;
+    if (blocks > rounds * 512) return {0, 0, 0};
     const int64_t want = std::min<int64_t>((WANT + blocks - 1) / blocks, MOST_CHUNKS);
     // (a grid that leaves most CUs idle anyway takes half as long chunks, unless one would do without the join: 1 entry, 2000 keys 12 -> 11 us)
     const int64_t least = d->Nk > LEAST && blocks * ((d->Nk + LEAST - 1) / LEAST) <= SPARSE ? LEAST / 2 : LEAST;
@@ -1160,14 +1286,15 @@ template <class K> void launch(K kernel, int64_t grid, int threads, size_t lds, 
 }
 template <int D, bool F16, bool KEEP> void forward(const Args& a, const Split& sp, hipStream_t s) {
     typedef Sweep<D> S;
-    constexpr int TILE = S::ROWS * (2 * D + S::VC) * 2;
     if (sp.nsplit) {
         typedef SplitOf<D> P;
         launch(diff_split_kernel<D, F16, KEEP>, (int64_t)a.B * a.Hkv * sp.tiles * sp.nsplit, P::NW * 64, (size_t)P::NW * P::TILE, s, a);
         if (sp.nsplit > 1) launch(diff_join_kernel<D, F16>, (int64_t)a.B * a.H * a.Nq, 256, 0, s, a);
         return;
     }
-    launch(diff_fwd_kernel<D, F16, KEEP>, (int64_t)a.B * a.H * ((a.Nq + S::OWN - 1) / S::OWN) * S::HALVES, S::NW * 64, (size_t)S::BUFS * TILE, s, a);
+    const int64_t blocks = (int64_t)a.B * a.H * ((a.Nq + S::OWN - 1) / S::OWN);
+    if constexpr (D == 128) launch(diff_fwd_wide_kernel<F16, KEEP>, blocks, Wide::NW * 64, (size_t)Wide::BUFS * Wide::TILE, s, a);
+    else launch(diff_fwd_kernel<D, F16, KEEP>, blocks, S::NW * 64, (size_t)S::BUFS * S::TILE, s, a);
 }
 template <int D, bool F16> void backward(const Args& a, hipStream_t s) {
     typedef Sweep<D> S;
