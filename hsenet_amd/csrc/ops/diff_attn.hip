@@ -335,12 +335,13 @@ __device__ __forceinline__ void values(const Lane& f, const bf16x8 (&p)[2][2], c
 // At d = 32 and 64 a block has 8 waves; w and w + 4 share a SIMD, and the later four run half a step behind: while one works on the vector units, the
 // other has the matrix pipe (left to themselves both do the same thing at the same time).  The vector phase is the longer one: sums of what it made, that
 // nobody waits for, are taken in the matrix phase (forward at d = 64: 4 % faster with one sum a map, 12 % with two).  At d = 128 a SIMD's registers hold one
-// wave only, and the forward pass has a kernel of its own.
+// wave only; nothing alternates there, the barrier behind the matrix phase goes (2 to 4 %: with a fourth buffer, the one that is sent to was left before the
+// barrier of the step before), and the forward pass has a kernel of its own.
 // Tile t is first read in the matrix phase of step t - 1 and left in step t's, half a step later by the later waves: it is sent for in step t - LEAD
 // into the buffer of tile t - BUFS.
 template <int D> struct Sweep {
     static constexpr bool PAIRED = D < 128;
-    static constexpr int NW = PAIRED ? 8 : 4, ROWS = 32, TILE = ROWS * D * 8, BUFS = PAIRED ? 5 : 3, LEAD = PAIRED ? 3 : 2, OWN = NW * 32;
+    static constexpr int NW = PAIRED ? 8 : 4, ROWS = 32, TILE = ROWS * D * 8, BUFS = PAIRED ? 5 : 4, LEAD = PAIRED ? 3 : 2, OWN = NW * 32;
     static __device__ __forceinline__ void fall_behind(int wave) { if (PAIRED && wave >= NW / 2) __syncthreads(); }
     static __device__ __forceinline__ void wait_for_late(int wave) { if (PAIRED && wave < NW / 2) __syncthreads(); }
     static __device__ __forceinline__ int next(int buf) { return buf == BUFS - 1 ? 0 : buf + 1; }
@@ -934,7 +935,7 @@ __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void d
         buf = S::next(buf);
         scores_dp<D, F16, ROWS>(fl.at(buf * TILE), qf, gf, s, dp);
         __builtin_amdgcn_s_setprio(0);
-        __syncthreads();
+        if (S::PAIRED) __syncthreads();
     }
     S::wait_for_late(wave);
     if (query >= a.Nq) return;
@@ -1134,7 +1135,7 @@ __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void d
         }
         next_scores(buf);
         __builtin_amdgcn_s_setprio(0);
-        __syncthreads();
+        if (S::PAIRED) __syncthreads();
     }
     S::wait_for_late(wave);
     if (CUT) {                                                            // [part][32 keys][32 columns][a lane's 4 at a time], for diff_dkv_join_kernel
