@@ -31,12 +31,12 @@ struct Args {
     const int *q_start, *kv_len;
     bf16_t *o, *maps;
     float* lse;                                // [B][H][hi of both maps, lo of both][Nq] (put_lse); hi = +inf: no visible key
-    f32x4* sums;                               // backward: parts of dk and dv
+    f32x4 *sums, *stats;                       // parts of the forward pass with their rows' (reference, sums); of dk and dv; of dq
     float *D, *x2, *rc;                        // backward: D_m [B][H][2][Nq], D_2 in full precision [B][H][Nq], constants of the rows (diff_rows_kernel)
     bf16_t *dq, *dk, *dv;
     float* part;                               // split forward: numerators, then (maximum, sum)
     long q_b, q_n, q_h, k_b, k_n, k_h, v_b, v_n, v_h, go_b, go_n, go_h;
-    int B, Nq, Nk, H, Hkv, G, causal, q_start0, lam_stride, nsplit, chunk, tiles, parts;
+    int B, Nq, Nk, H, Hkv, G, causal, q_start0, lam_stride, nsplit, chunk, tiles, parts, cuts;
     float c2, scale;                           // scale * log2(e), scale
 };
 
@@ -361,7 +361,8 @@ template <int D> struct Sweep {
 // 12 d operations a visible pair and head, both maps' products with V apart.  Bound: the matrix and vector instructions together (53 and 42 % of a SIMD's
 // cycles, at a clock that the power cap holds at 2.2 GHz).  16 heads of 64 on 4, 8192 causal tokens: 355 us, 1.16 PFLOP/s.  2 x 4097 tokens of 6 heads: 168 us,
 // 183 with the maps kept; its 204 blocks leave 52 of the 256 CUs idle.
-template <int D, bool F16, bool KEEP>
+// CUT: a block takes one of a.cuts parts of its keys, and diff_fwd_join_kernel puts them together.
+template <int D, bool F16, bool KEEP, bool CUT>
 __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void diff_fwd_kernel(Args a) {
     typedef Sweep<D> S;
     static_assert(S::PAIRED, "d = 128: diff_fwd_wide_kernel");
@@ -373,19 +374,21 @@ __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void d
     int id = block_order();
     const int blk = nblk - 1 - id % nblk;                                 // under a causal mask the last queries have most to do: first
     id /= nblk;
-    const int head = id % a.H, b = id / a.H, kvh = head / a.G;
+    const int head = id % a.H;
+    id /= a.H;
+    const int b = CUT ? id % a.B : id, part = CUT ? id / a.B : 0, kvh = head / a.G;
     const int len = key_count(a, b), start = first_pos(a, b);
     const int q0 = blk * (NW * 32) + wave * 32, query = q0 + c;
     const int kend = visible(a, len, start, min(blk * (NW * 32) + NW * 32, a.Nq) - 1);
-    const int lim = visible(a, len, start, query), lim_lo = visible(a, len, start, q0);
-    const int nj = (kend + ROWS - 1) / ROWS;
+    const int all = (kend + ROWS - 1) / ROWS, j0 = CUT ? all * part / a.cuts : 0, nj = CUT ? all * (part + 1) / a.cuts - j0 : all;     // tiles of 32 keys
+    const int lim = visible(a, len, start, query) - j0 * ROWS, lim_lo = visible(a, len, start, q0) - j0 * ROWS;
 
     Lane fl;
     fl.init(smem, lane);
     const unsigned lds0 = lds_addr(smem);
     Dma<D, 2 * D, ROWS, NW> dma;
     const bf16_t *kp = a.k + b * a.k_b + 2 * kvh * a.k_h, *vp = a.v + b * a.v_b + kvh * a.v_h;
-    dma.init(wave, lane, kp, a.k_n, a.k_h, vp, a.v_n, 0, len);
+    dma.init(wave, lane, kp, a.k_n, a.k_h, vp, a.v_n, j0 * ROWS, len);
     for (int t = 0; t < min(S::LEAD, nj); ++t) { dma.issue(lds0 + t * TILE); dma.skip(ROWS); }
     bf16x8 qf[2][D / 16];
     {
@@ -403,7 +406,7 @@ __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void d
     // range (fp16: 2^15, P itself; bf16: 2^40, which leaves 2^87 for the values), the block starts again and keeps a running maximum.
     for (bool running = false;; running = true) {
         if (running) {
-            dma.start(kp, vp, 0, len);
+            dma.start(kp, vp, j0 * ROWS, len);
             for (int t = 0; t < min(S::LEAD, nj); ++t) { dma.issue(lds0 + t * TILE); dma.skip(ROWS); }
         }
         m[0] = m[1] = NONE;
@@ -441,13 +444,27 @@ __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void d
         constexpr float MOST = F16 ? 32768.f : 1.0995116e12f;
         if (running || !__syncthreads_or(!(l[0][0] < MOST && l[1][0] < MOST))) break;
     }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int k = 0; k < SUMS; ++k) l[i][k] += __shfl_xor(l[i][k], 32, 64);
+    if (CUT) {                                                            // [part][32 rows][map, 32 columns][a lane's 4 at a time]; (reference, sums) a row and map
+        const long tile = (((long)part * a.B + b) * a.H + head) * nblk * NW + blk * NW + wave;
+        f32x4* to = a.sums + tile * (2 * NB * 256) + lane;
+#pragma unroll
+        for (int n = 0; n < 2 * NB; ++n) {
+            const f32x16& x = n < NB ? o1[n % NB] : o2[n % NB];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) to[n * 256 + i * 64] = f32x4{x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]};
+        }
+        a.stats[tile * 64 + lane] = f32x4{h ? m[1] : m[0], h ? l[1][0] : l[0][0], h ? l[1][SUMS - 1] : l[0][SUMS - 1], 0.f};
+        return;
+    }
     if (query >= a.Nq) return;
     const float lam = a.lam[head * a.lam_stride];
     float inv[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-#pragma unroll
-        for (int k = 0; k < SUMS; ++k) l[i][k] += __shfl_xor(l[i][k], 32, 64);
         inv[i] = l[i][0] > 0.f ? 1.0f / l[i][0] : l[i][0] == 0.f ? 0.f : l[i][0];      // (a NaN stays one)
     }
     const long row = ((long)b * a.Nq + query) * a.H + head, at = row * 2 * D;
@@ -466,6 +483,50 @@ __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void d
 #pragma unroll
         for (int r = 0; r < 16; ++r) o1[db][r] = __builtin_fmaf(-w2, o2[db][r], o1[db][r] * inv[0]);
     store_rows<F16>(a.o + at, o1, 1.0f, h);
+}
+
+// the parts of a forward pass put together: a wave 32 rows by 32 columns of both maps
+template <int D, bool F16, bool KEEP>
+__global__ __launch_bounds__(256) void diff_fwd_join_kernel(Args a) {
+    constexpr int NB = D / 16, NW = Sweep<D>::NW;
+    const int lane = threadIdx.x & 63, h = lane >> 5, c = lane & 31, nq = (a.Nq + Sweep<D>::OWN - 1) / Sweep<D>::OWN * NW;
+    const long piece = (long)blockIdx.x * 4 + (threadIdx.x >> 6), tile = piece / NB, tiles = (long)a.B * a.H * nq;
+    if (tile >= tiles) return;
+    const int db = piece % NB, query = (int)(tile % nq) * 32 + c, head = tile / nq % a.H;
+    const long b = tile / nq / a.H;
+    if (query >= a.Nq) return;
+    float M[2] = {NONE, NONE}, l[2] = {0.f, 0.f}, whole[2] = {0.f, 0.f};
+    for (int p = 0; p < a.cuts; ++p)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) M[i] = fmaxf(M[i], a.stats[(p * tiles + tile) * 64 + i * 32 + c][0]);
+    f32x16 x[2][1] = {{zero16()}, {zero16()}};
+    for (int p = 0; p < a.cuts; ++p)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const f32x4 st = a.stats[(p * tiles + tile) * 64 + i * 32 + c];
+            const float w = __builtin_amdgcn_exp2f(st[0] - M[i]);
+            l[i] += w * st[1];
+            whole[i] += w * st[2];
+            const f32x4* from = a.sums + ((p * tiles + tile) * 2 + i) * (NB * 256) + db * 256 + lane;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 t = from[g * 64];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[i][0][4 * g + e] += w * t[e];
+            }
+        }
+    const long at = ((b * a.Nq + query) * a.H + head) * 2 * D + db * 32;
+    float inv[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        inv[i] = l[i] > 0.f ? 1.0f / l[i] : l[i] == 0.f ? 0.f : l[i];      // (a NaN stays one)
+        if (KEEP) store_rows<F16>(a.maps + i * (long)a.B * a.Nq * a.H * 2 * D + at, x[i], inv[i], h);
+        if (KEEP && db == 0 && h == i) put_lse(a.lse + ((b * a.H + head) * 4 + i) * a.Nq + query, 2 * a.Nq, M[i], whole[i]);
+    }
+    const float w2 = a.lam[head * a.lam_stride] * inv[1];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[0][0][r] = __builtin_fmaf(-w2, x[1][0][r], x[0][0][r] * inv[0]);
+    store_rows<F16>(a.o + at, x[0], 1.0f, h);
 }
 
 // one map's scores at d = 128
@@ -1232,44 +1293,54 @@ bool misaligned(const void* p, unsigned n = 16) { return !p || (uintptr_t)p % n;
 
 struct Split { int tiles, nsplit, chunk; };
 constexpr int SPARSE = 128, WANT = 1024, LEAST = 512;       // blocks (two rounds even out ragged entries: 70 us against 78 with one); keys of a chunk (4 tiles a wave)
-// Whether the split forward runs, and how it cuts the keys.  The whole forward needs the time of one block over all keys for each round of its blocks on
-// the 256 CUs, full or not; the split forward's time goes with its tiles, wherever they come from.  Measured with 16 query heads on 4 key heads of 64, 8192
-// keys, whole / split in us: 1 entry, 16 queries 256 / 18, 256 queries 261 / 79; 16 entries, 16 queries 343 / 116, 32 (512 tiles) 328 / 205, 64 (1024 tiles)
+// Parts that a sweep is cut into.  A round of blocks (one a CU) takes about a microsecond a tile of 32 rows; cutting costs each block another start, a second
+// kernel, and `traffic` tiles' time for a part's sums of a block written and read.
+struct Cuts { int parts; double time; };
+Cuts cuts_of(int64_t blocks, double tiles, double start, double traffic) {
+    Cuts best = {1, 0};
+    for (int p = 1; p <= 16; ++p) {
+        const double time = (double)((blocks * p + 255) / 256) * (tiles / p + start) + (p > 1 ? 6 + traffic * (double)blocks * p : 0);
+        if (p == 1 || time < best.time) best = {p, time};
+    }
+    return best;
+}
+int own_of(const hs_diff_attn_desc* d) { return d->d == 128 ? Sweep<128>::OWN : Sweep<64>::OWN; }
+int64_t blocks_of(const hs_diff_attn_desc* d) { return (int64_t)d->B * d->H * ((d->Nq + own_of(d) - 1) / own_of(d)); }
+// the whole forward pass (at d = 128 not cut, and two sweeps)
+Cuts whole_of(const hs_diff_attn_desc* d) {
+    const double tiles = (double)((d->Nk + 31) / 32);
+    if (d->d == 128) return {1, (double)((blocks_of(d) + 255) / 256) * (2 * tiles + 4)};
+    return cuts_of(blocks_of(d), tiles, 3, 0.09 * d->d / 64);
+}
+// Whether the split forward runs, and how it cuts the keys.  The whole forward needs the time of one block over all (its part of the) keys for each round of
+// blocks on the 256 CUs, full or not; the split forward's time goes with its tiles, wherever they come from.  Measured with 16 query heads on 4 key heads of
+// 64, 8192 keys, whole (not cut) / split in us: 1 entry, 16 queries 256 / 18; 16 entries, 16 queries 343 / 116, 32 (512 tiles) 328 / 205, 64 (1024 tiles)
 // 317 / 352, 128 334 / 488.  8 on 2 of 128, 16 entries, 512 / 2048 keys: 32 queries (256 tiles) 36, 116 / 27, 74, 64 (512 tiles) 37, 117 / 36, 107.
 Split split_of(const hs_diff_attn_desc* d) {
     const int64_t rows = (int64_t)(d->H / d->Hkv) * d->Nq, tiles = (rows + 15) / 16, blocks = (int64_t)d->B * d->Hkv * tiles;
-    const int own = d->d == 128 ? Sweep<128>::OWN : Sweep<64>::OWN;
-    const int64_t rounds = ((int64_t)d->B * d->H * ((d->Nq + own - 1) / own) + 255) / 256;
-    if (blocks > rounds * 512) return {0, 0, 0};
+    if (8 + 0.0011 * (double)blocks * (double)((d->Nk + 31) / 32) > whole_of(d).time) return {0, 0, 0};
     const int64_t want = std::min<int64_t>((WANT + blocks - 1) / blocks, MOST_CHUNKS);
     // (a grid that leaves most CUs idle anyway takes half as long chunks, unless one would do without the join: 1 entry, 2000 keys 12 -> 11 us)
     const int64_t least = d->Nk > LEAST && blocks * ((d->Nk + LEAST - 1) / LEAST) <= SPARSE ? LEAST / 2 : LEAST;
     const int64_t chunk = std::max<int64_t>(((d->Nk + want - 1) / want + 127) / 128 * 128, least);
     return {(int)tiles, (int)((d->Nk + chunk - 1) / chunk), (int)chunk};
 }
-size_t split_bytes(const hs_diff_attn_desc* d, const Split& s) {
+// bytes of the parts' sums of a forward pass, and of all that it needs
+size_t cut_bytes(const hs_diff_attn_desc* d, int cuts) { return cuts > 1 ? (size_t)cuts * blocks_of(d) * own_of(d) * (size_t)d->d * 16 : 0; }
+size_t forward_bytes(const hs_diff_attn_desc* d, const Split& s, int cuts) {
     const size_t rows = std::min<int64_t>(16, (int64_t)(d->H / d->Hkv) * d->Nq);
+    if (!s.nsplit) return cuts > 1 ? cut_bytes(d, cuts) + (size_t)cuts * blocks_of(d) * own_of(d) * 32 : 0;
     return s.nsplit > 1 ? (size_t)d->B * d->Hkv * s.tiles * s.nsplit * 2 * rows * (2 * d->d + 2) * 4 : 0;
 }
-// Parts that the dk, dv sweep's list of tiles is cut into.  A round of blocks (one a CU) takes 1.4 us a tile; cutting costs each block another start (4
-// tiles' time), a second kernel, and 0.1 us for a part's sums of a block written and read: blocks over so few keys or so long lists that a cut pays.
-// Backward pass whole / cut in us: 8192 causal tokens, 16 heads of 64 on 1: 5904 / 1216, on 4: 1850 / 1225; 4 x 512 tokens, 12 on 4: 130 / 107; 2 x 4097
-// tokens, 6 on 6 (204 blocks): not cut.
+// Parts that the dk, dv sweep's list of tiles is cut into.  Backward pass whole / cut in us: 8192 causal tokens, 16 heads of 64 on 1: 5904 / 1216, on 4:
+// 1850 / 1225; 4 x 512 tokens, 12 on 4: 130 / 107; 2 x 4097 tokens, 6 on 6 (204 blocks): not cut.
 int parts_of(const hs_diff_attn_desc* d) {
-    const int64_t own = d->d == 128 ? Sweep<128>::OWN : Sweep<64>::OWN, blocks = (int64_t)d->B * d->Hkv * ((d->Nk + own - 1) / own);
-    const double tiles = (double)(d->H / d->Hkv) * ((d->Nq + 31) / 32);
-    int best = 1;
-    double least = 0;
-    for (int p = 1; p <= 16; ++p) {
-        const double time = (double)((blocks * p + 255) / 256) * (tiles / p + 4) + (p > 1 ? 6 + 0.07 * (double)blocks * p : 0);
-        if (p == 1 || time < least) { best = p; least = time; }
-    }
-    return best;
+    return cuts_of((int64_t)d->B * d->Hkv * ((d->Nk + own_of(d) - 1) / own_of(d)), (double)(d->H / d->Hkv) * ((d->Nq + 31) / 32), 4, 0.07).parts;
 }
 size_t rows_bytes(const hs_diff_attn_desc* d) { return (size_t)d->B * d->H * (d->Nq * 12 + (size_t)((d->Nq + 31) / 32) * 512); }
 size_t sums_at(const hs_diff_attn_desc* d) { return (rows_bytes(d) + 255) / 256 * 256; }
 size_t backward_bytes(const hs_diff_attn_desc* d) {
-    const size_t own = d->d == 128 ? Sweep<128>::OWN : Sweep<64>::OWN, p = parts_of(d);
+    const size_t own = own_of(d), p = parts_of(d);
     return p == 1 ? rows_bytes(d) : sums_at(d) + p * d->B * d->Hkv * ((d->Nk + own - 1) / own) * own * d->d * 16;
 }
 Args args_of(const hs_diff_attn_desc* d) {
@@ -1295,7 +1366,11 @@ template <int D, bool F16, bool KEEP> void forward(const Args& a, const Split& s
     }
     const int64_t blocks = (int64_t)a.B * a.H * ((a.Nq + S::OWN - 1) / S::OWN);
     if constexpr (D == 128) launch(diff_fwd_wide_kernel<F16, KEEP>, blocks, Wide::NW * 64, (size_t)Wide::BUFS * Wide::TILE, s, a);
-    else launch(diff_fwd_kernel<D, F16, KEEP>, blocks, S::NW * 64, (size_t)S::BUFS * S::TILE, s, a);
+    else if (a.cuts == 1) launch(diff_fwd_kernel<D, F16, KEEP, false>, blocks, S::NW * 64, (size_t)S::BUFS * S::TILE, s, a);
+    else {
+        launch(diff_fwd_kernel<D, F16, KEEP, true>, blocks * a.cuts, S::NW * 64, (size_t)S::BUFS * S::TILE, s, a);
+        launch(diff_fwd_join_kernel<D, F16, KEEP>, blocks * S::NW * (D / 16) / 4, 256, 0, s, a);
+    }
 }
 template <int D, bool F16> void backward(const Args& a, hipStream_t s) {
     typedef Sweep<D> S;
@@ -1318,7 +1393,7 @@ template <int D, bool F16> void backward(const Args& a, hipStream_t s) {
 
 }  // namespace
 
-extern "C" size_t hs_diff_attn_fwd_ws_bytes(const hs_diff_attn_desc* d) { return check(d, false) == HS_OK ? split_bytes(d, split_of(d)) : 0; }
+extern "C" size_t hs_diff_attn_fwd_ws_bytes(const hs_diff_attn_desc* d) { return check(d, false) == HS_OK ? forward_bytes(d, split_of(d), whole_of(d).parts) : 0; }
 extern "C" size_t hs_diff_attn_bwd_ws_bytes(const hs_diff_attn_desc* d) { return check(d, false) == HS_OK ? backward_bytes(d) : 0; }
 
 extern "C" int hs_diff_attn_fwd(const hs_diff_attn_desc* d, const void* q, const void* k, const void* v, const float* lam, const int32_t* q_start,
@@ -1328,12 +1403,14 @@ extern "C" int hs_diff_attn_fwd(const hs_diff_attn_desc* d, const void* q, const
     if (!q || !k || !v || !o || !lam || !maps != !lse) return HS_ERR_ARG;
     if (misaligned(q) || misaligned(k) || misaligned(v) || misaligned(o) || (maps && misaligned(maps))) return HS_ERR_SHAPE;
     const Split sp = split_of(d);
-    const size_t need = split_bytes(d, sp);
+    const int cuts = whole_of(d).parts;
+    const size_t need = forward_bytes(d, sp, cuts);
     if (need && (misaligned(ws) || ws_bytes < need)) return HS_ERR_SHAPE;
     Args a = args_of(d);
     a.q = (const bf16_t*)q; a.k = (const bf16_t*)k; a.v = (const bf16_t*)v; a.lam = lam; a.q_start = q_start; a.kv_len = kv_len;
     a.o = (bf16_t*)o; a.maps = (bf16_t*)maps; a.lse = lse; a.part = (float*)ws;
     a.tiles = sp.tiles; a.nsplit = sp.nsplit; a.chunk = sp.chunk;
+    a.cuts = cuts; a.sums = (f32x4*)ws; a.stats = (f32x4*)((char*)ws + cut_bytes(d, cuts));
     hipStream_t s = (hipStream_t)stream;
 #define CALL(D, F) maps ? forward<D, F, true>(a, sp, s) : forward<D, F, false>(a, sp, s)
     HS_BY_TYPE(CALL);
