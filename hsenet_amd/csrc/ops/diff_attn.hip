@@ -906,7 +906,7 @@ __global__ __launch_bounds__(256) void diff_rows_kernel(Args a) {
 }
 
 // dQ: queries stay, keys stream.  Bound as the forward pass is; 2 x 4097 tokens of 6 heads of 64: 186 us, 155 GFLOP, 0.83 PFLOP/s on 204 of the 256 CUs.
-template <int D, bool F16>
+template <int D, bool F16, bool CUT>
 __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void diff_dq_kernel(Args a) {
     typedef Sweep<D> S;
     constexpr int ROWS = S::ROWS, TILE = S::TILE, NW = S::NW, NQ = D / 32;
@@ -917,18 +917,20 @@ __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void d
     int id = block_order();
     const int blk = nblk - 1 - id % nblk;
     id /= nblk;
-    const int head = id % a.H, b = id / a.H, kvh = head / a.G;
+    const int head = id % a.H;
+    id /= a.H;
+    const int b = CUT ? id % a.B : id, part = CUT ? id / a.B : 0, kvh = head / a.G;
     const int len = key_count(a, b), start = first_pos(a, b);
     const int q0 = blk * (NW * 32) + wave * 32, query = q0 + c, qrow = min(query, a.Nq - 1);
     const int kend = visible(a, len, start, min(blk * (NW * 32) + NW * 32, a.Nq) - 1);
-    const int lim = visible(a, len, start, query), lim_lo = visible(a, len, start, q0);
-    const int nj = (kend + ROWS - 1) / ROWS;
+    const int all = (kend + ROWS - 1) / ROWS, j0 = CUT ? all * part / a.cuts : 0, nj = CUT ? all * (part + 1) / a.cuts - j0 : all;     // tiles of 32 keys
+    const int lim = visible(a, len, start, query) - j0 * ROWS, lim_lo = visible(a, len, start, q0) - j0 * ROWS;
 
     Lane fl;
     fl.init(smem, lane);
     const unsigned lds0 = lds_addr(smem);
     Dma<D, 2 * D, ROWS, NW> dma;
-    dma.init(wave, lane, a.k + b * a.k_b + 2 * kvh * a.k_h, a.k_n, a.k_h, a.v + b * a.v_b + kvh * a.v_h, a.v_n, 0, len);
+    dma.init(wave, lane, a.k + b * a.k_b + 2 * kvh * a.k_h, a.k_n, a.k_h, a.v + b * a.v_b + kvh * a.v_h, a.v_n, j0 * ROWS, len);
     for (int t = 0; t < min(S::LEAD, nj); ++t) { dma.issue(lds0 + t * TILE); dma.skip(ROWS); }
     bf16x8 qf[2][D / 16], gf[D / 8];
     {
@@ -999,15 +1001,57 @@ __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void d
         if (S::PAIRED) __syncthreads();
     }
     S::wait_for_late(wave);
+    x2 += __shfl_xor(x2, 32, 64);
+    if (CUT) {                                                            // [part][32 rows][32 columns][a lane's 4 at a time]; [part][row]
+        const long tile = (((long)part * a.B + b) * a.H + head) * nblk * NW + blk * NW + wave;
+        f32x4* to = a.sums + tile * (2 * NQ * 256) + lane;
+#pragma unroll
+        for (int n = 0; n < 2 * NQ; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const f32x16& x = dq[n / NQ][n % NQ];
+                to[n * 256 + i * 64] = f32x4{x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]};
+            }
+        if (h == 0) ((float*)a.stats)[tile * 32 + c] = x2;
+        return;
+    }
     if (query >= a.Nq) return;
     const float down = F16 ? 1.0f / (1 << SHIFT16) : 1.0f, mul = a.scale * down;
     const float un0 = __builtin_amdgcn_exp2f(-ls[2 * a.Nq]), un1 = __builtin_amdgcn_exp2f(-ls[3 * a.Nq]);
-    x2 += __shfl_xor(x2, 32, 64);
     // D_2 = sum P2 dP = D_1' + sum P2 (dP - D_1'), whatever D_1' is that stands for it in the row's dS (sum P2 = 1)
     if (h == 0) a.x2[bh * a.Nq + query] = x2 * down * un1 + D1;
     bf16_t* p = a.dq + (((long)b * a.Nq + query) * a.H + head) * 2 * D;
     store_rows<F16>(p, dq[0], mul * un0, h);
     store_rows<F16>(p + D, dq[1], -a.lam[head * a.lam_stride] * mul * un1, h);
+}
+
+// the sum of dq's parts, in their order: a wave 32 rows by 32 columns of [dq1 | dq2]
+template <int D, bool F16>
+__global__ __launch_bounds__(256) void diff_dq_join_kernel(Args a) {
+    constexpr int NQ = D / 32, PER = 2 * NQ, NW = Sweep<D>::NW;
+    const int lane = threadIdx.x & 63, h = lane >> 5, c = lane & 31, nq = (a.Nq + Sweep<D>::OWN - 1) / Sweep<D>::OWN * NW;
+    const long piece = (long)blockIdx.x * 4 + (threadIdx.x >> 6), tile = piece / PER, tiles = (long)a.B * a.H * nq;
+    if (tile >= tiles) return;
+    const int n = piece % PER, query = (int)(tile % nq) * 32 + c, head = tile / nq % a.H;
+    const long b = tile / nq / a.H, bh = b * a.H + head;
+    if (query >= a.Nq) return;
+    f32x16 x[1] = {zero16()};
+    float x2 = 0.f;
+    for (int p = 0; p < a.cuts; ++p) {
+        const f32x4* from = a.sums + ((p * tiles + tile) * PER + n) * 256 + lane;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const f32x4 t = from[i * 64];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[0][4 * i + e] += t[e];
+        }
+        x2 += ((const float*)a.stats)[(p * tiles + tile) * 32 + c];
+    }
+    const float down = F16 ? 1.0f / (1 << SHIFT16) : 1.0f, mul = a.scale * down;
+    const float* ls = a.lse + bh * 4 * a.Nq + query;
+    const float un0 = __builtin_amdgcn_exp2f(-ls[2 * a.Nq]), un1 = __builtin_amdgcn_exp2f(-ls[3 * a.Nq]);
+    if (n == 0 && h == 0) a.x2[bh * a.Nq + query] = x2 * down * un1 + a.D[(bh * 2 + 1) * a.Nq + query];
+    store_rows<F16>(a.dq + ((b * a.Nq + query) * a.H + head) * 2 * D + n * 32, x, n < NQ ? mul * un0 : -a.lam[head * a.lam_stride] * mul * un1, h);
 }
 
 // dK, dV: keys stay, the queries of every head of the group stream.  With the constants of a row (row_constants)
@@ -1294,7 +1338,9 @@ bool misaligned(const void* p, unsigned n = 16) { return !p || (uintptr_t)p % n;
 struct Split { int tiles, nsplit, chunk; };
 constexpr int SPARSE = 128, WANT = 1024, LEAST = 512;       // blocks (two rounds even out ragged entries: 70 us against 78 with one); keys of a chunk (4 tiles a wave)
 // Parts that a sweep is cut into.  A round of blocks (one a CU) takes about a microsecond a tile of 32 rows; cutting costs each block another start, a second
-// kernel, and `traffic` tiles' time for a part's sums of a block written and read.
+// kernel, and `traffic` tiles' time for a part's sums of a block written and read.  Whole / cut in us: forward, 4096 tokens of 4 heads of 64 136 / 74, causal
+// 137 / 64; 2048 causal tokens of 8 heads 72 / 46; 512 queries of 16 heads on 8192 keys 135 / 75; the backward pass with dq cut, the same four but the last:
+// 253 / 172, 242 / 159, 145 / 107.
 struct Cuts { int parts; double time; };
 Cuts cuts_of(int64_t blocks, double tiles, double start, double traffic) {
     Cuts best = {1, 0};
@@ -1338,10 +1384,15 @@ int parts_of(const hs_diff_attn_desc* d) {
     return cuts_of((int64_t)d->B * d->Hkv * ((d->Nk + own_of(d) - 1) / own_of(d)), (double)(d->H / d->Hkv) * ((d->Nq + 31) / 32), 4, 0.07).parts;
 }
 size_t rows_bytes(const hs_diff_attn_desc* d) { return (size_t)d->B * d->H * (d->Nq * 12 + (size_t)((d->Nq + 31) / 32) * 512); }
+// parts of the dq sweep's keys (see cuts_of)
+int cuts_of_dq(const hs_diff_attn_desc* d) { return cuts_of(blocks_of(d), (double)((d->Nk + 31) / 32), 4, 0.045 * d->d / 64).parts; }
+// Behind the rows' numbers lie dq's parts (sums, then a number a row), and, when these have been put together, those of dk and dv.
 size_t sums_at(const hs_diff_attn_desc* d) { return (rows_bytes(d) + 255) / 256 * 256; }
+size_t dq_bytes(const hs_diff_attn_desc* d, int cuts) { return cuts > 1 ? (size_t)cuts * blocks_of(d) * own_of(d) * (size_t)d->d * 8 : 0; }
 size_t backward_bytes(const hs_diff_attn_desc* d) {
-    const size_t own = own_of(d), p = parts_of(d);
-    return p == 1 ? rows_bytes(d) : sums_at(d) + p * d->B * d->Hkv * ((d->Nk + own - 1) / own) * own * d->d * 16;
+    const size_t own = own_of(d), p = parts_of(d), c = cuts_of_dq(d);
+    const size_t kv = p > 1 ? p * d->B * d->Hkv * ((d->Nk + own - 1) / own) * own * d->d * 16 : 0, q = c > 1 ? dq_bytes(d, c) + c * blocks_of(d) * own * 4 : 0;
+    return kv || q ? sums_at(d) + std::max(kv, q) : rows_bytes(d);
 }
 Args args_of(const hs_diff_attn_desc* d) {
     Args a = {};
@@ -1376,7 +1427,12 @@ template <int D, bool F16> void backward(const Args& a, hipStream_t s) {
     typedef Sweep<D> S;
     constexpr int LANES = D / 4;
     launch(diff_rows_kernel<D, F16>, ((int64_t)a.B * ((a.Nq + 31) / 32 * 32) * a.H * LANES + 255) / 256, 256, 0, s, a);
-    launch(diff_dq_kernel<D, F16>, (int64_t)a.B * a.H * ((a.Nq + S::OWN - 1) / S::OWN), S::NW * 64, (size_t)S::BUFS * S::TILE, s, a);
+    const int64_t rows = (int64_t)a.B * a.H * ((a.Nq + S::OWN - 1) / S::OWN);
+    if (a.cuts == 1) launch(diff_dq_kernel<D, F16, false>, rows, S::NW * 64, (size_t)S::BUFS * S::TILE, s, a);
+    else {
+        launch(diff_dq_kernel<D, F16, true>, rows * a.cuts, S::NW * 64, (size_t)S::BUFS * S::TILE, s, a);
+        launch(diff_dq_join_kernel<D, F16>, rows * S::NW * (D / 16) / 4, 256, 0, s, a);
+    }
     const int64_t blocks = (int64_t)a.B * a.Hkv * ((a.Nk + S::OWN - 1) / S::OWN);
     const size_t lds = (size_t)S::BUFS * (S::TILE + 512) + (D == 64 ? S::OWN * D * 4 : 0);
     if (a.parts == 1) return launch(diff_dkv_kernel<D, F16, false>, blocks, S::NW * 64, lds, s, a);
@@ -1433,7 +1489,8 @@ extern "C" int hs_diff_attn_bwd(const hs_diff_attn_desc* d, const void* q, const
     a.q_start = q_start; a.kv_len = kv_len; a.maps = (bf16_t*)maps; a.lse = (float*)lse;
     a.D = (float*)ws; a.x2 = a.D + (size_t)d->B * d->H * 2 * d->Nq;
     a.rc = a.x2 + (size_t)d->B * d->H * d->Nq;
-    a.parts = parts_of(d); a.sums = (f32x4*)((char*)ws + sums_at(d));
+    a.parts = parts_of(d); a.cuts = cuts_of_dq(d);
+    a.sums = (f32x4*)((char*)ws + sums_at(d)); a.stats = (f32x4*)((char*)a.sums + dq_bytes(d, a.cuts));
     a.dq = (bf16_t*)dq; a.dk = (bf16_t*)dk; a.dv = (bf16_t*)dv;
     hipStream_t s = (hipStream_t)stream;
 #define CALL(D, F) backward<D, F>(a, s)

@@ -243,7 +243,8 @@ def test_diff_attention_of_many_rows(dev, case):
 @pytest.mark.parametrize("case", [                             # many rows of few heads: the whole forward's keys come in parts
     dict(B=1, Nq=600, Nk=2000, Hq=16, Hkv=16, d=64, dtype=BF, causal=True), dict(B=2, Nq=520, Nk=2047, Hq=8, Hkv=4, d=64, dtype=F16, grow=36.0),
     dict(B=2, Nq=600, Nk=1500, Hq=10, Hkv=10, d=32, dtype=BF, lens=[33, 1499], lam="one"), dict(B=1, Nq=1300, Nk=1300, Hq=8, Hkv=8, d=64, dtype=BF, causal=True),
-    dict(B=3, Nq=700, Nk=1100, Hq=6, Hkv=6, d=32, dtype=F16, causal=True, lens=[0, 1100, 64], start=[0, -650, 30])],
+    dict(B=3, Nq=700, Nk=1100, Hq=6, Hkv=6, d=32, dtype=F16, causal=True, lens=[0, 1100, 64], start=[0, -650, 30]),
+    dict(B=1, Nq=300, Nk=1500, Hq=4, Hkv=2, d=128, dtype=F16, causal=True), dict(B=2, Nq=70, Nk=1000, Hq=2, Hkv=2, d=128, dtype=BF, lens=[1000, 40])],
     ids=lambda c: f"{c['B']}x{c['Nq']}x{c['Nk']}-{c['Hq']}/{c['Hkv']}x{c['d']}")
 def test_diff_attention_of_few_heads(dev, case):
     test_diff_attention_values_and_gradients(dev, case)
