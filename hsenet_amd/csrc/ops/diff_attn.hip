@@ -1352,11 +1352,11 @@ Cuts cuts_of(int64_t blocks, double tiles, double start, double traffic) {
 }
 int own_of(const hs_diff_attn_desc* d) { return d->d == 128 ? Sweep<128>::OWN : Sweep<64>::OWN; }
 int64_t blocks_of(const hs_diff_attn_desc* d) { return (int64_t)d->B * d->H * ((d->Nq + own_of(d) - 1) / own_of(d)); }
-// the whole forward pass (at d = 128 not cut, and two sweeps)
+// the whole forward pass, in us: at d = 32, 64 and 128 0.8, 1.06 and twice 0.92 a tile (at d = 128 not cut)
 Cuts whole_of(const hs_diff_attn_desc* d) {
-    const double tiles = (double)((d->Nk + 31) / 32);
-    if (d->d == 128) return {1, (double)((blocks_of(d) + 255) / 256) * (2 * tiles + 4)};
-    return cuts_of(blocks_of(d), tiles, 3, 0.09 * d->d / 64);
+    const double time = (double)((d->Nk + 31) / 32) * (d->d == 32 ? 0.8 : d->d == 64 ? 1.06 : 1.84);
+    if (d->d == 128) return {1, (double)((blocks_of(d) + 255) / 256) * (time + 4)};
+    return cuts_of(blocks_of(d), time, 3, 0.09 * d->d / 64);
 }
 // Whether the split forward runs, and how it cuts the keys.  The whole forward needs the time of one block over all (its part of the) keys for each round of
 // blocks on the 256 CUs, full or not; the split forward's time goes with its tiles, wherever they come from.  Measured with 16 query heads on 4 key heads of
@@ -1364,7 +1364,8 @@ Cuts whole_of(const hs_diff_attn_desc* d) {
 // 317 / 352, 128 334 / 488.  8 on 2 of 128, 16 entries, 512 / 2048 keys: 32 queries (256 tiles) 36, 116 / 27, 74, 64 (512 tiles) 37, 117 / 36, 107.
 Split split_of(const hs_diff_attn_desc* d) {
     const int64_t rows = (int64_t)(d->H / d->Hkv) * d->Nq, tiles = (rows + 15) / 16, blocks = (int64_t)d->B * d->Hkv * tiles;
-    if (8 + 0.0011 * (double)blocks * (double)((d->Nk + 31) / 32) > whole_of(d).time) return {0, 0, 0};
+    const double time = (d->d == 128 ? 0.0019 : 0.00135) * (double)blocks * (double)((d->Nk + 31) / 32);      // us beside 8 of start and join
+    if (time > 4 && time + 8 > whole_of(d).time) return {0, 0, 0};          // (small calls take launches either way, and the split forward rounds less)
     const int64_t want = std::min<int64_t>((WANT + blocks - 1) / blocks, MOST_CHUNKS);
     // (a grid that leaves most CUs idle anyway takes half as long chunks, unless one would do without the join: 1 entry, 2000 keys 12 -> 11 us)
     const int64_t least = d->Nk > LEAST && blocks * ((d->Nk + LEAST - 1) / LEAST) <= SPARSE ? LEAST / 2 : LEAST;

@@ -234,7 +234,12 @@ def test_diff_attention_values_and_gradients(dev, case):
     dict(B=70, Nq=70, Nk=31, Hq=2, Hkv=2, d=64, dtype=F16, scale=0.3), dict(B=2, Nq=130, Nk=300, Hq=32, Hkv=32, d=128, dtype=BF, causal=True),
     dict(B=6, Nq=40, Nk=200, Hq=32, Hkv=32, d=128, dtype=F16, lens=[0, 1, 200, 31, 32, 33], lam="one"),
     dict(B=2, Nq=140, Nk=150, Hq=32, Hkv=32, d=128, dtype=F16, grow=20.0, causal=True), dict(B=2, Nq=129, Nk=161, Hq=32, Hkv=32, d=128, dtype=BF, grow=36.0),
-    dict(B=5, Nq=100, Nk=70, Hq=32, Hkv=16, d=128, dtype=BF, causal=True, lens=[70, 64, 0, 1, 65], start=[-30, -99, 0, 5, -40], lam="none")],
+    dict(B=5, Nq=100, Nk=70, Hq=32, Hkv=16, d=128, dtype=BF, causal=True, lens=[70, 64, 0, 1, 65], start=[-30, -99, 0, 5, -40], lam="none"),
+    dict(B=8, Nq=65, Nk=100, Hq=32, Hkv=32, d=64, dtype=F16, causal=True), dict(B=4, Nq=130, Nk=97, Hq=32, Hkv=32, d=64, dtype=BF, causal=True),
+    dict(B=12, Nq=97, Nk=97, Hq=32, Hkv=8, d=32, dtype=BF, causal=True, lens=[0, 50, 97] * 4, start=[0, -20, 3] * 4),
+    dict(B=4, Nq=130, Nk=300, Hq=32, Hkv=32, d=128, dtype=BF, causal=True), dict(B=4, Nq=129, Nk=161, Hq=32, Hkv=32, d=128, dtype=BF, grow=36.0),
+    dict(B=8, Nq=40, Nk=200, Hq=32, Hkv=32, d=128, dtype=F16, lens=[0, 1, 200, 31, 32, 33, 199, 64], lam="one"),
+    dict(B=4, Nq=140, Nk=150, Hq=32, Hkv=32, d=128, dtype=F16, grow=20.0, causal=True)],
     ids=lambda c: f"{c['B']}x{c['Nq']}x{c['Nk']}-{c['Hq']}/{c['Hkv']}x{c['d']}")
 def test_diff_attention_of_many_rows(dev, case):
     test_diff_attention_values_and_gradients(dev, case)
@@ -320,14 +325,14 @@ def test_diff_caches_views_and_what_lies_behind(dev):
         assert H.diff_attention(q[:, :0], k, v, lam).shape == (B, 0, Hq, 2 * d) and not H.diff_attention(q, k[:, :0], v[:, :0], lam).any()
 
 
-@pytest.mark.parametrize("B,Nq,Hq,Hkv,d", [(2, 1, 4, 2, 64), (2, 5, 8, 2, 128), (3, 40, 2, 2, 32), (8, 70, 16, 16, 64), (4, 100, 16, 16, 128), (8, 100, 16, 16, 128)])
+@pytest.mark.parametrize("B,Nq,Hq,Hkv,d", [(2, 1, 4, 2, 64), (2, 5, 8, 2, 128), (3, 40, 2, 2, 32), (8, 70, 16, 16, 64), (4, 100, 16, 16, 128), (8, 100, 16, 16, 128), (16, 100, 16, 16, 128)])
 def test_diff_causal_cache_filled_to_its_queries(dev, B, Nq, Hq, Hkv, d):
     """a cache that holds NaN behind the last query's own position: the causal mask alone says that nothing there counts"""
     g = torch.Generator("cuda").manual_seed(Nq)
     S = Nq + 90
     q, k, v = rnd(g, B, Nq, 2 * Hq, d, dtype=BF), rnd(g, B, S, 2 * Hkv, d, dtype=BF), rnd(g, B, S, Hkv, 2 * d, dtype=BF)
     lam, go = torch.full((Hq,), 0.3, device="cuda"), rnd(g, B, Nq, Hq, 2 * d, dtype=BF)
-    start = torch.tensor([0, 61, -3, 40, 0, 61, -3, 40][:B], dtype=torch.int32, device="cuda")
+    start = torch.tensor(([0, 61, -3, 40] * 4)[:B], dtype=torch.int32, device="cuda")
     kw = dict(causal=True, q_start=start)
     want = run_diff(q, k, v, lam, go, dict(kw, kv_len=(start + Nq).clamp_(0, S).to(torch.int32)))
     gap = torch.arange(S, device="cuda")[None, :] >= (start + Nq)[:, None]
