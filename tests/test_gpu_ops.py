@@ -648,6 +648,58 @@ def test_adamw_steps_a_tower(dev):
     assert torch.equal(new, b(x)[0]) and not torch.equal(new, old)
 
 
+# ---- offsets beyond 32 bits --------------------------------------------------------------------------------------------------------
+def test_tokens_that_lie_far_apart(dev):
+    """tokens 2^20 and 2^21 elements apart, over more than 2^32 elements: the bits of the same tensors side by side"""
+    g = torch.Generator("cuda").manual_seed(21)
+    Nk, d, far = 4200, 64, 1 << 20
+    room = torch.empty(Nk * far, dtype=BF, device="cuda")
+    for Nq, Hq, Hkv in ((1, 4, 2), (40, 16, 16), (300, 16, 8)):
+        q, k, v = rnd(g, 1, Nq, 2 * Hq, d, dtype=BF), rnd(g, 1, Nk, 2 * Hkv, d, dtype=BF), rnd(g, 1, Nk, Hkv, 2 * d, dtype=BF)
+        K = room.as_strided((1, Nk, 2 * Hkv, d), (Nk * far, far, d, 1))
+        V = room.as_strided((1, Nk, Hkv, 2 * d), (Nk * far, far, 2 * d, 1), 4096)
+        K.copy_(k), V.copy_(v)
+        lam, go = torch.full((Hq,), 0.3, device="cuda"), rnd(g, 1, Nq, Hq, 2 * d, dtype=BF)
+        want, got = run_diff(q, k, v, lam, go, dict(causal=True)), run_diff(q, K, V, lam, go, dict(causal=True))
+        assert all(torch.equal(want[n], got[n]) for n in want)
+    plan, N = H.RotaryAxes((9, 10, 12)), 1000
+    x, pos = rnd(g, 2, N, 2, d, dtype=BF), torch.randint(0, 500, (3, 2, N), generator=g, device="cuda")
+    X = room.as_strided((2, N, 2, d), (N * 2 * far, 2 * far, d, 1))
+    X.copy_(x)
+    want = H.rotary_axes(x, None, pos, plan)
+    assert torch.equal(H.rotary_axes(X, None, pos, plan), want)
+    with torch.no_grad():
+        H.rotary_axes(X, None, pos, plan, inplace=True)
+    assert torch.equal(X, want)
+
+
+def test_diff_more_than_2_31_outputs(dev):
+    Nq, Hq, d = (1 << 17) + 5, 256, 32
+    g = torch.Generator("cuda").manual_seed(22)
+    q = torch.zeros(1, Nq, 2 * Hq, d, dtype=BF, device="cuda")
+    k, v = rnd(g, 1, 40, 2, d, dtype=BF), rnd(g, 1, 40, 1, 2 * d, dtype=BF)
+    o = H.diff_attention(q, k, v, torch.tensor(0.5, device="cuda"), kv_len=torch.tensor([1], dtype=torch.int32, device="cuda"))
+    want = 0.5 * v[:, :1]
+    for part in (o[:, :3000], o[:, 65000:68000], o[:, -3000:]):
+        assert torch.equal(part, want.expand_as(part))
+
+
+def test_adamw_more_than_2_31_elements(dev):
+    n = (1 << 31) + 777
+    tail = (n // 256 - 20) * 256
+    g = torch.Generator("cuda").manual_seed(23)
+    p, grad = torch.zeros(n, dtype=BF, device="cuda"), torch.zeros(n, dtype=BF, device="cuda")
+    p[tail:], grad[tail:] = rnd(g, n - tail, dtype=BF), rnd(g, n - tail, dtype=BF)
+    small = p[tail:].clone()
+    small.grad = grad[tail:].clone()
+    p.grad = grad
+    big, other = H.AdamW([p], state_bits=8, **NUM), H.AdamW([small], state_bits=8, **NUM)
+    big.step(), other.step()
+    assert torch.equal(p[tail:], small) and not p[:1 << 20].any() and not p[tail - (1 << 20):tail].any()
+    for name in ("exp_avg", "exp_avg_sq"):
+        assert torch.equal(big.state[p][name][tail:], other.state[small][name]) and not big.state[p][name][tail - (1 << 20):tail].any()
+
+
 # ---- the three together ----------------------------------------------------------------------------------------------------------
 def test_one_training_step_of_an_attention_layer(dev):
     """projection -> rotary positions of a volume's tokens -> differential attention -> output projection -> loss -> AdamW on all weights, beside the
