@@ -61,6 +61,9 @@ __device__ __forceinline__ int visible(const Args& a, int len, int start, int i)
 // A wave's instruction moves 8 rows of an image, 16 bytes a lane; the image's swizzle is applied to the source.  It is written out because its builtin
 // makes the compiler wait for it in front of the next LDS read, whatever that reads: issue() only starts the transfers, landed() waits for this
 // wave's; a barrier behind landed() makes a tile readable to the others.
+// The compiler does not look into the text, so the text itself holds the five wait states between a vector instruction that writes a scalar register (the
+// descriptor and the offset come out of v_readfirstlane) and a memory instruction that reads it; M0 needs one of them.
+#define HS_LDS_DMA_WAITS "s_mov_b32 m0, %0\n\ts_nop 3\n\t"
 template <int D, int VC, int ROWS, int NW> struct Dma {
     static constexpr int PAIRS = D / 32, IMAGES = PAIRS + VC / 64, GROUPS = ROWS / 8, PER = IMAGES * GROUPS / NW;
     static_assert(PER * NW == IMAGES * GROUPS && (NW == 1 || NW % GROUPS == 0), "whole pieces");
@@ -107,7 +110,7 @@ template <int D, int VC, int ROWS, int NW> struct Dma {
             off = row + more < left ? off : HS_OOB_OFF;
             const unsigned so = (unsigned)(pair ? more * x_n + (D == 32 ? 0 : D == 64 ? im * x_h : (im >> 1) * x_h + (im & 1) * 128) : more * y_n + im * 128);
             const unsigned at = lds + image * (ROWS * 128) + group * 1024;
-            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+            asm volatile(HS_LDS_DMA_WAITS "buffer_load_dwordx4 %1, %2, %3 offen lds"
                          :: "s"(__builtin_amdgcn_readfirstlane(at)), "v"(off), "s"(pair ? rx : ry), "s"(__builtin_amdgcn_readfirstlane(so)) : "memory");
         }
     }
@@ -1143,7 +1146,7 @@ __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void d
         dma.issue(lds0 + sbuf * TILE);
         if (wave < 2) {
             const u32x4 r = Dma<D, 2 * D, ROWS, NW>::resource(srow);
-            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+            asm volatile(HS_LDS_DMA_WAITS "buffer_load_dword %1, %2, 0 offen lds"
                          :: "s"(__builtin_amdgcn_readfirstlane(lds0 + NBUF * TILE + sbuf * 512 + wave * 256)), "v"(lane * 4), "s"(r) : "memory");
         }
         sbuf = S::next(sbuf);
