@@ -1322,7 +1322,8 @@ int check(const hs_diff_attn_desc* d, bool backward) {
     if (!(d->scale > 0.f) || !(d->scale < 1e6f) || d->lam_stride < 0) return HS_ERR_ARG;
     if (d->B < 1 || d->Nq < 1 || d->Nk < 1 || d->H < 1 || d->Hkv < 1 || d->H % d->Hkv) return HS_ERR_SHAPE;
     if (d->d != 32 && d->d != 64 && d->d != 128) return HS_ERR_SHAPE;
-    if (d->Nq > (1 << 28) || d->Nk > (1 << 28) || d->H > (1 << 16) || (int64_t)d->B * d->H * ((int64_t)d->Nq + d->Nk) > ((int64_t)1 << 36)) return HS_ERR_SHAPE;
+    if (d->Nq > (1 << 28) || d->Nk > (1 << 28) || d->H > (1 << 16)) return HS_ERR_SHAPE;
+    if ((int64_t)d->B * d->H > ((int64_t)1 << 36) / ((int64_t)d->Nq + d->Nk)) return HS_ERR_SHAPE;
     // every launch stays under 2^32 threads: the sweeps have 512 for 256 rows or 256 for 64 or 128, the split forward 256 for 16, twice as many at most as
     // the whole forward, and the rows' constants d / 4 for one
     if ((int64_t)d->B * d->H * (((int64_t)(d->Nq > d->Nk ? d->Nq : d->Nk) + 127) / 128) >= (1 << 22)) return HS_ERR_SHAPE;
@@ -1387,7 +1388,7 @@ size_t forward_bytes(const hs_diff_attn_desc* d, const Split& s, int cuts) {
 int parts_of(const hs_diff_attn_desc* d) {
     return cuts_of((int64_t)d->B * d->Hkv * ((d->Nk + own_of(d) - 1) / own_of(d)), (double)(d->H / d->Hkv) * ((d->Nq + 31) / 32), 4, 0.07).parts;
 }
-size_t rows_bytes(const hs_diff_attn_desc* d) { return (size_t)d->B * d->H * (d->Nq * 12 + (size_t)((d->Nq + 31) / 32) * 512); }
+size_t rows_bytes(const hs_diff_attn_desc* d) { return (size_t)d->B * d->H * ((size_t)d->Nq * 12 + (size_t)((d->Nq + 31) / 32) * 512); }
 // parts of the dq sweep's keys (see cuts_of)
 int cuts_of_dq(const hs_diff_attn_desc* d) { return cuts_of(blocks_of(d), (double)((d->Nk + 31) / 32), 4, 0.045 * d->d / 64).parts; }
 // Behind the rows' numbers lie dq's parts (sums, then a number a row), and, when these have been put together, those of dk and dv.

@@ -229,6 +229,7 @@ extern "C" int hs_rotary_axes(const hs_rotary_desc* d, const void* x0, void* y0,
     if (d->B < 1 || d->N < 1 || d->heads[0] < 1 || d->heads[1] < 0 || d->pairs < 1 || d->pairs > HS_ROTARY_MAX_PAIRS || d->axes < 1) return HS_ERR_SHAPE;
     if (d->dh < 2 * d->pairs || d->dh > 4096 || (int64_t)d->B * d->N > 0x7fffffff - 64) return HS_ERR_SHAPE;
     if (d->heads[1] && (!x1 || !y1)) return HS_ERR_ARG;
+    if (d->heads[0] > 4096 || d->heads[1] > 4096) return HS_ERR_SHAPE;
     const int heads = d->heads[0] + d->heads[1];
     if (heads > 4096 || (int64_t)heads * d->dh > (1 << 18)) return HS_ERR_SHAPE;      // a block's item numbers stay far inside fp32's whole numbers
     const int size = d->dtype == HS_PREC_F32 ? 4 : 2, full = 16 / size;

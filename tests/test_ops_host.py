@@ -147,3 +147,20 @@ def test_rotary_ladders():
     assert shared.axis.tolist() == per.axis.tolist() == [0, 0, 1, 1, 1, 2, 2, 2] and shared.freq.dtype == torch.float64
     assert torch.allclose(shared.freq, 100.0 ** (-torch.arange(8, dtype=torch.float64) / 8), rtol=1e-14)
     assert torch.allclose(per.freq, 100.0 ** -torch.tensor([0, 1 / 2, 0, 1 / 3, 2 / 3, 0, 1 / 3, 2 / 3], dtype=torch.float64), rtol=1e-14)
+
+
+def test_diff_attention_workspace_beyond_2_31_bytes_of_rows():
+    """twelve bytes a query pass 2^31 from 178956971 queries on"""
+    for Nq in (178956970, 178956971, 200_000_000, 1 << 28):
+        need = O.load().hs_diff_attn_bwd_ws_bytes(C.byref(_diff(B=1, Nq=Nq, Nk=40, H=1, Hkv=1, d=32)))
+        assert need >= Nq * 12 + -(-Nq // 32) * 512, Nq
+
+
+@no_gpu_only
+def test_sizes_whose_products_wrap_are_refused():
+    lib, big = O.load(), _diff(B=1 << 30, H=1 << 16, Hkv=1 << 16, Nq=1 << 28, Nk=1 << 28)
+    assert lib.hs_diff_attn_fwd(C.byref(big), P, P, P, P, None, None, P, None, None, P, (1 << 63) - 1, None) == L.HS_ERR_SHAPE
+    assert lib.hs_diff_attn_bwd(C.byref(big), P, P, P, P, None, None, P, P, P, P, P, P, P, P, (1 << 63) - 1, None) == L.HS_ERR_SHAPE
+    heads = _rot()
+    heads.heads[0] = heads.heads[1] = (1 << 31) - 1
+    assert lib.hs_rotary_axes(C.byref(heads), P, P, P, P, P, P, P, None) == L.HS_ERR_SHAPE
