@@ -1324,8 +1324,8 @@ int check(const hs_diff_attn_desc* d, bool backward) {
     if (d->d != 32 && d->d != 64 && d->d != 128) return HS_ERR_SHAPE;
     if (d->Nq > (1 << 28) || d->Nk > (1 << 28) || d->H > (1 << 16)) return HS_ERR_SHAPE;
     if ((int64_t)d->B * d->H > ((int64_t)1 << 36) / ((int64_t)d->Nq + d->Nk)) return HS_ERR_SHAPE;
-    // every launch stays under 2^32 threads: the sweeps have 512 for 256 rows or 256 for 64 or 128, the split forward 256 for 16, twice as many at most as
-    // the whole forward, and the rows' constants d / 4 for one
+    // every launch stays under 2^32 threads: the sweeps have 512 for 256 rows or 256 for 64 or 128, the rows' constants d / 4 for one (split_of sees to the
+    // split forward, 256 for 16)
     if ((int64_t)d->B * d->H * (((int64_t)(d->Nq > d->Nk ? d->Nq : d->Nk) + 127) / 128) >= (1 << 22)) return HS_ERR_SHAPE;
     if (backward && (int64_t)d->B * d->H * (((int64_t)d->Nq + 31) / 32) * 8 * d->d >= (int64_t)1 << 32) return HS_ERR_SHAPE;
     for (int64_t s : {d->q_b, d->q_n, d->q_h, d->k_b, d->k_n, d->k_h, d->v_b, d->v_n, d->v_h})
@@ -1370,6 +1370,7 @@ Split split_of(const hs_diff_attn_desc* d) {
     const int64_t rows = (int64_t)(d->H / d->Hkv) * d->Nq, tiles = (rows + 15) / 16, blocks = (int64_t)d->B * d->Hkv * tiles;
     const double time = (d->d == 128 ? 0.0019 : 0.00135) * (double)blocks * (double)((d->Nk + 31) / 32);      // us beside 8 of start and join
     if (time > 4 && time + 8 > whole_of(d).time) return {0, 0, 0};          // (small calls take launches either way, and the split forward rounds less)
+    if (blocks >= 1 << 24) return {0, 0, 0};                                // (a block of 256 threads for each 16 rows: a launch ends at 2^32)
     const int64_t want = std::min<int64_t>((WANT + blocks - 1) / blocks, MOST_CHUNKS);
     // (a grid that leaves most CUs idle anyway takes half as long chunks, unless one would do without the join: 1 entry, 2000 keys 12 -> 11 us)
     const int64_t least = d->Nk > LEAST && blocks * ((d->Nk + LEAST - 1) / LEAST) <= SPARSE ? LEAST / 2 : LEAST;

@@ -11,6 +11,7 @@ import torch
 
 import hsenet_amd as H
 from hsenet_amd import _lib as L
+from hsenet_amd import _ops as O
 
 pytestmark = pytest.mark.gpu
 BF, F16, F32 = torch.bfloat16, torch.float16, torch.float32
@@ -682,6 +683,20 @@ def test_diff_more_than_2_31_outputs(dev):
     want = 0.5 * v[:, :1]
     for part in (o[:, :3000], o[:, 65000:68000], o[:, -3000:]):
         assert torch.equal(part, want.expand_as(part))
+
+
+def test_diff_more_blocks_than_a_launch_holds(dev):
+    """129 queries of one key each in 2^21 - 1 entries: 16 rows a block would be 2^32 threads and more"""
+    B, Nq, d = (1 << 21) - 1, 129, 32
+    g = torch.Generator("cuda").manual_seed(25)
+    q, k, v = torch.zeros(1, Nq, 2, d, dtype=BF, device="cuda"), torch.zeros(1, 1, 2, d, dtype=BF, device="cuda"), rnd(g, B, 1, 1, 2 * d, dtype=BF)
+    lam, o = torch.tensor(0.5, device="cuda"), torch.full((B, Nq, 1, 2 * d), math.nan, dtype=BF, device="cuda")
+    # (the C call: q and k of one entry stand for all)
+    desc = O.DIFF_PACK.pack(O.DIFF_PACK.size, B, Nq, 1, 1, 1, d, O.DTYPE[BF], 0, 0, 0, 0.5, 0, 2 * d, d, 0, 0, d, 2 * d, 0, 0, 0, 0, 0)
+    assert O.load().hs_diff_attn_fwd_ws_bytes(desc) == 0
+    O.call(0, "hs_diff_attn_fwd", desc, q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), None, None, o.data_ptr(), None, None, None, 0)
+    for at in range(0, B, 1 << 17):
+        assert torch.equal(o[at:at + (1 << 17)], (0.5 * v[at:at + (1 << 17)]).expand(-1, Nq, -1, -1))
 
 
 def test_adamw_more_than_2_31_elements(dev):
