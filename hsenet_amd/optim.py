@@ -86,7 +86,21 @@ class AdamW(torch.optim.Optimizer):
         self.state[p] = {"step": rec.to(p.device), **new}
 
     @staticmethod
+    def _fits(st, bits, n, dev) -> bool:
+        """whether a state is of the bits, the size and the device of a parameter of n elements and lies dense: what can be seen without its shape"""
+        m, v, t, (dm, dv) = st["exp_avg"], st["exp_avg_sq"], st["step"], _BYTES[bits]
+        if not (m.dtype is dm and v.dtype is dv and m.numel() == n == v.numel() and m.get_device() == dev == v.get_device() == t.get_device()
+                and t.numel() == 4 and m.is_contiguous() and v.is_contiguous()):
+            return False
+        if bits == 32:
+            return True
+        m, v, n = st["exp_avg_scale"], st["exp_avg_sq_scale"], -(-n // O.ADAMW_BLOCK)
+        return m.numel() == n == v.numel() and m.get_device() == dev == v.get_device()
+
+    @staticmethod
     def _check_state(p, st, bits) -> None:
+        if not _dense(p):
+            raise L.HsError("a parameter's elements must fill one stretch of memory")
         dm, dv = _BYTES[bits]
         for name, dt in (("exp_avg", dm), ("exp_avg_sq", dv)):
             t = st.get(name)
@@ -123,7 +137,7 @@ class AdamW(torch.optim.Optimizer):
                 loss = closure()
         for group in self.param_groups:
             numbers, bits = self._check_numbers(group), group["state_bits"]
-            tables, changed, state, key, words = {}, [], self.state, None, None       # (device, type) -> (addresses, gradients)
+            tables, changed, state, key, words, fits = {}, [], self.state, None, None, self._fits       # (device, type) -> (addresses, gradients)
             for p in group["params"]:
                 g = p.grad
                 if g is None:
@@ -135,14 +149,10 @@ class AdamW(torch.optim.Optimizer):
                     raise L.HsError("a gradient must be dense, of its parameter's type and on its device")
                 st = state.get(p) or self._init_state(p, bits)
                 m, v, n = st["exp_avg"], st["exp_avg_sq"], p.numel()
-                if not (p.is_contiguous() and g.is_contiguous() and m.is_contiguous() and v.is_contiguous()):
-                    if not _dense(p):
-                        raise L.HsError("a parameter's elements must fill one stretch of memory")
+                if not (p.is_contiguous() and g.is_contiguous() and fits(st, bits, n, dev)):
+                    self._check_state(p, st, bits)
                     if g.stride() != p.stride():
                         g = torch.empty_like(p).copy_(g)
-                    self._check_state(p, st, bits)
-                elif m.numel() != n or m.get_device() != dev:  # (the parameter has been moved or given other data)
-                    self._check_state(p, st, bits)
                 if key != (dev, dtype):
                     key = (dev, dtype)
                     if key not in tables:
@@ -185,7 +195,10 @@ class AdamW(torch.optim.Optimizer):
                 if not st:
                     m.zero_()
                     v.zero_()
-                elif bits == 32:
+                    continue
+                if not (p.is_contiguous() and self._fits(st, bits, p.numel(), dev)):
+                    self._check_state(p, st, bits)
+                if bits == 32:
                     m.copy_(st["exp_avg"])
                     v.copy_(st["exp_avg_sq"])
                 else:

@@ -164,3 +164,71 @@ def test_sizes_whose_products_wrap_are_refused():
     heads = _rot()
     heads.heads[0] = heads.heads[1] = (1 << 31) - 1
     assert lib.hs_rotary_axes(C.byref(heads), P, P, P, P, P, P, P, None) == L.HS_ERR_SHAPE
+
+
+def _launches(monkeypatch):
+    """the launches of what follows, recorded instead of made, with host tensors that pass for tensors of device 0"""
+    seen = []
+    monkeypatch.setattr(O, "call", lambda dev, name, *a: seen.append(name))
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda t: 0)
+    return seen
+
+
+def _state(p, bits, step=1):
+    n = -(-p.numel() // 256)
+    m = torch.zeros_like(p, dtype=torch.int8 if bits == 8 else torch.float32, requires_grad=False)
+    v = torch.zeros_like(p, dtype=torch.uint8 if bits == 8 else torch.float32, requires_grad=False)
+    return dict(step=step, exp_avg=m, exp_avg_sq=v, **(dict(exp_avg_scale=torch.zeros(n), exp_avg_sq_scale=torch.zeros(n)) if bits == 8 else {}))
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_adamw_states_that_no_longer_fit_are_not_read(monkeypatch, bits):
+    """neither a step nor a reading of the moments hands a kernel a state that another size, type or order of the parameter needs"""
+    seen = _launches(monkeypatch)
+    p = torch.nn.Parameter(torch.zeros(6, 4))
+    opt = H.AdamW([p], state_bits=bits)
+    opt.set_state(p, **_state(p, bits))
+    p.grad = torch.zeros(6, 4)
+    opt.step()
+    opt.moments(p)
+    assert seen == ["hs_adamw_multi"] + ["hs_adamw_moments"] * (bits == 8)
+    seen.clear()
+    def refused():
+        p.grad = torch.zeros_like(p)
+        for f in (opt.step, lambda: opt.moments(p)):
+            with pytest.raises(L.HsError):
+                f()
+        assert not seen
+    for data in (torch.zeros(600, 400), torch.zeros(0), torch.zeros(4, 6).t(), torch.zeros(6, 8)[:, :4]):
+        p.grad = None
+        p.data = data
+        refused()
+    p.grad = None
+    p.data = torch.zeros(6, 4)
+    opt.param_groups[0]["state_bits"] = 40 - bits
+    refused()
+    opt.param_groups[0]["state_bits"] = bits
+    for name in ("exp_avg", "exp_avg_sq", "step", *(("exp_avg_scale", "exp_avg_sq_scale") if bits == 8 else ())):
+        held = opt.state[p][name]
+        opt.state[p][name] = held.flatten()[:0]
+        refused()
+        opt.state[p][name] = held
+    opt.step()
+    assert seen == ["hs_adamw_multi"]
+
+
+def test_adamw_states_on_another_device_are_not_read(monkeypatch):
+    seen = _launches(monkeypatch)
+    p = torch.nn.Parameter(torch.zeros(6, 4))
+    opt = H.AdamW([p], state_bits=8)
+    opt.set_state(p, **_state(p, 8))
+    p.grad = torch.zeros(6, 4)
+    for name in list(opt.state[p]):
+        held = opt.state[p][name]
+        opt.state[p][name] = torch.empty_like(held, device="meta")
+        monkeypatch.setattr(torch.Tensor, "get_device", lambda t: 1 if t.is_meta else 0)
+        for f in (opt.step, lambda: opt.moments(p)):
+            with pytest.raises(L.HsError, match="device"):
+                f()
+        opt.state[p][name] = held
+    assert not seen
