@@ -219,7 +219,8 @@ class AdamW(torch.optim.Optimizer):
         return m, v
 
     def load_state_dict(self, state_dict) -> None:
-        """as torch's, but codes and scales keep their types (torch casts a floating parameter's state to the parameter's type)"""
+        """as torch's, but codes and scales keep their types (torch casts a floating parameter's state to the parameter's type).  Moments of 32 bits go to
+        the order that the parameter's elements have in memory; codes have to come in that order, for their scales are those of 256 neighbours there."""
         super().load_state_dict(state_dict)
         saved: List = [i for g in state_dict["param_groups"] for i in g["params"]]
         for i, (p, bits) in zip(saved, [(p, g["state_bits"]) for g in self.param_groups for p in g["params"]]):
@@ -229,6 +230,11 @@ class AdamW(torch.optim.Optimizer):
             new = {}
             for k, t in st.items():
                 if k in ("exp_avg", "exp_avg_sq"):
+                    if t.shape != p.shape:
+                        raise L.HsError(f"{k} must be of its parameter's shape {tuple(p.shape)}, got {tuple(t.shape)}")
+                    if bits == 8 and any(n > 1 and a != b for n, a, b in zip(p.shape, p.stride(), t.stride())):
+                        raise L.HsError(f"{k}: codes of 8 bits belong to the memory order that they were made in, strides {t.stride()}; their parameter "
+                                        f"has {p.stride()}")
                     t = torch.empty_like(p, dtype=t.dtype, requires_grad=False).copy_(t)
                 elif isinstance(t, torch.Tensor):
                     t = t.detach().to(p.device, copy=True).contiguous()

@@ -232,3 +232,38 @@ def test_adamw_states_on_another_device_are_not_read(monkeypatch):
                 f()
         opt.state[p][name] = held
     assert not seen
+
+
+@pytest.mark.parametrize("order", [lambda t: t.contiguous(memory_format=torch.channels_last), lambda t: t.transpose(0, 1).contiguous().transpose(0, 1)])
+def test_adamw_codes_are_loaded_in_their_memory_order_alone(order):
+    """a scale belongs to 256 neighbours in memory: codes of another order would be read with others' scales"""
+    g = torch.Generator().manual_seed(1)
+    def made(data, bits):
+        p = torch.nn.Parameter(data)
+        opt = H.AdamW([p], state_bits=bits)
+        st = _state(p, bits)
+        st["exp_avg"].copy_(torch.randint(-127, 128, p.shape, generator=g))
+        opt.set_state(p, **st)
+        return opt, p
+    plain, other = torch.zeros(4, 16, 3, 8), order(torch.zeros(4, 16, 3, 8))
+    for bits in (8, 32):
+        (a, p), (b, q), (c, r) = made(other, bits), made(plain, bits), made(other.clone(memory_format=torch.preserve_format), bits)
+        want = a.state[p]["exp_avg"]
+        c.load_state_dict(a.state_dict())                     # the same order: taken over as it is
+        assert torch.equal(c.state[r]["exp_avg"], want) and c.state[r]["exp_avg"].stride() == r.stride()
+        if bits == 8:
+            there, back = a.state_dict(), b.state_dict()
+            for opt, saved in ((b, there), (a, back)):
+                with pytest.raises(L.HsError, match="memory order"):
+                    opt.load_state_dict(saved)
+        else:
+            b.load_state_dict(a.state_dict())
+            assert torch.equal(b.state[q]["exp_avg"], want) and b.state[q]["exp_avg"].is_contiguous()
+
+
+def test_adamw_states_of_another_shape_are_not_spread():
+    p, q = torch.nn.Parameter(torch.zeros(8, 6)), torch.nn.Parameter(torch.zeros(6))
+    a, b = H.AdamW([p]), H.AdamW([q])
+    b.set_state(q, **_state(q, 32))
+    with pytest.raises(L.HsError, match="shape"):
+        a.load_state_dict(b.state_dict())
