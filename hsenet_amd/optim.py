@@ -220,8 +220,24 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict) -> None:
         """as torch's, but codes and scales keep their types (torch casts a floating parameter's state to the parameter's type).  Moments of 32 bits go to
-        the order that the parameter's elements have in memory; codes have to come in that order, for their scales are those of 256 neighbours there."""
-        super().load_state_dict(state_dict)
+        the order that the parameter's elements have in memory; codes have to come in that order, for their scales are those of 256 neighbours there.
+        A state_dict that is refused leaves the optimizer as it was."""
+        held = self.state, self.param_groups
+        try:
+            super().load_state_dict(state_dict)
+            self._take_states(state_dict)
+        except Exception:
+            self.state, self.param_groups = held
+            raise
+
+    def _take_states(self, state_dict) -> None:
+        for g in self.param_groups:
+            lost = [k for k in ("lr", "betas", "eps", "weight_decay", "state_bits") if k not in g]
+            if lost:
+                raise L.HsError(f"a loaded group has no {', '.join(lost)}")
+            self._check_numbers(g)
+            if g["state_bits"] not in (8, 32):
+                raise L.HsError(f"state_bits must be 8 or 32, got {g['state_bits']}")
         saved: List = [i for g in state_dict["param_groups"] for i in g["params"]]
         for i, (p, bits) in zip(saved, [(p, g["state_bits"]) for g in self.param_groups for p in g["params"]]):
             st = state_dict["state"].get(i)

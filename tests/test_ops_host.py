@@ -1,5 +1,6 @@
 """The operators' library without a GPU: what it exports is what its header declares, bad arguments are refused before anything could be launched
 (the pointers here are fakes that are never read), and the Python entry points refuse what the kernels cannot take."""
+import copy
 import ctypes as C
 import os
 import re
@@ -267,3 +268,29 @@ def test_adamw_states_of_another_shape_are_not_spread():
     b.set_state(q, **_state(q, 32))
     with pytest.raises(L.HsError, match="shape"):
         a.load_state_dict(b.state_dict())
+
+
+def test_adamw_that_refuses_a_state_dict_is_as_before():
+    ps = [torch.nn.Parameter(torch.zeros(6, 4)), torch.nn.Parameter(torch.zeros(300))]
+    opt = H.AdamW(ps, lr=0.25, state_bits=8)
+    for p in ps:
+        opt.set_state(p, **_state(p, 8, step=7))
+    good = opt.state_dict()
+    def bad(where, what):
+        d = copy.deepcopy(good)
+        d["param_groups"][0]["lr"] = 0.5
+        where(d).update(what) if isinstance(what, dict) else where(d).pop(what)
+        return d
+    first, second, group = lambda d: d["state"][0], lambda d: d["state"][1], lambda d: d["param_groups"][0]
+    cases = [bad(second, dict(exp_avg=torch.zeros(299, dtype=torch.int8))), bad(second, dict(exp_avg=torch.zeros(300))), bad(second, "exp_avg_sq_scale"),
+             bad(second, dict(step=torch.tensor(3.0))), bad(first, "exp_avg_sq"), bad(group, "state_bits"), bad(group, dict(state_bits=16)),
+             bad(group, dict(lr=-1.0)), bad(group, dict(params=[0])), torch.optim.AdamW(ps).state_dict()]
+    held = [{k: t for k, t in opt.state[p].items()} for p in ps]
+    for d in cases:
+        with pytest.raises((L.HsError, ValueError)):
+            opt.load_state_dict(d)
+        assert opt.param_groups[0]["lr"] == 0.25 and opt.param_groups[0]["state_bits"] == 8 and len(opt.state) == 2
+        for p, st in zip(ps, held):
+            assert list(opt.state[p]) == list(st) and all(opt.state[p][k] is t for k, t in st.items())
+    opt.load_state_dict(good)
+    assert all(int(opt.state[p]["step"][0]) == 7 and opt.state[p]["exp_avg"].dtype == torch.int8 for p in ps)
