@@ -135,9 +135,10 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        launches, changed = [], []                             # (a step that is refused for one parameter is taken for none)
         for group in self.param_groups:
             numbers, bits = self._check_numbers(group), group["state_bits"]
-            tables, changed, state, key, words, fits = {}, [], self.state, None, None, self._fits       # (device, type) -> (addresses, gradients)
+            tables, state, key, words, fits = {}, self.state, None, None, self._fits       # (device, type) -> (addresses, gradients)
             for p in group["params"]:
                 g = p.grad
                 if g is None:
@@ -167,10 +168,11 @@ class AdamW(torch.optim.Optimizer):
                 else:
                     words.extend((p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), 0, 0, st["step"].data_ptr(), n))
                 changed.append(p)
-            for (dev, dtype), (words, _) in tables.items():
-                O.call(dev, "hs_adamw_multi", words.buffer_info()[0], len(words) // 8, O.DTYPE[dtype], bits, *numbers)
-            if changed:
-                torch.autograd.graph.increment_version(changed)
+            launches += [(dev, words, held, O.DTYPE[dtype], bits, numbers) for (dev, dtype), (words, held) in tables.items()]
+        for dev, words, _, dtype, bits, numbers in launches:
+            O.call(dev, "hs_adamw_multi", words.buffer_info()[0], len(words) // 8, dtype, bits, *numbers)
+        if changed:
+            torch.autograd.graph.increment_version(changed)
         return loss
 
     @torch.no_grad()

@@ -294,3 +294,23 @@ def test_adamw_that_refuses_a_state_dict_is_as_before():
             assert list(opt.state[p]) == list(st) and all(opt.state[p][k] is t for k, t in st.items())
     opt.load_state_dict(good)
     assert all(int(opt.state[p]["step"][0]) == 7 and opt.state[p]["exp_avg"].dtype == torch.int8 for p in ps)
+
+
+def test_adamw_step_that_is_refused_for_one_is_taken_for_none(monkeypatch):
+    seen = _launches(monkeypatch)
+    p, q = torch.nn.Parameter(torch.zeros(6, 4)), torch.nn.Parameter(torch.zeros(5))
+    opt = H.AdamW([{"params": [p]}, {"params": [q], "lr": 0.1}])
+    for x in (p, q):
+        opt.set_state(x, **_state(x, 32))
+        x.grad = torch.zeros_like(x)
+    q.data, versions = torch.zeros(7), (p._version, q._version)
+    with pytest.raises(L.HsError):
+        opt.step()
+    q.data = torch.zeros(5)
+    opt.param_groups[1]["lr"] = -0.1
+    with pytest.raises(ValueError):
+        opt.step()
+    assert not seen and p._version == versions[0]
+    opt.param_groups[1]["lr"] = 0.1
+    opt.step()
+    assert seen == ["hs_adamw_multi"] * 2 and p._version > versions[0]
