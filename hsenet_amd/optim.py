@@ -70,7 +70,10 @@ class AdamW(torch.optim.Optimizer):
         return float(lr), float(b1), float(b2), float(eps), float(wd)
 
     def _bits(self, p) -> int:
-        return next(g["state_bits"] for g in self.param_groups if any(q is p for q in g["params"]))
+        for g in self.param_groups:
+            if any(q is p for q in g["params"]):
+                return g["state_bits"]
+        raise L.HsError("not a parameter of this optimizer")
 
     def set_state(self, p: torch.Tensor, *, step: int, exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor, exp_avg_scale: Optional[torch.Tensor] = None,
                   exp_avg_sq_scale: Optional[torch.Tensor] = None) -> None:
@@ -80,10 +83,13 @@ class AdamW(torch.optim.Optimizer):
             new.update(exp_avg_scale=exp_avg_scale, exp_avg_sq_scale=exp_avg_sq_scale)
         elif exp_avg_scale is not None or exp_avg_sq_scale is not None:
             raise L.HsError("32-bit moments have no scales")
+        if not 0 <= int(step) < 1 << 31:
+            raise L.HsError(f"step must be the number of steps done, 0 or more, got {step}")
         rec = torch.zeros(4, dtype=torch.int32)
         rec[0] = int(step)
-        self._check_state(p, {"step": rec.to(p.device), **new}, bits)
-        self.state[p] = {"step": rec.to(p.device), **new}
+        st = {"step": rec.to(p.device), **new}
+        self._check_state(p, st, bits)
+        self.state[p] = st
 
     @staticmethod
     def _fits(st, bits, n, dev) -> bool:

@@ -314,3 +314,14 @@ def test_adamw_step_that_is_refused_for_one_is_taken_for_none(monkeypatch):
     opt.param_groups[1]["lr"] = 0.1
     opt.step()
     assert seen == ["hs_adamw_multi"] * 2 and p._version > versions[0]
+
+
+def test_adamw_refuses_bad_counts_and_strangers():
+    p, q = torch.nn.Parameter(torch.zeros(6, 4)), torch.nn.Parameter(torch.zeros(6, 4))
+    opt = H.AdamW([p])
+    for step in (-1, 1 << 31):                                # (with -1 the next step would divide by 1 - beta^0)
+        with pytest.raises(L.HsError, match="step"):
+            opt.set_state(p, **_state(p, 32, step=step))
+    for f in (lambda: opt.set_state(q, **_state(q, 32)), lambda: opt.moments(q)):
+        with pytest.raises(L.HsError, match="not a parameter"):
+            f()
