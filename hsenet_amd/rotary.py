@@ -46,6 +46,63 @@ class RotaryAxes:
         return RotaryAxes(self.sections, self.theta, self.ladder, self.interleaved, device)
 
 
+def _apart(B, N, dh, live) -> bool:
+    """a quick proof, for the usual layouts, that no two elements of one or two tensors lie in the same place: entries, tokens and heads step over each
+    other in that order, and the tensors lie behind one another, or both inside each row of the same larger tensor"""
+    spans = []
+    for h, _, (sb, sn, sh), _, _ in live:
+        head = (h - 1) * sh + dh
+        entry = (N - 1) * sn + head
+        if (h > 1 and sh < dh) or (N > 1 and sn < head) or (B > 1 and sb < entry):
+            return False
+        spans.append((head, (B - 1) * sb + entry))
+    if len(live) == 1:
+        return True
+    (_, x, (sb, sn, _), _, _), (_, y, (tb, tn, _), _, _) = live
+    gap, size = y.data_ptr() - x.data_ptr(), x.element_size()
+    if gap >= spans[0][1] * size or -gap >= spans[1][1] * size:
+        return True
+    row = sn if N > 1 else sb
+    at, part = divmod(gap % (row * size), size) if row else (0, 1)
+    return not part and row == (tn if N > 1 else tb) and sb % row == 0 == tb % row and spans[0][0] <= at <= row - spans[1][0]
+
+
+def _extent(x, below=None):
+    """(elements from x's first to its last, whether every stride steps over all that shorter ones reach); of the strides under `below` alone"""
+    reach, plain = 1, True
+    for s, n in sorted((s, n) for s, n in zip(x.stride(), x.shape) if n > 1 and (below is None or s < below)):
+        plain &= s >= reach
+        reach += (n - 1) * s
+    return reach, plain
+
+
+def _share_memory(xs) -> bool:
+    """whether two elements of the tensors (one or two [B, N, heads, columns] with their columns side by side) lie in the same place"""
+    if all(_extent(x)[1] for x in xs):
+        if len(xs) == 1:
+            return False
+        x, y = sorted(xs, key=torch.Tensor.data_ptr)
+        size = x.element_size()
+        gap, part = divmod(y.data_ptr() - x.data_ptr(), size)
+        if gap >= _extent(x)[0]:
+            return False
+        # views of the same rows (the thirds of a projection): where all longer strides are multiples of one, places modulo it tell them apart
+        for m in {s for s, n in zip(x.stride(), x.shape) if n > 1 and s > 1} if part == 0 else ():
+            if all(s < m or s % m == 0 for t in xs for s, n in zip(t.stride(), t.shape) if n > 1):
+                at, left, right = gap % m, _extent(x, m)[0], _extent(y, m)[0]
+                if left <= at and at + right <= m:
+                    return False
+    # rows of `columns` elements side by side share some where two starts are nearer than that
+    starts = []
+    for x in xs:
+        at = torch.tensor(x.data_ptr(), dtype=torch.int64)
+        for s, n in zip(x.stride()[:3], x.shape[:3]):
+            at = at[..., None] + torch.arange(n, dtype=torch.int64) * (s * x.element_size())
+        starts.append(at.flatten())
+    at = torch.cat(starts).sort().values
+    return bool((at.diff() < xs[0].shape[3] * xs[0].element_size()).any())
+
+
 def _turn(xs, positions, plan, inverse, inplace):
     """the turned tensors of xs (one or two [B, N, heads, dh] of one type), new ones or xs themselves"""
     if not isinstance(plan, RotaryAxes):
@@ -90,6 +147,8 @@ def _turn(xs, positions, plan, inverse, inplace):
         outs.append(y)
         if B * N * h * dh:
             live.append((h, x, O.bnh(xshape, stride), y, O.bnh(xshape, ystride)))
+    if inplace and live and not _apart(B, N, dh, live) and _share_memory([x for _, x, _, _, _ in live]):
+        raise L.HsError("tensors that overlap, or one that overlaps itself, cannot be turned in place")
     if live:
         h0, x0, s0, y0, t0 = live[0]
         h1, x1, s1, y1, t1 = live[1] if len(live) > 1 else (0, None, (0, 0, 0), None, (0, 0, 0))
@@ -125,7 +184,7 @@ def rotary_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Ten
     """q [B, N, H, dh] and k [B, N, Hkv, dh] (or None) turned by ``positions`` ([axes, N], or [axes, B, N] where the batch entries differ; int32, int64
     or float32) in one launch: (q', k'), or q' where k is None.  bf16, fp16 or fp32; angles are held in 64 bits.  The tensors may be
     views with their columns side by side (the q and k thirds of one projection); the results are dense.  Differentiable in q and k.
-    ``inplace``: the tensors themselves are turned and returned, without a graph (a new token's q and k)."""
+    ``inplace``: the tensors themselves are turned and returned, without a graph (a new token's q and k); no two of their elements may share a place."""
     xs = (q,) if k is None else (q, k)
     if inplace:
         if k is not None and k.numel() and k.data_ptr() == q.data_ptr():

@@ -117,6 +117,18 @@ def test_rotary_refusals(dev):
         H.rotary_axes(q.detach()[:, :, :1].expand(2, 6, 3, 32), None, pos, plan, inplace=True)
 
 
+def test_rotary_in_place_refuses_overlaps(dev):
+    plan, pos = H.RotaryAxes((4, 6, 6)), torch.zeros(3, 2, 6, dtype=torch.int32, device="cuda")
+    x = torch.zeros(2, 6, 8, 32, dtype=BF, device="cuda")
+    own = torch.zeros(999, dtype=BF, device="cuda").as_strided((2, 6, 3, 32), (300, 32, 32, 1))
+    with torch.no_grad():
+        for q, k in ((x[:, :, :4], x[:, :, 3:]), (x[:, :, 3:], x[:, :, :4]), (own, None)):
+            with pytest.raises(L.HsError, match="overlap"):
+                H.rotary_axes(q, k, pos, plan, inplace=True)
+        H.rotary_axes(x[:, :, 0::2], x[:, :, 1::2], pos, plan, inplace=True)
+        H.rotary_axes(x[:, :, 0::2], x[:, :, 0:0], pos, plan, inplace=True)
+
+
 # ---- differential attention ----------------------------------------------------------------------------------------------------
 def diff_reference(q, k, v, lam, go, scale, causal, start, lens):
     """values and bounds {o, q, k, v, lam: (value, bound)} in 64 bits"""

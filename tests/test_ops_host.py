@@ -325,3 +325,37 @@ def test_adamw_refuses_bad_counts_and_strangers():
     for f in (lambda: opt.set_state(q, **_state(q, 32)), lambda: opt.moments(q)):
         with pytest.raises(L.HsError, match="not a parameter"):
             f()
+
+
+def test_tensors_that_share_memory_are_found():
+    """against the places of all elements, one by one"""
+    import random
+    from hsenet_amd.rotary import _apart, _share_memory
+    def quick(xs):
+        return _apart(*xs[0].shape[:2], xs[0].shape[3], [(x.shape[2], x, O.bnh(x.shape, x.stride()), None, None) for x in xs])
+    rng, room, found, proved = random.Random(5), torch.zeros(4096, dtype=torch.bfloat16), [0, 0], 0
+    def places(x):
+        at = x.storage_offset() + sum(torch.arange(n).view([-1 if i == a else 1 for i in range(4)]) * s for a, (n, s) in enumerate(zip(x.shape, x.stride())))
+        return at.flatten().tolist()
+    def one():
+        shape = [rng.choice([1, 2, 3]), rng.choice([1, 2, 4]), rng.choice([1, 2, 3]), 4]
+        strides = rng.choice([[shape[1] * shape[2] * 4, shape[2] * 4, 4], [96, 24, 8], [96, 24, 4], [48, 12, 4], [rng.choice([8, 60, 100]), rng.choice([4, 12, 50]), rng.choice([2, 4, 6, 16])],
+                              [24, 96, 8], [128, 32, 16]])
+        return room.as_strided(shape, [*strides, 1], rng.choice([0, 4, 8, 12, 16, 24, 3, 200, 400]))
+    for i in range(4000):
+        xs = [one() for _ in range(1 + i % 4 // 2)]
+        if len(xs) == 2:
+            xs[1] = room.as_strided([*xs[0].shape[:2], *xs[1].shape[2:]], xs[1].stride(), xs[1].storage_offset())
+        all_ = sum((places(x) for x in xs), [])
+        want = len(set(all_)) < len(all_)
+        assert _share_memory(xs) == want and not (want and quick(xs)), [(x.shape, x.stride(), x.storage_offset()) for x in xs]
+        found[want] += 1
+        proved += quick(xs)
+    assert min(found) > 500 and proved > 500
+    qkv = torch.zeros(2, 1000, 36, 64)                         # the thirds of a projection, heads of q and k in turn, another tensor
+    for q, k in ((qkv[:, :, :12], qkv[:, :, 12:24]), (qkv[:, :, 0::3], qkv[:, :, 1::3]), (qkv[:1], qkv[1:]), (qkv[:, :, :3], torch.zeros(2, 1000, 3, 64))):
+        assert not _share_memory([q, k]) and (quick([q, k]) or q.stride(2) == 192)
+    for q, k in ((qkv[:, :1, :12], qkv[:, :1, 12:24]), (qkv[:1, :1, :12], qkv[:1, :1, 12:24])):
+        assert quick([q, k]) and quick([k, q])
+    for q, k in ((qkv[:, :, :12], qkv[:, :, 11:24]), (qkv[:, :-1], qkv[:, 1:]), (qkv[..., :40], qkv[..., 24:])):
+        assert _share_memory([q, k])
