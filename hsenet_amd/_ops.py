@@ -8,6 +8,7 @@ import struct
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib as L
 
@@ -110,6 +111,14 @@ def device_of(*tensors) -> int:
         elif i != dev:
             raise L.HsError(f"the tensors of one call lie on different devices (cuda:{dev} and cuda:{i})")
     return dev
+
+
+def refuse_tangents(*tensors) -> None:
+    """HsError for a tensor that carries a tangent (torch.autograd.forward_ad): a kernel would return a value without one, which reads as a derivative of 0"""
+    if getattr(forward_ad, "_current_level", 0) >= 0:
+        for t in tensors:
+            if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+                raise L.HsError("forward-mode derivatives are not supported: call this on the primal, or differentiate backward")
 
 
 _current_device, _raw_stream = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device, None

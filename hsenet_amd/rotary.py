@@ -183,9 +183,10 @@ class RotaryAxesFn(torch.autograd.Function):
 def rotary_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, plan: RotaryAxes, inplace: bool = False):
     """q [B, N, H, dh] and k [B, N, Hkv, dh] (or None) turned by ``positions`` ([axes, N], or [axes, B, N] where the batch entries differ; int32, int64
     or float32) in one launch: (q', k'), or q' where k is None.  bf16, fp16 or fp32; angles are held in 64 bits.  The tensors may be
-    views with their columns side by side (the q and k thirds of one projection); the results are dense.  Differentiable in q and k.
+    views with their columns side by side (the q and k thirds of one projection); the results are dense.  Differentiable in q and k (backward).
     ``inplace``: the tensors themselves are turned and returned, without a graph (a new token's q and k); no two of their elements may share a place."""
     xs = (q,) if k is None else (q, k)
+    O.refuse_tangents(*xs, positions)
     if inplace:
         if k is not None and k.numel() and k.data_ptr() == q.data_ptr():
             raise L.HsError("one tensor cannot be turned in place twice in a call")

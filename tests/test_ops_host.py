@@ -359,3 +359,22 @@ def test_tensors_that_share_memory_are_found():
         assert quick([q, k]) and quick([k, q])
     for q, k in ((qkv[:, :, :12], qkv[:, :, 11:24]), (qkv[:, :-1], qkv[:, 1:]), (qkv[..., :40], qkv[..., 24:])):
         assert _share_memory([q, k])
+
+
+def test_tensors_with_tangents_are_refused():
+    """a result without a tangent would read as a derivative of zero"""
+    from torch.autograd import forward_ad
+    plan, pos = H.RotaryAxes((4, 6, 6), device="cpu"), torch.zeros(3, 2)
+    args = [torch.zeros(1, 2, 4, 32), torch.zeros(1, 2, 4, 32), torch.zeros(1, 2, 2, 64), torch.ones(2)]
+    with forward_ad.dual_level():
+        for i in range(4):
+            dual = [forward_ad.make_dual(t, torch.ones_like(t)) if j == i else t for j, t in enumerate(args)]
+            with pytest.raises(L.HsError, match="forward-mode"):
+                H.diff_attention(*dual)
+        q, k, p = (forward_ad.make_dual(t, torch.ones_like(t)) for t in (args[0], args[1], pos))
+        for call in ((q, None, pos), (args[0], k, pos), (args[0], None, p)):
+            for inplace in (False, True):
+                with pytest.raises(L.HsError, match="forward-mode"):
+                    H.rotary_axes(*call, plan, inplace=inplace)
+        with pytest.raises(L.HsError, match="no CPU fallback"):                  # (without one the call goes on)
+            H.rotary_axes(args[0], None, pos, plan)
