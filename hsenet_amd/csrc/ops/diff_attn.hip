@@ -235,6 +235,7 @@ __device__ __forceinline__ void two_part_weights(f32x16& s, float c2, float m, f
         rest[sp] = pack8<F16>(s, sp);
     }
 }
+__device__ __forceinline__ float exp2_neg(float x) { return __builtin_amdgcn_exp2f(-x); }
 // What the backward pass needs of a row's softmax: P = 2^(c2 s - hi - lo), hi whole (the reference m is), 0 <= lo < 1.  One fp32 number of their sum's
 // size would put a common error of 5e-7 on all of a row's P, which the sum that is lam's gradient would keep.
 __device__ __forceinline__ void put_lse(float* p, long next, float m, float l) {
@@ -949,8 +950,10 @@ __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void d
     constexpr float UP = F16 ? SHIFT16 : 0;
     const long bh = (long)b * a.H + head;
     const float* ls = a.lse + bh * 4 * a.Nq + qrow;
-    const float hi0 = ls[0] - UP, hi1 = ls[a.Nq] - UP;                    // (P comes out times 2^lo: taken off the sums at the end)
+    const float hi0 = ls[0] - UP, hi1 = ls[a.Nq] - UP;                    // (P comes out times 2^lo)
     const float D0 = a.D[bh * 2 * a.Nq + qrow], D1 = a.D[(bh * 2 + 1) * a.Nq + qrow];
+    // bf16: 2^lo is taken off the sums at the end.  fp16: off dP - D, so that dS is packed as 2^4 P (dP - D), as it is for dk
+    const float un0 = exp2_neg(ls[2 * a.Nq]), un1 = exp2_neg(ls[3 * a.Nq]), Du0 = D0 * un0, Du1 = D1 * un1;
     float x2 = 0.f;
     f32x16 dq[2][NQ], s[2], dp;
     clear(dq[0]); clear(dq[1]);
@@ -970,8 +973,8 @@ __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void d
         for (int r = 0; r < 16; ++r) {
             const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][r], a.c2, -hi0));
             const float p2 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[1][r], a.c2, -hi1));
-            s[0][r] = p1 * (dp[r] - D0);
-            s[1][r] = p2 * (dp[r] - D1);
+            s[0][r] = p1 * (F16 ? __builtin_fmaf(dp[r], un0, -Du0) : dp[r] - D0);
+            s[1][r] = p2 * (F16 ? __builtin_fmaf(dp[r], un1, -Du1) : dp[r] - D1);
         }
         bf16x8 ds[2][2];
         pack2maps<F16>(s, ds);
@@ -1019,13 +1022,12 @@ __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void d
         return;
     }
     if (query >= a.Nq) return;
-    const float down = F16 ? 1.0f / (1 << SHIFT16) : 1.0f, mul = a.scale * down;
-    const float un0 = __builtin_amdgcn_exp2f(-ls[2 * a.Nq]), un1 = __builtin_amdgcn_exp2f(-ls[3 * a.Nq]);
+    const float down0 = F16 ? 1.0f / (1 << SHIFT16) : un0, down1 = F16 ? 1.0f / (1 << SHIFT16) : un1;
     // D_2 = sum P2 dP = D_1' + sum P2 (dP - D_1'), whatever D_1' is that stands for it in the row's dS (sum P2 = 1)
-    if (h == 0) a.x2[bh * a.Nq + query] = x2 * down * un1 + D1;
+    if (h == 0) a.x2[bh * a.Nq + query] = x2 * down1 + D1;
     bf16_t* p = a.dq + (((long)b * a.Nq + query) * a.H + head) * 2 * D;
-    store_rows<F16>(p, dq[0], mul * un0, h);
-    store_rows<F16>(p + D, dq[1], -a.lam[head * a.lam_stride] * mul * un1, h);
+    store_rows<F16>(p, dq[0], a.scale * down0, h);
+    store_rows<F16>(p + D, dq[1], -a.lam[head * a.lam_stride] * a.scale * down1, h);
 }
 
 // the sum of dq's parts, in their order: a wave 32 rows by 32 columns of [dq1 | dq2]
@@ -1050,11 +1052,10 @@ __global__ __launch_bounds__(256) void diff_dq_join_kernel(Args a) {
         }
         x2 += ((const float*)a.stats)[(p * tiles + tile) * 32 + c];
     }
-    const float down = F16 ? 1.0f / (1 << SHIFT16) : 1.0f, mul = a.scale * down;
     const float* ls = a.lse + bh * 4 * a.Nq + query;
-    const float un0 = __builtin_amdgcn_exp2f(-ls[2 * a.Nq]), un1 = __builtin_amdgcn_exp2f(-ls[3 * a.Nq]);
-    if (n == 0 && h == 0) a.x2[bh * a.Nq + query] = x2 * down * un1 + a.D[(bh * 2 + 1) * a.Nq + query];
-    store_rows<F16>(a.dq + ((b * a.Nq + query) * a.H + head) * 2 * D + n * 32, x, n < NQ ? mul * un0 : -a.lam[head * a.lam_stride] * mul * un1, h);
+    const float down0 = F16 ? 1.0f / (1 << SHIFT16) : exp2_neg(ls[2 * a.Nq]), down1 = F16 ? 1.0f / (1 << SHIFT16) : exp2_neg(ls[3 * a.Nq]);      // (see there)
+    if (n == 0 && h == 0) a.x2[bh * a.Nq + query] = x2 * down1 + a.D[(bh * 2 + 1) * a.Nq + query];
+    store_rows<F16>(a.dq + ((b * a.Nq + query) * a.H + head) * 2 * D + n * 32, x, n < NQ ? a.scale * down0 : -a.lam[head * a.lam_stride] * a.scale * down1, h);
 }
 
 // dK, dV: keys stay, the queries of every head of the group stream.  With the constants of a row (row_constants)

@@ -121,8 +121,8 @@ def diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch
     query of the entry sees is not used either; a NaN at a key that some see may show in all queries of the entry.
 
     Differentiable in q, k, v and lam (backward), without atomics (equal inputs, equal bits); the maps' own outputs are kept for it.  A few queries against many
-    keys (a token and its cache) are split over the keys.  In fp16 a backward pass holds P (dP - D) times 16: scale the loss so that the gradients
-    of a layer stay in fp16's range."""
+    keys (a token and its cache) are split over the keys.  In fp16 a backward pass holds P (dP - D), for dk with lam in it, times 16: scale the loss
+    so that |P (dP - D)| max(1, |lam|) stays under 4094."""
     O.refuse_tangents(q, k, v, lam)
     if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (q, k, v, lam)):
         return DiffAttnFn.apply(q, k, v, lam, scale, causal, q_start, kv_len)

@@ -67,7 +67,8 @@ size_t hs_diff_attn_bwd_ws_bytes(const hs_diff_attn_desc* desc);
 int hs_diff_attn_fwd(const hs_diff_attn_desc* desc, const void* q, const void* k, const void* v, const float* lam, const int32_t* q_start,
                      const int32_t* kv_len, void* o, void* maps, float* lse, void* ws, size_t ws_bytes, void* stream);
 /* dq, dk, dv: dense, in the layouts of q, k, v; dlam: fp32 [H] (one number with lam_stride 0).  All are written whole.  No atomics: equal
- * inputs give equal bits.  fp16: the products' gradients are held times 2^4, so |P (dP - D)| has to stay under 4094. */
+ * inputs give equal bits.  fp16: the products' gradients are held times 2^4, the second map's for dk with lam in them, so
+ * |P (dP - D)| max(1, |lam|) has to stay under 4094; so has 1 + |lam|, for dv. */
 int hs_diff_attn_bwd(const hs_diff_attn_desc* desc, const void* q, const void* k, const void* v, const float* lam, const int32_t* q_start,
                      const int32_t* kv_len, const void* d_o, const void* maps, const float* lse, void* dq, void* dk, void* dv, float* dlam,
                      void* ws, size_t ws_bytes, void* stream);

@@ -289,6 +289,26 @@ def test_diff_one_visible_key_gives_its_value(dev, d, Nq, B):
     assert torch.equal(o[:, :, 0], (0.5 * v[:, :1, 0]).expand_as(o[:, :, 0])) and torch.equal(o[:, :, 1], v[:, :1, 1].expand_as(o[:, :, 1]))
 
 
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("Nk", [2, 2000])
+@pytest.mark.parametrize("weight,size", [(0.5, 4000.0), (-3.0, 1300.0)])
+def test_diff_fp16_gradients_up_to_their_limit(dev, d, Nk, weight, size):
+    """|P (dP - D)| max(1, |lam|) just under 4094, where two equal scores of -0.04 powers of two make a row's sum 1.94 times its power of two: dq, dk
+    and dlam are as far from their 64-bit values as roundings are, and finite"""
+    B, Nq, Hq = 1, 40, 2
+    q, k = torch.zeros(B, Nq, 2 * Hq, d, dtype=F16, device="cuda"), torch.full((B, Nk, 2 * Hq, d), math.nan, dtype=F16, device="cuda")
+    v, go = torch.full((B, Nk, Hq, 2 * d), math.nan, dtype=F16, device="cuda"), torch.full((B, Nq, Hq, 2 * d), 50.0, dtype=F16, device="cuda")
+    q[..., 0], k[:, :2] = 0.125, 0.0                       # (dk, 40 queries' sum of dS q, is 20000 at most: fp16 ends at 65504)
+    k[:, :2, :, 0] = -0.2216
+    for j, side in enumerate((1.0, -1.0)):
+        k[:, j, :, 1], v[:, j] = side / 16, side * size / (50.0 * d)
+    lam, lens = torch.full((Hq,), weight, device="cuda"), None if Nk == 2 else [2]
+    got = run_diff(q, k, v, lam, go, dict(scale=1.0, kv_len=None if lens is None else torch.tensor(lens, dtype=torch.int32, device="cuda")))
+    for n, (value, bound) in diff_reference(q, k[:, :2], v[:, :2], lam, go, 1.0, False, [0], None).items():
+        within(got[n][:, :2] if n in "kv" else got[n], value, bound, n)
+    assert float(got["q"][..., 0::2, 1].abs().max()) > size / 16
+
+
 def test_diff_gradient_against_differences(dev):
     """<gradient, u> against the difference of two runs' losses along u.  The loss is taken of 64-bit references, so that only the formula is in question."""
     q, k, v, lam, go, kw, ref = diff_case(5, 1, 19, 23, 2, 1, 32, F16, causal=True)
