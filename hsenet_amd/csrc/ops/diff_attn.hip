@@ -56,6 +56,8 @@ __device__ __forceinline__ int key_count(const Args& a, int b) {
 }
 // number of leading keys that query i sees
 __device__ __forceinline__ int visible(const Args& a, int len, int start, int i) { return a.causal ? max(0, min(len, start + i + 1)) : len; }
+// number of leading queries that the causal mask leaves no key: their rows may hold anything (a batch padded on the left)
+__device__ __forceinline__ int blind(const Args& a, int start) { return a.causal ? min(max(0, -start), a.Nq) : 0; }
 
 // ---- a tile: ROWS rows of [two heads of d | VC value columns], sent straight into LDS images ------------------------------------------------------
 // A wave's instruction moves 8 rows of an image, 16 bytes a lane; the image's swizzle is applied to the source.  It is written out because its builtin
@@ -868,7 +870,8 @@ __global__ __launch_bounds__(256) void diff_join_kernel(Args a) {
 
 // ---- backward ----------------------------------------------------------------------------------------------------------------------------------
 // D_m = dO . O_m, 2 d / 8 lanes a row (HBM-bound: three tensors once), and from it the constants of a row that the dk, dv sweep reads, 32 rows together:
-// the scores' offsets of both maps (the second with lam's size in it), -D_1 and sign(lam) (D_2 - D_1); rows behind the last have P = 0.
+// the scores' offsets of both maps (the second with lam's size in it), -D_1 and sign(lam) (D_2 - D_1).  They are counted from the first query that sees a
+// key; rows behind the last have P = 0.
 template <int D, bool F16>
 __global__ __launch_bounds__(256) void diff_rows_kernel(Args a) {
     constexpr int LANES = D / 4;
@@ -877,7 +880,8 @@ __global__ __launch_bounds__(256) void diff_rows_kernel(Args a) {
     const int part = threadIdx.x % LANES;
     if (id >= (long)a.B * qt * 32 * a.H) return;                          // (whole groups of LANES leave)
     const long rows = (long)a.B * a.Nq * a.H;
-    const int head = id % a.H, query = id / a.H % (qt * 32), b = id / a.H / (qt * 32);
+    const int head = id % a.H, place = id / a.H % (qt * 32), b = id / a.H / (qt * 32);
+    const int start = first_pos(a, b), query = place + blind(a, start);
     float d[2] = {0.f, 0.f};
     if (query < a.Nq) {
         const u32x4 g = *(const u32x4*)(a.go + b * a.go_b + query * a.go_n + head * a.go_h + part * 8);
@@ -905,7 +909,7 @@ __global__ __launch_bounds__(256) void diff_rows_kernel(Args a) {
         p[0] = d[0];
         p[a.Nq] = d[1];
     }
-    float* r = a.rc + (bh * qt + (query >> 5)) * 128 + (query & 31);
+    float* r = a.rc + (bh * qt + (place >> 5)) * 128 + (place & 31);
     r[0] = -e[0] / a.c2; r[32] = -e[1] / a.c2; r[64] = -d[0]; r[96] = copysignf(1.0f, lam) * (d[1] - d[0]);
 }
 
@@ -1023,8 +1027,10 @@ __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void d
     }
     if (query >= a.Nq) return;
     const float down0 = F16 ? 1.0f / (1 << SHIFT16) : un0, down1 = F16 ? 1.0f / (1 << SHIFT16) : un1;
+    const bool sees = visible(a, len, start, query) > 0;
+    if (!sees) { clear(dq[0]); clear(dq[1]); }                            // (whatever its q and dO hold)
     // D_2 = sum P2 dP = D_1' + sum P2 (dP - D_1'), whatever D_1' is that stands for it in the row's dS (sum P2 = 1)
-    if (h == 0) a.x2[bh * a.Nq + query] = x2 * down1 + D1;
+    if (h == 0) a.x2[bh * a.Nq + query] = sees ? x2 * down1 + D1 : 0.f;
     bf16_t* p = a.dq + (((long)b * a.Nq + query) * a.H + head) * 2 * D;
     store_rows<F16>(p, dq[0], a.scale * down0, h);
     store_rows<F16>(p + D, dq[1], -a.lam[head * a.lam_stride] * a.scale * down1, h);
@@ -1054,7 +1060,9 @@ __global__ __launch_bounds__(256) void diff_dq_join_kernel(Args a) {
     }
     const float* ls = a.lse + bh * 4 * a.Nq + query;
     const float down0 = F16 ? 1.0f / (1 << SHIFT16) : exp2_neg(ls[2 * a.Nq]), down1 = F16 ? 1.0f / (1 << SHIFT16) : exp2_neg(ls[3 * a.Nq]);      // (see there)
-    if (n == 0 && h == 0) a.x2[bh * a.Nq + query] = x2 * down1 + a.D[(bh * 2 + 1) * a.Nq + query];
+    const bool sees = visible(a, key_count(a, b), first_pos(a, b), query) > 0;
+    if (!sees) clear(x);
+    if (n == 0 && h == 0) a.x2[bh * a.Nq + query] = sees ? x2 * down1 + a.D[(bh * 2 + 1) * a.Nq + query] : 0.f;
     store_rows<F16>(a.dq + ((b * a.Nq + query) * a.H + head) * 2 * D + n * 32, x, n < NQ ? a.scale * down0 : -a.lam[head * a.lam_stride] * a.scale * down1, h);
 }
 
@@ -1115,10 +1123,11 @@ __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void d
     const int kvh = id % a.Hkv;
     id /= a.Hkv;
     const int b = CUT ? id % a.B : id, part = CUT ? id / a.B : 0;
-    const int len = key_count(a, b), start = first_pos(a, b);
+    const int len = key_count(a, b), skip = blind(a, first_pos(a, b)), start = first_pos(a, b) + skip, Nq = a.Nq - skip;
     const int kb = blk * KEYS, k0 = kb + wave * 32, key = k0 + c;
-    // first query that sees the block's first key; the tiles of a head begin at its tile
-    const int t0 = (a.causal ? max(0, kb - start) : 0) / ROWS, qt = (a.Nq + ROWS - 1) / ROWS;
+    // Queries are counted from the first that sees a key: the others' rows are not touched.  First query that sees the block's first key; the tiles of a
+    // head begin at its tile
+    const int t0 = (a.causal ? max(0, kb - start) : 0) / ROWS, qt = (Nq + ROWS - 1) / ROWS;
     // the block's list of tiles, head by head, and its part of it
     const int per = kb < len ? max(0, qt - t0) : 0, all = per * a.G;
     const int j0 = CUT ? (int)((long)all * part / a.parts) : 0, nj = CUT ? (int)((long)all * (part + 1) / a.parts) - j0 : all;
@@ -1138,8 +1147,8 @@ __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void d
     const char* srow = nullptr;                                           // the tile's row constants
     auto head_start = [&]() {
         const int head = kvh * a.G + sg;
-        dma.start(a.q + b * a.q_b + 2 * head * a.q_h, a.go + b * a.go_b + head * a.go_h, st * ROWS, a.Nq);
-        srow = (const char*)(a.rc + (((long)b * a.H + head) * qt + st) * 128) + wave * 256;
+        dma.start(a.q + b * a.q_b + skip * a.q_n + 2 * head * a.q_h, a.go + b * a.go_b + skip * a.go_n + head * a.go_h, st * ROWS, Nq);
+        srow = (const char*)(a.rc + (((long)b * a.H + head) * ((a.Nq + ROWS - 1) / ROWS) + st) * 128) + wave * 256;
     };
     dma.init(wave, lane, a.q, a.q_n, a.q_h, a.go, a.go_n, 0, 0);
     if (!CUT || nj > 0) head_start();

@@ -117,7 +117,8 @@ def diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch
 
     kv_len (int32 [B]): the keys of each entry that count (its first; 0 to Nk); what k and v hold behind them is not used.
     causal: query i of entry b sees the keys j <= q_start[b] + i.  q_start (int32 [B]) is the position of an entry's first query: without it,
-    Nk - Nq (the queries are the last tokens).  A query that sees no key gets zeros, and nothing flows back from it.  What k and v hold at keys that no
+    Nk - Nq (the queries are the last tokens).  A query that sees no key gets zeros, and nothing flows back from it,
+    whatever q and o's gradient hold there.  What k and v hold at keys that no
     query of the entry sees is not used either; a NaN at a key that some see may show in all queries of the entry.
 
     Differentiable in q, k, v and lam (backward), without atomics (equal inputs, equal bits); the maps' own outputs are kept for it.  A few queries against many

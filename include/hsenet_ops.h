@@ -47,7 +47,8 @@ int hs_rotary_axes(const hs_rotary_desc* desc, const void* x0, void* y0, const v
  * head h reads key head h / (H / Hkv).  d is 32, 64 or 128; dtype bf16 or fp16; lam: fp32, lam[h * lam_stride] (0: one for all heads).
  * kv_len (device, or NULL: Nk): the first kv_len[b] keys of batch entry b count, 0 to Nk (values outside are clamped).  causal: query i of
  * entry b sees the keys j <= q_start[b] + i (q_start NULL: q_start0).  A query that sees no key gets zeros, and no gradient comes from it.
- * What lies in k and v behind kv_len[b], or at keys that no query of the entry sees, is never used, whatever it holds.
+ * What lies in k and v behind kv_len[b], or at keys that no query of the entry sees, and in q and d_o at queries that see no key, is never used, whatever
+ * it holds.
  * o: [B][Nq][H][2 d], dense.  For a backward pass: maps: dense [2][B][Nq][H][2 d], the two maps' own outputs; lse: fp32 [B][H][4][Nq].
  * The strides of q, k, v and of d_o (see below) are multiples of 8 elements, their bases 16-byte aligned, a column's stride is 1; tokens and heads
  * lie at most 2^24 elements apart. */

@@ -375,6 +375,31 @@ def test_diff_causal_cache_filled_to_its_queries(dev, B, Nq, Hq, Hkv, d):
     assert not got["k"][gap].any() and not got["v"][gap].any()
 
 
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("B,Nq,Nk,Hq,Hkv,d", [(3, 70, 50, 2, 1, 64), (3, 70, 50, 4, 2, 128), (3, 45, 40, 4, 1, 32), (3, 300, 2100, 2, 2, 64), (3, 300, 2100, 2, 2, 32),
+                                              (3, 300, 2100, 2, 1, 128), (9, 130, 70, 32, 32, 64), (9, 130, 70, 32, 32, 32), (9, 130, 70, 32, 32, 128), (3, 5, 900, 4, 2, 64)])
+def test_diff_what_queries_without_keys_hold(dev, B, Nq, Nk, Hq, Hkv, d, dtype):
+    """a batch padded on the left, and entries without keys: NaN and infinities in q and dO of the queries that see nothing show nowhere"""
+    g = torch.Generator("cuda").manual_seed(Nq + d)
+    q, k, v = rnd(g, B, Nq, 2 * Hq, d, dtype=dtype), rnd(g, B, Nk, 2 * Hkv, d, dtype=dtype), rnd(g, B, Nk, Hkv, 2 * d, dtype=dtype)
+    lam, go = torch.full((Hq,), 0.3, device="cuda"), rnd(g, B, Nq, Hq, 2 * d, dtype=dtype)
+    start = torch.tensor(([-40, -3, 5] * 3)[:B], dtype=torch.int32, device="cuda")
+    lens = torch.tensor(([Nk, Nk - 7, 0] * 3)[:B], dtype=torch.int32, device="cuda")
+    for kw in (dict(causal=True, q_start=start), dict(causal=True, q_start=start, kv_len=lens), dict(kv_len=lens)):
+        blind = torch.zeros(B, Nq, dtype=torch.bool, device="cuda")
+        if kw.get("causal"):
+            blind |= torch.arange(Nq, device="cuda")[None] < -start[:, None]
+        if "kv_len" in kw:
+            blind |= (lens == 0)[:, None]
+        at = blind[..., None, None]
+        want = run_diff(q.masked_fill(at, 0), k, v, lam, go.masked_fill(at, 0), kw)
+        assert all(torch.isfinite(x).all() for x in want.values()) and not want["o"][blind].any() and not want["q"][blind].any()
+        for x, y in ((math.nan, math.nan), (math.inf, -math.inf), (math.nan, 1.0), (1.0, math.inf)):
+            got = run_diff(q.masked_fill(at, x), k, v, lam, go.masked_fill(at, y), kw)
+            for n in want:
+                assert torch.equal(got[n], want[n]), (n, x, y)
+
+
 def test_diff_shared_and_broadcast_weight(dev):
     q, k, v, _, go, kw, _ = diff_case(21, 2, 50, 60, 4, 2, 32, BF)
     lam = torch.tensor(0.7, device="cuda")
