@@ -92,18 +92,6 @@ class AdamW(torch.optim.Optimizer):
         self.state[p] = st
 
     @staticmethod
-    def _fits(st, bits, n, dev) -> bool:
-        """whether a state is of the bits, the size and the device of a parameter of n elements and lies dense: what can be seen without its shape"""
-        m, v, t, (dm, dv) = st["exp_avg"], st["exp_avg_sq"], st["step"], _BYTES[bits]
-        if not (m.dtype is dm and v.dtype is dv and m.numel() == n == v.numel() and m.get_device() == dev == v.get_device() == t.get_device()
-                and t.numel() == 4 and m.is_contiguous() and v.is_contiguous()):
-            return False
-        if bits == 32:
-            return True
-        m, v, n = st["exp_avg_scale"], st["exp_avg_sq_scale"], -(-n // O.ADAMW_BLOCK)
-        return m.numel() == n == v.numel() and m.get_device() == dev == v.get_device()
-
-    @staticmethod
     def _check_state(p, st, bits) -> None:
         if not _dense(p):
             raise L.HsError("a parameter's elements must fill one stretch of memory")
@@ -144,19 +132,27 @@ class AdamW(torch.optim.Optimizer):
         launches, changed = [], []                             # (a step that is refused for one parameter is taken for none)
         for group in self.param_groups:
             numbers, bits = self._check_numbers(group), group["state_bits"]
-            tables, state, key, words, fits = {}, self.state, None, None, self._fits       # (device, type) -> (addresses, gradients)
+            tables, state, key, words, (dm, dv), block = {}, self.state, None, None, _BYTES[bits], O.ADAMW_BLOCK      # (device, type) -> (addresses, gradients)
             for p in group["params"]:
                 g = p.grad
                 if g is None:
                     continue
-                dev, dtype = p.get_device(), p.dtype
+                dev, dtype, n = p.get_device(), p.dtype, p.numel()
                 if dev < 0:
                     raise L.HsError("hsenet_amd kernels need tensors on an MI355X ('cuda') device; there is no CPU fallback")
-                if g.dtype is not dtype or g.get_device() != dev or g.is_sparse:
-                    raise L.HsError("a gradient must be dense, of its parameter's type and on its device")
+                if g.dtype is not dtype or g.get_device() != dev or g.numel() != n:
+                    raise L.HsError("a gradient must be of its parameter's type and size and on its device")
                 st = state.get(p) or self._init_state(p, bits)
-                m, v, n = st["exp_avg"], st["exp_avg_sq"], p.numel()
-                if not (p.is_contiguous() and g.is_contiguous() and fits(st, bits, n, dev)):
+                m, v, t = st["exp_avg"], st["exp_avg_sq"], st["step"]
+                # what can be seen without the state's shapes; where it is not as usual, all is looked at
+                usual = m.dtype is dm and v.dtype is dv and m.numel() == n == v.numel() and t.numel() == 4 \
+                    and m.get_device() == dev == v.get_device() == t.get_device()
+                if usual and bits == 8:
+                    sm, su = st["exp_avg_scale"], st["exp_avg_sq_scale"]
+                    usual = sm.numel() == -(-n // block) == su.numel() and sm.get_device() == dev == su.get_device()
+                if not (usual and p.is_contiguous() and g.is_contiguous() and m.is_contiguous() and v.is_contiguous()):
+                    if g.layout is not torch.strided or g.shape != p.shape:
+                        raise L.HsError("a gradient must be dense and of its parameter's shape")
                     self._check_state(p, st, bits)
                     if g.stride() != p.stride():
                         g = torch.empty_like(p).copy_(g)
@@ -168,11 +164,8 @@ class AdamW(torch.optim.Optimizer):
                         tables[key] = (array("q"), [])
                     words, held = tables[key]
                 held.append(g)                                 # (a gradient that was copied lives until the launch)
-                if bits == 8:
-                    words.extend((p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), st["exp_avg_scale"].data_ptr(),
-                                  st["exp_avg_sq_scale"].data_ptr(), st["step"].data_ptr(), n))
-                else:
-                    words.extend((p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), 0, 0, st["step"].data_ptr(), n))
+                words.extend((p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), sm.data_ptr(), su.data_ptr(), t.data_ptr(), n) if bits == 8 else
+                             (p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), 0, 0, t.data_ptr(), n))
                 changed.append(p)
             launches += [(dev, words, held, O.DTYPE[dtype], bits, numbers) for (dev, dtype), (words, held) in tables.items()]
         for dev, words, _, dtype, bits, numbers in launches:
@@ -193,28 +186,35 @@ class AdamW(torch.optim.Optimizer):
             raise L.HsError("moments go into bf16 or fp32 tensors")
         for group in self.param_groups:
             bits = group["state_bits"]
+            (dm, dv), block = _BYTES[bits], O.ADAMW_BLOCK
             for p in group["params"]:
-                m, v, dev, shape, stride = exp_avg[i], exp_avg_sq[i], p.get_device(), p.shape, p.stride()
+                x, y, dev, shape, n, plain = exp_avg[i], exp_avg_sq[i], p.get_device(), p.shape, p.numel(), p.is_contiguous()
                 i += 1
-                for t in (m, v):
-                    if t.dtype is not dtype or t.get_device() != dev or t.shape != shape or (t.stride() != stride and p.numel() > 1):
-                        raise L.HsError("moments go into tensors of one type, each of its parameter's shape, strides and device")
+                if x.dtype is not dtype or y.dtype is not dtype or x.get_device() != dev or y.get_device() != dev or x.shape != shape or y.shape != shape \
+                        or not (plain and x.is_contiguous() and y.is_contiguous() or n < 2 or x.stride() == p.stride() == y.stride()):
+                    raise L.HsError("moments go into tensors of one type, each of its parameter's shape, strides and device")
                 st = self.state.get(p)
                 if not st:
-                    m.zero_()
-                    v.zero_()
+                    x.zero_()
+                    y.zero_()
                     continue
-                if not (p.is_contiguous() and self._fits(st, bits, p.numel(), dev)):
+                m, v = st["exp_avg"], st["exp_avg_sq"]
+                usual = plain and m.dtype is dm and v.dtype is dv and m.numel() == n == v.numel() and m.get_device() == dev == v.get_device() \
+                    and m.is_contiguous() and v.is_contiguous()
+                if usual and bits == 8:
+                    sm, su = st["exp_avg_scale"], st["exp_avg_sq_scale"]
+                    usual = sm.numel() == -(-n // block) == su.numel() and sm.get_device() == dev == su.get_device()
+                if not usual:
                     self._check_state(p, st, bits)
                 if bits == 32:
-                    m.copy_(st["exp_avg"])
-                    v.copy_(st["exp_avg_sq"])
+                    x.copy_(m)
+                    y.copy_(v)
                 else:
                     words = tables.get(dev)
                     if words is None:
                         words = tables[dev] = array("q")
-                    words.extend((m.data_ptr(), v.data_ptr(), st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr(), st["exp_avg_scale"].data_ptr(),
-                                  st["exp_avg_sq_scale"].data_ptr(), 0, p.numel()))
+                    sm, su = st["exp_avg_scale"], st["exp_avg_sq_scale"]
+                    words.extend((x.data_ptr(), y.data_ptr(), m.data_ptr(), v.data_ptr(), sm.data_ptr(), su.data_ptr(), 0, n))
         for dev, words in tables.items():
             O.call(dev, "hs_adamw_moments", words.buffer_info()[0], len(words) // 8, O.DTYPE[dtype])
 

@@ -194,9 +194,9 @@ def test_adamw_states_that_no_longer_fit_are_not_read(monkeypatch, bits):
     opt.moments(p)
     assert seen == ["hs_adamw_multi"] + ["hs_adamw_moments"] * (bits == 8)
     seen.clear()
-    def refused():
+    def refused(calls=(opt.step, lambda: opt.moments(p))):
         p.grad = torch.zeros_like(p)
-        for f in (opt.step, lambda: opt.moments(p)):
+        for f in calls:
             with pytest.raises(L.HsError):
                 f()
         assert not seen
@@ -212,7 +212,7 @@ def test_adamw_states_that_no_longer_fit_are_not_read(monkeypatch, bits):
     for name in ("exp_avg", "exp_avg_sq", "step", *(("exp_avg_scale", "exp_avg_sq_scale") if bits == 8 else ())):
         held = opt.state[p][name]
         opt.state[p][name] = held.flatten()[:0]
-        refused()
+        refused((opt.step,) if name == "step" else (opt.step, lambda: opt.moments(p)))      # (a count is not read with the moments)
         opt.state[p][name] = held
     opt.step()
     assert seen == ["hs_adamw_multi"]
@@ -228,7 +228,7 @@ def test_adamw_states_on_another_device_are_not_read(monkeypatch):
         held = opt.state[p][name]
         opt.state[p][name] = torch.empty_like(held, device="meta")
         monkeypatch.setattr(torch.Tensor, "get_device", lambda t: 1 if t.is_meta else 0)
-        for f in (opt.step, lambda: opt.moments(p)):
+        for f in (opt.step, *[lambda: opt.moments(p)] * (name != "step")):
             with pytest.raises(L.HsError, match="device"):
                 f()
         opt.state[p][name] = held
@@ -378,3 +378,19 @@ def test_tensors_with_tangents_are_refused():
                     H.rotary_axes(*call, plan, inplace=inplace)
         with pytest.raises(L.HsError, match="no CPU fallback"):                  # (without one the call goes on)
             H.rotary_axes(args[0], None, pos, plan)
+
+
+def test_adamw_gradients_of_another_shape_are_not_read(monkeypatch):
+    """a gradient that was there before p.data was replaced, with a state of the new size"""
+    seen = _launches(monkeypatch)
+    p = torch.nn.Parameter(torch.zeros(6, 4))
+    opt = H.AdamW([p], state_bits=8)
+    for grad, data in ((torch.zeros(6, 4), torch.zeros(600, 400)), (torch.zeros(1, 4), torch.zeros(6, 4)), (torch.zeros(4, 1).t(), torch.zeros(4, 6).t()),
+                       (torch.zeros(6, 4), torch.zeros(6, 4).t())):
+        p.data = torch.zeros(grad.shape)
+        p.grad = grad
+        p.data = data
+        opt.set_state(p, **_state(p, 8))
+        with pytest.raises(L.HsError, match="gradient"):
+            opt.step()
+    assert not seen
