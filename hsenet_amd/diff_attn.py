@@ -28,7 +28,7 @@ def _placed(t):
 
 
 def _prepare(q, k, v, lam, scale, causal, q_start, kv_len):
-    """(device, descriptor's numbers, q, k, v, lam) with the operands where the kernels can read them; HsError for what they cannot take"""
+    """(device, descriptor's numbers and strides, q, k, v, lam) with the operands where the kernels can read them; HsError for what they cannot take"""
     dev = O.device_of(q, k, v, lam, q_start, kv_len)
     qs, ks, vs, dt = q.shape, k.shape, v.shape, q.dtype
     if not len(qs) == len(ks) == len(vs) == 4:
@@ -53,13 +53,13 @@ def _prepare(q, k, v, lam, scale, causal, q_start, kv_len):
         raise L.HsError(f"scale must be positive (below 1e6), got {scale}")
     (q, sq), (k, sk), (v, sv) = _placed(q), _placed(k), _placed(v)
     lam = lam.contiguous()
-    numbers = (O.DIFF_PACK.size, B, Nq, Nk, H, Hkv, d, O.DTYPE[dt], bool(causal), Nk - Nq, int(H > 1 and lam.numel() > 1), scale, *sq, *sk, *sv)
-    return dev, numbers, q, k, v, lam
+    numbers = (O.DIFF_PACK.size, B, Nq, Nk, H, Hkv, d, O.DTYPE[dt], bool(causal), Nk - Nq, int(H > 1 and lam.numel() > 1), scale)
+    return dev, numbers, (*sq, *sk, *sv), q, k, v, lam
 
 
 def _forward(q, k, v, lam, scale, causal, q_start, kv_len, keep):
     """-> (o, and for a backward pass the descriptor's numbers, the operands as they were read, the maps' outputs and statistics)"""
-    dev, numbers, q, k, v, lam = _prepare(q, k, v, lam, scale, causal, q_start, kv_len)
+    dev, numbers, strides, q, k, v, lam = _prepare(q, k, v, lam, scale, causal, q_start, kv_len)
     _, B, Nq, Nk, H, _, d = numbers[:7]
     o = q.new_empty((B, Nq, H, 2 * d))
     maps = q.new_empty((2, B, Nq, H, 2 * d)) if keep else None
@@ -68,7 +68,7 @@ def _forward(q, k, v, lam, scale, causal, q_start, kv_len, keep):
         if Nk == 0:
             o.zero_()
         else:
-            desc = O.DIFF_PACK.pack(*numbers, 0, 0, 0)
+            desc = O.DIFF_PACK.pack(*numbers, *strides, 0, 0, 0)
             n = O.load().hs_diff_attn_fwd_ws_bytes(desc)
             ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
             O.call(dev, "hs_diff_attn_fwd", desc, q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), _ptr(q_start), _ptr(kv_len),
@@ -94,12 +94,14 @@ class DiffAttnFn(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, go):
         q, k, v, lam, q_start, kv_len, maps, lse = ctx.saved_tensors
-        dev = O.device_of(q, go)
-        go, sg = _placed(go)
+        dev = O.device_of(q, k, v, lam, q_start, kv_len, maps, lse, go)
+        # (what comes back may lie otherwise than what was saved: torch.autograd.graph.save_on_cpu returns dense copies)
+        (q, sq), (k, sk), (v, sv), (go, sg) = _placed(q), _placed(k), _placed(v), _placed(go)
+        lam, maps, lse = lam.contiguous(), maps.contiguous(), lse.contiguous()
         dq, dk, dv, dlam = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v, lam))
         if q.numel() == 0 or k.numel() == 0:
             return (*(t.zero_() for t in (dq, dk, dv, dlam)), None, None, None, None)
-        desc = O.DIFF_PACK.pack(*ctx.numbers, *sg)
+        desc = O.DIFF_PACK.pack(*ctx.numbers, *sq, *sk, *sv, *sg)
         n = O.load().hs_diff_attn_bwd_ws_bytes(desc)
         ws = torch.empty(n, dtype=torch.uint8, device=q.device)
         O.call(dev, "hs_diff_attn_bwd", desc, q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), _ptr(q_start), _ptr(kv_len), go.data_ptr(),

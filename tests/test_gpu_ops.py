@@ -400,6 +400,26 @@ def test_diff_what_queries_without_keys_hold(dev, B, Nq, Nk, Hq, Hkv, d, dtype):
                 assert torch.equal(got[n], want[n]), (n, x, y)
 
 
+@pytest.mark.parametrize("d", [32, 64, 128])
+def test_diff_saved_tensors_that_come_back_dense(dev, d):
+    """operands that are views, saved to host memory for the backward pass: the copies that come back have strides of their own"""
+    g = torch.Generator("cuda").manual_seed(d)
+    B, N, Hq = 2, 150, 2
+    proj = rnd(g, B, N, 3 * 2 * Hq * d, dtype=BF).requires_grad_()
+    lam, go = torch.full((Hq,), 0.3, device="cuda", requires_grad=True), rnd(g, B, Hq, N, 2 * d, dtype=BF).transpose(1, 2)
+    lens, start = torch.tensor([N, N - 9], dtype=torch.int32, device="cuda"), torch.tensor([0, -5], dtype=torch.int32, device="cuda")
+    plan, pos = H.RotaryAxes((4, 6, 6)), torch.randint(0, 99, (3, N), generator=g, device="cuda")
+    def grads():
+        q, k, v = proj.chunk(3, -1)
+        q = H.rotary_axes(q.view(B, N, 2 * Hq, d), None, pos.t().contiguous().t(), plan)
+        o = H.diff_attention(q, k.view(B, N, 2 * Hq, d), v.view(B, N, Hq, 2 * d), lam, causal=True, q_start=start, kv_len=lens)
+        return lambda: (o, *torch.autograd.grad(o, (proj, lam), go))
+    want = grads()()
+    with torch.autograd.graph.save_on_cpu():
+        later = grads()
+    assert all(torch.equal(a, b) for a, b in zip(want, later()))
+
+
 def test_diff_shared_and_broadcast_weight(dev):
     q, k, v, _, go, kw, _ = diff_case(21, 2, 50, 60, 4, 2, 32, BF)
     lam = torch.tensor(0.7, device="cuda")
