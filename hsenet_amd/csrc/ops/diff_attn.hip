@@ -1329,7 +1329,7 @@ __global__ __launch_bounds__(1024) void diff_dlam_kernel(Args a, float* dlam) {
 int check(const hs_diff_attn_desc* d, bool backward) {
     if (!d || d->struct_size != sizeof(hs_diff_attn_desc)) return HS_ERR_ARG;
     if (d->dtype != HS_PREC_BF16 && d->dtype != HS_PREC_F16) return HS_ERR_ARG;
-    if (!(d->scale > 0.f) || !(d->scale < 1e6f) || d->lam_stride < 0) return HS_ERR_ARG;
+    if (!(d->scale > 1e-30f) || !(d->scale < 1e6f) || d->lam_stride < 0) return HS_ERR_ARG;      // (diff_rows_kernel divides by it)
     if (d->B < 1 || d->Nq < 1 || d->Nk < 1 || d->H < 1 || d->Hkv < 1 || d->H % d->Hkv) return HS_ERR_SHAPE;
     if (d->d != 32 && d->d != 64 && d->d != 128) return HS_ERR_SHAPE;
     if (d->Nq > (1 << 28) || d->Nk > (1 << 28) || d->H > (1 << 16)) return HS_ERR_SHAPE;

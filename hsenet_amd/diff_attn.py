@@ -49,8 +49,8 @@ def _prepare(q, k, v, lam, scale, causal, q_start, kv_len):
     _per_entry(q_start, "q_start", B)
     _per_entry(kv_len, "kv_len", B)
     scale = d ** -0.5 if scale is None else float(scale)
-    if not 0 < scale < 1e6:
-        raise L.HsError(f"scale must be positive (below 1e6), got {scale}")
+    if not 1e-30 < scale < 1e6:
+        raise L.HsError(f"scale must be positive (between 1e-30 and 1e6), got {scale}")
     (q, sq), (k, sk), (v, sv) = _placed(q), _placed(k), _placed(v)
     lam = lam.contiguous()
     numbers = (O.DIFF_PACK.size, B, Nq, Nk, H, Hkv, d, O.DTYPE[dt], bool(causal), Nk - Nq, int(H > 1 and lam.numel() > 1), scale)

@@ -44,7 +44,7 @@ int hs_rotary_axes(const hs_rotary_desc* desc, const void* x0, void* y0, const v
 
 /* ---- differential attention: o = softmax(scale q1 k1^T) v - lam[h] softmax(scale q2 k2^T) v.
  * q: [B][Nq][2 H][d], heads 2h and 2h + 1 are the two queries of head h; k: [B][Nk][2 Hkv][d] likewise; v: [B][Nk][Hkv][2 d];
- * head h reads key head h / (H / Hkv).  d is 32, 64 or 128; dtype bf16 or fp16; lam: fp32, lam[h * lam_stride] (0: one for all heads).
+ * head h reads key head h / (H / Hkv).  d is 32, 64 or 128; scale between 1e-30 and 1e6; dtype bf16 or fp16; lam: fp32, lam[h * lam_stride] (0: one for all heads).
  * kv_len (device, or NULL: Nk): the first kv_len[b] keys of batch entry b count, 0 to Nk (values outside are clamped).  causal: query i of
  * entry b sees the keys j <= q_start[b] + i (q_start NULL: q_start0).  A query that sees no key gets zeros, and no gradient comes from it.
  * What lies in k and v behind kv_len[b], or at keys that no query of the entry sees, and in q and d_o at queries that see no key, is never used, whatever

@@ -394,3 +394,12 @@ def test_adamw_gradients_of_another_shape_are_not_read(monkeypatch):
         with pytest.raises(L.HsError, match="gradient"):
             opt.step()
     assert not seen
+
+
+@no_gpu_only
+@pytest.mark.parametrize("scale", [1e-38, 1e-31, 1e6, float("inf")])
+def test_diff_attention_refuses_scales_out_of_range(scale):
+    """the backward pass divides a row's statistics by the scale: of 1e-38 they would be infinite, and dv zero"""
+    lib, bad = O.load(), _diff(scale=scale)
+    assert lib.hs_diff_attn_fwd(C.byref(bad), P, P, P, P, None, None, P, None, None, P, 1 << 40, None) == L.HS_ERR_ARG
+    assert lib.hs_diff_attn_bwd(C.byref(bad), P, P, P, P, None, None, P, P, P, P, P, P, P, P, 1 << 40, None) == L.HS_ERR_ARG
