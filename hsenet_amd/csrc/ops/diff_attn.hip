@@ -8,8 +8,11 @@
 // with D_m = sum over keys of P_m dP = dO . O_m (O_m: the map's own output, kept by the forward pass).  dP is one product for both maps, and dV too.
 // Tiles of 32 rows are staged in LDS images R (common.h: 128-byte rows, read by rows and by columns): d / 32 images of a head pair's two keys
 // (queries) side by side and d / 32 of its values (dO).
-// P and dS are rounded to the operands' 16 bits for the matrix products, as every softmax weight that goes through them has to be: with o's own rounding that
-// leaves bf16 outputs 2.5e-3 off (o's rounding alone: 1.7e-3), fp16 3.2e-4.  Scores, sums, D and all accumulators are fp32.
+// P and dS are rounded to the operands' 16 bits for the matrix products.  That is a choice for speed: P in two numbers of 16 bits, as the split forward takes it
+// where bandwidth leaves the matrix pipe room, would make 32 of the whole forward's 40 matrix instructions a step (d = 64) products with V, instead of 16
+// of 24.  With o's own rounding it leaves bf16 outputs of normally distributed inputs 2.5e-3 off (o's rounding alone: 1.7e-3), fp16 3.2e-4; P's error is relative
+// to each map, so that it grows beside o where the maps cancel.  The maps' outputs are kept in 16 bits, and D is summed from them.  Scores, sums, statistics,
+// D and all accumulators are fp32.
 #include "../common.h"
 #include "../attn_util.h"
 #include <type_traits>
@@ -365,8 +368,8 @@ template <int D> struct Sweep {
 
 // ---- forward ----------------------------------------------------------------------------------------------------------------------------------
 // 12 d operations a visible pair and head, both maps' products with V apart.  Bound: the matrix and vector instructions together (53 and 42 % of a SIMD's
-// cycles, at a clock that the power cap holds at 2.2 GHz).  16 heads of 64 on 4, 8192 causal tokens: 355 us, 1.16 PFLOP/s.  2 x 4097 tokens of 6 heads: 168 us,
-// 183 with the maps kept; its 204 blocks leave 52 of the 256 CUs idle.
+// cycles, at a clock that the power cap holds at 2.2 GHz).  16 heads of 64 on 4, 8192 causal tokens: 364 us, 1.14 PFLOP/s.  2 x 4097 tokens of 6 heads: 168 us,
+// 183 with the maps kept: 204 blocks on 256 CUs, and 12 of these hold one row each, at the time of a full one.
 // CUT: a block takes one of a.cuts parts of its keys, and diff_fwd_join_kernel puts them together.
 template <int D, bool F16, bool KEEP, bool CUT>
 __global__ __launch_bounds__(Sweep<D>::NW * 64, Sweep<D>::PAIRED ? 2 : 1) void diff_fwd_kernel(Args a) {
@@ -1351,8 +1354,10 @@ bool misaligned(const void* p, unsigned n = 16) { return !p || (uintptr_t)p % n;
 
 struct Split { int tiles, nsplit, chunk; };
 constexpr int SPARSE = 128, WANT = 1024, LEAST = 512;       // blocks (two rounds even out ragged entries: 70 us against 78 with one); keys of a chunk (4 tiles a wave)
-// Parts that a sweep is cut into.  A round of blocks (one a CU) takes about a microsecond a tile of 32 rows; cutting costs each block another start, a second
-// kernel, and `traffic` tiles' time for a part's sums of a block written and read.  Whole / cut in us: forward, 4096 tokens of 4 heads of 64 136 / 74, causal
+// Parts that a sweep is cut into.  A round of blocks (one a CU) takes `tiles` microseconds; cutting costs each block another start, a second kernel, and
+// `traffic` of a microsecond for a part's sums of a block written and read.  The forward pass gives the time that it measured (whole_of).  The backward sweeps
+// are taken at one microsecond a tile of 32 rows at every width, less than they measure (full rounds: dq 1.4 at d = 64 and 1.8 at 128, dk, dv 2.1 and 2.8), so that
+// they are cut later than would pay.  Whole / cut in us: forward, 4096 tokens of 4 heads of 64 136 / 74, causal
 // 137 / 64; 2048 causal tokens of 8 heads 72 / 46; 512 queries of 16 heads on 8192 keys 135 / 75; the backward pass with dq cut, the same four but the last:
 // 253 / 172, 242 / 159, 145 / 107.
 struct Cuts { int parts; double time; };

@@ -25,7 +25,7 @@ const char* hs_ops_build_id(void);
  * (the gradient of the turn).  Columns behind 2 * pairs are copied.  One or two tensors [B][N][heads[i]][dh] (q and k: heads[1] = 0
  * for one) in one launch, each with strides of its own; a column's stride is 1.  y may be x (in place, equal strides); apart from that
  * they do not overlap.  positions: int32, int64 or float32 [axes][B][N] (strides of 0 broadcast).  freq: double [pairs], axis: int32
- * [pairs], entries in [0, axes) (device). */
+ * [pairs], entries in [0, axes) (device).  dh is at most 4096, heads[0] + heads[1] at most 4096, their product at most 2^18. */
 #define HS_POS_I32 0
 #define HS_POS_I64 1
 #define HS_POS_F32 2
