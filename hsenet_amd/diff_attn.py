@@ -123,11 +123,12 @@ def diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch
     o's gradient hold there.  What k and v hold at keys that no query of the entry sees is not used either; a NaN at a key that some see may show in all
     queries of the entry.
 
-    Scores, sums and outputs are made in fp32; the softmax weights go through the products with v in 16 bits, an error relative to each map that shows beside o where
-    the maps cancel.  A few queries against many keys (a token and its cache) are split over the keys, and there the weights keep 32: the same operands may
-    differ by that rounding between the two, which a rule on the sizes chooses.
-    Differentiable in q, k, v and lam (backward), without atomics (equal inputs, equal bits); the maps' own outputs are kept for it.  In fp16 a backward pass holds P (dP - D), for dk with lam in it, times 16: scale the loss
-    so that |P (dP - D)| max(1, |lam|) stays under 4094."""
+    Scores, sums and outputs are made in fp32; the softmax weights go through the products with v in 16 bits, an error relative to each map that shows
+    beside o where the maps cancel.  A few queries against many keys (a token and its cache) are split over the keys, and there the weights go through in
+    two numbers of 16 bits: the same operands may differ by that rounding between the two, which a rule on the sizes chooses.
+
+    Differentiable in q, k, v and lam (backward), without atomics (equal inputs, equal bits); the maps' own outputs are kept for it.  In fp16 a backward
+    pass holds P (dP - D), for dk with lam in it, times 16: scale the loss so that |P (dP - D)| max(1, |lam|) stays under 4094."""
     O.refuse_tangents(q, k, v, lam)
     if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (q, k, v, lam)):
         return DiffAttnFn.apply(q, k, v, lam, scale, causal, q_start, kv_len)
